@@ -27,7 +27,7 @@
 extern "C" {
 #endif
 
-#define NSA_ABI_VERSION 4
+#define NSA_ABI_VERSION 5
 
 typedef enum nsa_status {
   NSA_OK = 0,
@@ -419,6 +419,127 @@ nsa_status nsa_glu(const nsa_glu_desc* desc, const float* X, void* Y, void* stre
 nsa_status nsa_glu_interleave(const void* src, void* dst, int32_t I, int64_t row_bytes, void* stream);
 
 /* ------------------------------------------------------------------------------------------------
+ * Decode steps: the layer's linears, the cache of keys and values and the attention over it for a few new
+ * tokens per sequence, with weights and cache held in 4 bits.  No counterpart in the reference, whose text
+ * encoder runs whole prompts only (app/models/gemma3.js:49-96); the layer computed is the same.
+ *
+ * The 4-bit format.  A group of consecutive values has one scale s, the smallest number with five
+ * significant bits that is >= (largest magnitude of the group) / 7, and codes c = round(x / s), ties to
+ * even, -7 <= c <= 7, stored as c + 8.  s * c is a bf16 number exactly.  Groups whose largest magnitude is
+ * below 2^-110 are stored as zeros, magnitudes above 2^120 saturate, and a group with an infinity or a NaN
+ * reads back as NaN.
+ *
+ * Weights [N][K] in groups of 32, 64 or 128 along K.  Rows are padded to 16 (Nt tiles) and K to 128 (Kc
+ * chunks) with zeros:
+ *   codes  uint8 [Nt][Kc][16][64]: of the 128 values of a row's chunk, the 32-bit word at byte 16 c + 4 i
+ *          holds values 32 i + 8 c + e, e = 0..7, in nibble e / 2 (e even) or 4 + (e - 1) / 2 (e odd);
+ *   scales bf16 [Nt][Kc][16][128 / group].  nsa_linear4 takes any finite scales, not only five-bit ones.
+ *
+ * nsa_quantize4 makes codes and scales from W fp32 or bf16 (any K).  nsa_expand4 writes the bf16 values
+ * (exact for the quantiser's scales, rounded to nearest for others): the weight nsa_linear takes when a
+ * prompt brings many rows.
+ * ------------------------------------------------------------------------------------------------ */
+typedef struct nsa_weight4 {
+  int32_t N, K;
+  int32_t group;         /* 32, 64 or 128 */
+  uint8_t* codes;        /* 16-byte aligned */
+  void* scales;          /* bf16, 16-byte aligned */
+} nsa_weight4;
+/* Bytes of codes and scales for N, K and group (NULL outputs are skipped). */
+nsa_status nsa_weight4_sizes(int32_t N, int32_t K, int32_t group, size_t* codes_bytes, size_t* scales_bytes);
+/* W [N][ldw] (0: K), fp32 or bf16 by dtype, at its element alignment. */
+nsa_status nsa_quantize4(const nsa_weight4* w, const void* W, int32_t dtype, int64_t ldw, void* stream);
+/* out bf16 [N][ldo] (0: K). */
+nsa_status nsa_expand4(const nsa_weight4* w, void* out, int64_t ldo, void* stream);
+
+/* nsa_linear4: ops.linear (app/gpu/ops.js:50-66) with a 4-bit weight, for decode steps:
+ *   C[m*ldc + n] = r, or += r with resid, where r = sum_k A[m][k] W[n][k] (+ bias[n]).
+ * A bf16 [M][lda]; K and lda multiples of 8, A 16-byte aligned; C fp32 or (store form) bf16, at its
+ * element alignment; C must not overlap A.  The products are exact and sums are kept in fp32, so the result
+ * is the fp32 linear's.  Any M runs; the weights are read once per 32 rows of A, so from a few hundred rows
+ * on nsa_linear over the nsa_expand4 copy is faster. */
+typedef struct nsa_linear4_desc {
+  int32_t M;
+  int64_t lda;           /* A row pitch in elements (0: K) */
+  int64_t ldc;           /* C row pitch in elements (0: N) */
+  int32_t resid;         /* 1: accumulate into C (fp32 only) */
+  int32_t out_dtype;     /* NSA_F32 or NSA_BF16 */
+} nsa_linear4_desc;
+nsa_status nsa_linear4(const nsa_linear4_desc* desc, const nsa_weight4* w, const void* A, const float* bias,
+                       void* C, void* stream);
+
+/* The cache: a pool of pages of P tokens for Hkv key/value heads of D values, in groups of 32 along D:
+ *   codes  uint8 [n_pages][2][Hkv][P][D / 2] (keys, then values; value 2 j in the low nibble of byte j),
+ *   scales bf16 [n_pages][2][Hkv][P][D / 32].
+ * D 64, 128 or 256; P a multiple of 16, at most 1024; both 16-byte aligned.  A slot that was never written
+ * is never read. */
+typedef struct nsa_kv4_cache {
+  int32_t n_pages, P, Hkv, D;
+  uint8_t* codes;
+  void* scales;
+} nsa_kv4_cache;
+/* One step: B sequences with up to L new tokens each.  New token i of sequence b has position start[b] + i
+ * and lives in slot position % P of page table[b*table_ld + position / P]; start[b] is the number of tokens
+ * stored before the step.  count (optional): new tokens of each sequence, clamped to [0, L]; rows past them
+ * are neither read nor written.  table, start and count are device int32 arrays, read when the kernels run.
+ * Pages may be shared between sequences for reading; no slot may be written twice in one call.
+ * A position outside the table, or past the RoPE table, and a page id outside the pool are skipped and
+ * recorded: nsa_check_device then returns NSA_ERR_DEVICE.  Skipped tokens are not written; as keys they are
+ * masked. */
+typedef struct nsa_kv4_batch {
+  int32_t B, L;
+  int32_t max_pages;     /* page table columns; max_pages * P <= 2^31 - 1 */
+  int64_t table_ld;      /* page table row pitch in elements (0: max_pages) */
+  const int32_t* table;
+  const int32_t* start;
+  const int32_t* count;  /* or NULL */
+} nsa_kv4_batch;
+
+/* nsa_kv4_append: the step's q | k | v rows, element (b, i, col) at qkv[b*bstride + i*ld + col], q heads at
+ * qOff + h*D, k at kOff, v at vOff.  Per head, q and k get the RMSNorm and the split-half RoPE of
+ * ops.headNorm (app/gpu/ops.js:131-138) in the same pass, at RoPE row position; q' is written as bf16 to
+ * q_out[b*qo_bstride + i*qo_ld + h*D], k' and v are quantised into the cache.  Keys are computed in fp64, so
+ * which code a value on the border of two gets does not depend on an order of sums.  cs NULL: no rotation.
+ * qkv fp32 or bf16; its base 16-byte aligned, ld, bstride and offsets multiples of 4 elements. */
+typedef struct nsa_kv4_append_desc {
+  int32_t Hq;            /* a multiple of Hkv */
+  int32_t in_dtype;      /* nsa_dtype of qkv */
+  int64_t ld, bstride;   /* qkv pitches */
+  int64_t qOff, kOff, vOff;
+  int64_t qo_ld, qo_bstride;   /* q_out pitches */
+  int64_t sinOff;        /* offset of the sin block in cs */
+  int32_t rope_rows;     /* rows of cs */
+  float eps;
+} nsa_kv4_append_desc;
+nsa_status nsa_kv4_append(const nsa_kv4_append_desc* desc, const nsa_kv4_cache* cache, const nsa_kv4_batch* batch,
+                          const void* qkv, const float* q_norm_w, const float* k_norm_w, const float* cs,
+                          void* q_out, void* stream);
+/* nsa_kv4_read: positions start[b] .. of the cache back as bf16 rows k | v, the packed layout of
+ * nsa_seq_shard_*: out[b*bstride + i*ldo + h*D] keys, + Hkv*D values.  out 16-byte aligned, ldo and bstride
+ * multiples of 8.  Rows past count[b], and rows skipped for their page or position, are left as they were. */
+nsa_status nsa_kv4_read(const nsa_kv4_cache* cache, const nsa_kv4_batch* batch, void* out, int64_t ldo,
+                        int64_t bstride, void* stream);
+/* nsa_kv4_attention: ops.attention (app/gpu/ops.js:194-242) of the step's queries over the cache, which
+ * holds the new tokens already.  The query at position p sees keys j <= p; with window > 0, only those with
+ * j > p - window (nsa_attention's window) or j < sinks.  q and out bf16, head h of row (b, i) at
+ * b*bstride + i*ld + h*D; bases 16-byte aligned, pitches multiples of 8.  out must not overlap q.  A query
+ * with no key left (its pages or position invalid) writes zeros. */
+typedef struct nsa_kv4_attention_desc {
+  int32_t Hq;            /* a multiple of Hkv; query heads h*Hq/Hkv .. share key/value head h */
+  int64_t q_ld, q_bstride;
+  int64_t o_ld, o_bstride;
+  int32_t window, sinks; /* 0: none; sinks needs a window */
+  float scale;           /* 0: 1 / sqrt(D) */
+} nsa_kv4_attention_desc;
+/* The workspace needs no initialisation and keeps nothing between calls; calls that overlap on the GPU
+ * need one each. */
+size_t nsa_kv4_attention_workspace_size(const nsa_kv4_attention_desc* desc, const nsa_kv4_cache* cache,
+                                        const nsa_kv4_batch* batch);
+nsa_status nsa_kv4_attention(const nsa_kv4_attention_desc* desc, const nsa_kv4_cache* cache,
+                             const nsa_kv4_batch* batch, const void* q, void* out, void* workspace,
+                             size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
  * RoPE tables in the reference layout: cos block [L][D/2] then sin block [L][D/2] (sinOff = L*D/2).
  *   nsa_rope2d_table: app/models/common.js:28-43 (tools/reference.py:220-227): L = h*w tokens,
  *     the first D/4 pairs rotate by the centred column, the next D/4 by the centred row, theta 1e4.
@@ -431,7 +552,8 @@ nsa_status nsa_rope1d_table(int32_t L, int32_t D, float theta, float* out, void*
 /* ------------------------------------------------------------------------------------------------
  * Device-side failure surfacing (app/gpu/device.js:224-231 turns async validation errors into a
  * throw at the next read/sync).  Synchronises `stream`, reads and clears the device error word of
- * the current device: NSA_ERR_DEVICE if any kernel gave up a bounded wait since the last check.
+ * the current device: NSA_ERR_DEVICE if any kernel gave up a bounded wait, or skipped a cache token for its
+ * page or position, since the last check.
  * ------------------------------------------------------------------------------------------------ */
 nsa_status nsa_check_device(void* stream);
 

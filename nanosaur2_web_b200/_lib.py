@@ -98,6 +98,40 @@ class GluDesc(ctypes.Structure):
     _fields_ = [("rows", _i32), ("I", _i32), ("ldx", _i64), ("ldy", _i64), ("act", _i32), ("out_dtype", _i32)]
 
 
+class Weight4Desc(ctypes.Structure):
+    """nsa_weight4 (include/nsattn.h)."""
+    _fields_ = [("N", _i32), ("K", _i32), ("group", _i32), ("codes", _vp), ("scales", _vp)]
+
+
+class Linear4Desc(ctypes.Structure):
+    """nsa_linear4_desc (include/nsattn.h)."""
+    _fields_ = [("M", _i32), ("lda", _i64), ("ldc", _i64), ("resid", _i32), ("out_dtype", _i32)]
+
+
+class Kv4CacheDesc(ctypes.Structure):
+    """nsa_kv4_cache (include/nsattn.h)."""
+    _fields_ = [("n_pages", _i32), ("P", _i32), ("Hkv", _i32), ("D", _i32), ("codes", _vp), ("scales", _vp)]
+
+
+class Kv4Batch(ctypes.Structure):
+    """nsa_kv4_batch (include/nsattn.h)."""
+    _fields_ = [("B", _i32), ("L", _i32), ("max_pages", _i32), ("table_ld", _i64), ("table", _vp), ("start", _vp),
+                ("count", _vp)]
+
+
+class Kv4AppendDesc(ctypes.Structure):
+    """nsa_kv4_append_desc (include/nsattn.h)."""
+    _fields_ = [("Hq", _i32), ("in_dtype", _i32), ("ld", _i64), ("bstride", _i64), ("qOff", _i64), ("kOff", _i64),
+                ("vOff", _i64), ("qo_ld", _i64), ("qo_bstride", _i64), ("sinOff", _i64), ("rope_rows", _i32),
+                ("eps", _f32)]
+
+
+class Kv4AttentionDesc(ctypes.Structure):
+    """nsa_kv4_attention_desc (include/nsattn.h)."""
+    _fields_ = [("Hq", _i32), ("q_ld", _i64), ("q_bstride", _i64), ("o_ld", _i64), ("o_bstride", _i64),
+                ("window", _i32), ("sinks", _i32), ("scale", _f32)]
+
+
 class KernelStat(ctypes.Structure):
     _fields_ = [("name", ctypes.c_char * 32), ("launches", _i64), ("total_ms", ctypes.c_double),
                 ("flops", ctypes.c_double), ("bytes", ctypes.c_double)]
@@ -136,6 +170,17 @@ SIGNATURES = {
     "nsa_rmsnorm": (_i32, [ctypes.POINTER(RmsnormDesc), _vp, _vp, _vp, _vp]),
     "nsa_glu": (_i32, [ctypes.POINTER(GluDesc), _vp, _vp, _vp]),
     "nsa_glu_interleave": (_i32, [_vp, _vp, _i32, _i64, _vp]),
+    "nsa_weight4_sizes": (_i32, [_i32, _i32, _i32, ctypes.POINTER(_sz), ctypes.POINTER(_sz)]),
+    "nsa_quantize4": (_i32, [ctypes.POINTER(Weight4Desc), _vp, _i32, _i64, _vp]),
+    "nsa_expand4": (_i32, [ctypes.POINTER(Weight4Desc), _vp, _i64, _vp]),
+    "nsa_linear4": (_i32, [ctypes.POINTER(Linear4Desc), ctypes.POINTER(Weight4Desc), _vp, _vp, _vp, _vp]),
+    "nsa_kv4_append": (_i32, [ctypes.POINTER(Kv4AppendDesc), ctypes.POINTER(Kv4CacheDesc), ctypes.POINTER(Kv4Batch),
+                              _vp, _vp, _vp, _vp, _vp, _vp]),
+    "nsa_kv4_read": (_i32, [ctypes.POINTER(Kv4CacheDesc), ctypes.POINTER(Kv4Batch), _vp, _i64, _i64, _vp]),
+    "nsa_kv4_attention_workspace_size": (_sz, [ctypes.POINTER(Kv4AttentionDesc), ctypes.POINTER(Kv4CacheDesc),
+                                               ctypes.POINTER(Kv4Batch)]),
+    "nsa_kv4_attention": (_i32, [ctypes.POINTER(Kv4AttentionDesc), ctypes.POINTER(Kv4CacheDesc),
+                                 ctypes.POINTER(Kv4Batch), _vp, _vp, _vp, _sz, _vp]),
     "nsa_rope2d_table": (_i32, [_i32, _i32, _i32, _vp, _vp]),
     "nsa_rope1d_table": (_i32, [_i32, _i32, _f32, _vp, _vp]),
     "nsa_check_device": (_i32, [_vp]),

@@ -755,8 +755,11 @@ nsa_status nsa_check_device(void* stream) {
   if (e == cudaSuccess) e = cudaStreamSynchronize(s);
   if (e != cudaSuccess) return cuda_fail(e, "device check");
   if (host != 0) {
-    char buf[96];
-    std::snprintf(buf, sizeof buf, "device-side error 0x%x (a bounded wait expired)", host);
+    const char* what = host == nsa::kErrKvPage       ? "a page table entry outside the cache's pool"
+                       : host == nsa::kErrKvPosition ? "a token position outside the page table or the RoPE table"
+                                                     : "a bounded wait expired";
+    char buf[128];
+    std::snprintf(buf, sizeof buf, "device-side error 0x%x (%s)", host, what);
     return fail(NSA_ERR_DEVICE, buf);
   }
   return NSA_OK;
@@ -1553,6 +1556,310 @@ nsa_status nsa_seq_shard_attention(const nsa_fused_desc* d, const nsa_seq_shard*
                            [&] { return nsa::launch_attention(ap, pl.D, tq, tkv, tkv, tkv, strm); },
                            attn_pairs(pl, sp.a), kv_len ? kv_len + pl.b0 : nullptr);
   if (e != cudaSuccess) return cuda_fail(e, "attention launch");
+  return NSA_OK;
+}
+
+// ------------------------------------------------------------------------------------ decode steps in 4 bits
+
+nsa_status nsa_weight4_sizes(int32_t N, int32_t K, int32_t group, size_t* codes_bytes, size_t* scales_bytes) {
+  if (N < 1 || K < 1) return fail(NSA_ERR_INVALID_ARGUMENT, "need N >= 1 and K >= 1");
+  if (group != 32 && group != 64 && group != 128) return fail(NSA_ERR_INVALID_ARGUMENT, "group must be 32, 64 or 128");
+  const size_t rows = ((size_t)N + 15) / 16 * 16, chunks = ((size_t)K + 127) / 128;
+  if (codes_bytes) *codes_bytes = rows * chunks * 64;
+  if (scales_bytes) *scales_bytes = rows * chunks * (size_t)(128 / group) * 2;
+  return NSA_OK;
+}
+
+static nsa_status check_weight4(const nsa_weight4* w) {
+  if (!w) return fail(NSA_ERR_INVALID_ARGUMENT, "the weight is NULL");
+  const nsa_status st = nsa_weight4_sizes(w->N, w->K, w->group, nullptr, nullptr);
+  if (st != NSA_OK) return st;
+  if (w->N > 0x7FFFFFFF - 15 || w->K > 0x7FFFFFFF - 127) return fail(NSA_ERR_INVALID_ARGUMENT, "N or K too large");
+  if (!w->codes || !w->scales || !aligned16(w->codes) || !aligned16(w->scales))
+    return fail(NSA_ERR_INVALID_ARGUMENT, "codes and scales must be 16-byte aligned device pointers");
+  return NSA_OK;
+}
+
+static nsa::Quant4Params quant4_params(const nsa_weight4* w) {
+  nsa::Quant4Params p{};
+  p.N = w->N;
+  p.K = w->K;
+  p.G = w->group;
+  p.Nt = (w->N + 15) / 16;
+  p.Kc = (w->K + 127) / 128;
+  p.codes = w->codes;
+  p.scales = static_cast<__nv_bfloat16*>(w->scales);
+  return p;
+}
+
+nsa_status nsa_quantize4(const nsa_weight4* w, const void* W, int32_t dtype, int64_t ldw, void* stream) {
+  const nsa_status st = check_weight4(w);
+  if (st != NSA_OK) return st;
+  if (!W) return fail(NSA_ERR_INVALID_ARGUMENT, "W must be a device pointer");
+  if (dtype != NSA_F32 && dtype != NSA_BF16) return fail(NSA_ERR_INVALID_ARGUMENT, "bad dtype");
+  if (reinterpret_cast<uintptr_t>(W) & (dtype == NSA_F32 ? 3 : 1))
+    return fail(NSA_ERR_INVALID_ARGUMENT, "W must be aligned to its elements");
+  if (ldw && ldw < w->K) return fail(NSA_ERR_INVALID_ARGUMENT, "ldw must be >= K");
+  nsa::Quant4Params p = quant4_params(w);
+  p.w = W;
+  p.ldw = ldw ? ldw : w->K;
+  p.in_f32 = dtype == NSA_F32;
+  const cudaStream_t strm = static_cast<cudaStream_t>(stream);
+  const double bytes = (double)w->N * w->K * ((p.in_f32 ? 4.0 : 2.0) + 0.5 + 2.0 / w->group);
+  cudaError_t e = profiled("quantize4", 0.0, bytes, strm, [&] { return nsa::launch_quantize4(p, strm); });
+  if (e != cudaSuccess) return cuda_fail(e, "quantize4 launch");
+  return NSA_OK;
+}
+
+nsa_status nsa_expand4(const nsa_weight4* w, void* out, int64_t ldo, void* stream) {
+  const nsa_status st = check_weight4(w);
+  if (st != NSA_OK) return st;
+  if (!out || (reinterpret_cast<uintptr_t>(out) & 1)) return fail(NSA_ERR_INVALID_ARGUMENT, "out must be an aligned device pointer");
+  if (ldo && ldo < w->K) return fail(NSA_ERR_INVALID_ARGUMENT, "ldo must be >= K");
+  const nsa::Quant4Params p = quant4_params(w);
+  const cudaStream_t strm = static_cast<cudaStream_t>(stream);
+  const double bytes = (double)w->N * w->K * (2.5 + 2.0 / w->group);
+  cudaError_t e = profiled("expand4", 0.0, bytes, strm, [&] {
+    return nsa::launch_expand4(p, static_cast<__nv_bfloat16*>(out), ldo ? ldo : w->K, strm);
+  });
+  if (e != cudaSuccess) return cuda_fail(e, "expand4 launch");
+  return NSA_OK;
+}
+
+nsa_status nsa_linear4(const nsa_linear4_desc* d, const nsa_weight4* w, const void* A, const float* bias, void* C,
+                       void* stream) {
+  if (!d) return fail(NSA_ERR_INVALID_ARGUMENT, "desc is NULL");
+  const nsa_status st = check_weight4(w);
+  if (st != NSA_OK) return st;
+  if (d->M < 0) return fail(NSA_ERR_INVALID_ARGUMENT, "M must be >= 0");
+  if (w->K % 8) return fail(NSA_ERR_INVALID_ARGUMENT, "K must be a multiple of 8");
+  const int64_t lda = d->lda ? d->lda : w->K, ldc = d->ldc ? d->ldc : w->N;
+  if (lda < w->K || lda % 8) return fail(NSA_ERR_INVALID_ARGUMENT, "lda must be >= K and a multiple of 8");
+  if (ldc < w->N) return fail(NSA_ERR_INVALID_ARGUMENT, "ldc must be >= N");
+  if (d->out_dtype != NSA_F32 && d->out_dtype != NSA_BF16) return fail(NSA_ERR_INVALID_ARGUMENT, "bad out_dtype");
+  if (d->resid && d->out_dtype != NSA_F32) return fail(NSA_ERR_INVALID_ARGUMENT, "resid needs an fp32 C");
+  if (d->M == 0) return NSA_OK;   // no rows (empty tensors may carry NULL pointers)
+  const int esz = d->out_dtype == NSA_F32 ? 4 : 2;
+  if (!A || !aligned16(A)) return fail(NSA_ERR_INVALID_ARGUMENT, "A must be a 16-byte aligned device pointer");
+  if (!C || (reinterpret_cast<uintptr_t>(C) & (esz - 1)) || (reinterpret_cast<uintptr_t>(bias) & 3))
+    return fail(NSA_ERR_INVALID_ARGUMENT, "C and bias must be device pointers aligned to their elements");
+  const uintptr_t a0 = reinterpret_cast<uintptr_t>(A), c0 = reinterpret_cast<uintptr_t>(C);
+  const uintptr_t a1 = a0 + (uintptr_t)(((int64_t)(d->M - 1) * lda + w->K) * 2);
+  const uintptr_t c1 = c0 + (uintptr_t)(((int64_t)(d->M - 1) * ldc + w->N) * esz);
+  if (a0 < c1 && c0 < a1) return fail(NSA_ERR_INVALID_ARGUMENT, "A and C must not overlap");
+  nsa::Linear4Params p{};
+  p.M = d->M;
+  p.N = w->N;
+  p.K = w->K;
+  p.G = w->group;
+  p.Nt = (w->N + 15) / 16;
+  p.Kc = (w->K + 127) / 128;
+  p.x = static_cast<const __nv_bfloat16*>(A);
+  p.ldx = lda;
+  p.codes = w->codes;
+  p.scales = static_cast<const __nv_bfloat16*>(w->scales);
+  p.bias = bias;
+  p.c = C;
+  p.ldc = ldc;
+  p.out_bf16 = d->out_dtype == NSA_BF16;
+  p.resid = d->resid ? 1 : 0;
+  const cudaStream_t strm = static_cast<cudaStream_t>(stream);
+  const double bytes = (double)w->N * w->K * (0.5 + 2.0 / w->group) + 2.0 * d->M * w->K +
+                       (double)d->M * w->N * esz * (d->resid ? 2 : 1);
+  cudaError_t e = profiled("linear4", 2.0 * d->M * w->N * w->K, bytes, strm, [&] { return nsa::launch_linear4(p, strm); });
+  if (e != cudaSuccess) return cuda_fail(e, "linear4 launch");
+  return NSA_OK;
+}
+
+// Checks of the cache and the step; fills everything but the error word.  *empty: no sequence or no row.
+static nsa_status kv4_params(const nsa_kv4_cache* c, const nsa_kv4_batch* s, nsa::Kv4Params* p, bool* empty) {
+  if (!c || !s) return fail(NSA_ERR_INVALID_ARGUMENT, "cache and batch must not be NULL");
+  if (c->D != 64 && c->D != 128 && c->D != 256)
+    return fail(NSA_ERR_UNSUPPORTED, "the 4-bit cache holds head dims 64, 128 and 256");
+  if (c->P < 16 || c->P > 1024 || c->P % 16) return fail(NSA_ERR_INVALID_ARGUMENT, "P must be a multiple of 16 in [16, 1024]");
+  if (c->n_pages < 0 || c->Hkv < 1) return fail(NSA_ERR_INVALID_ARGUMENT, "need n_pages >= 0 and Hkv >= 1");
+  if (s->B < 0 || s->L < 0 || s->max_pages < 0) return fail(NSA_ERR_INVALID_ARGUMENT, "need B, L and max_pages >= 0");
+  if ((int64_t)s->max_pages * c->P > 0x7FFFFFFFLL)
+    return fail(NSA_ERR_INVALID_ARGUMENT, "the page table spans more than 2^31 - 1 tokens");
+  const int64_t ld = s->table_ld ? s->table_ld : s->max_pages;
+  if (ld < s->max_pages && s->B > 1) return fail(NSA_ERR_INVALID_ARGUMENT, "table_ld must be >= max_pages");
+  *empty = s->B == 0 || s->L == 0;
+  *p = nsa::Kv4Params{};
+  p->n_pages = c->n_pages;
+  p->P = c->P;
+  p->Hkv = c->Hkv;
+  p->D = c->D;
+  p->codes = c->codes;
+  p->scales = static_cast<__nv_bfloat16*>(c->scales);
+  p->B = s->B;
+  p->L = s->L;
+  p->max_pages = s->max_pages;
+  p->table = s->table;
+  p->table_ld = ld;
+  p->start = s->start;
+  p->count = s->count;
+  if (*empty) return NSA_OK;
+  if (!s->start || (s->max_pages > 0 && !s->table)) return fail(NSA_ERR_INVALID_ARGUMENT, "table and start must be device pointers");
+  if ((reinterpret_cast<uintptr_t>(s->table) | reinterpret_cast<uintptr_t>(s->start) | reinterpret_cast<uintptr_t>(s->count)) & 3)
+    return fail(NSA_ERR_INVALID_ARGUMENT, "table, start and count must be 4-byte aligned");
+  if (c->n_pages > 0 && (!c->codes || !c->scales || !aligned16(c->codes) || !aligned16(c->scales)))
+    return fail(NSA_ERR_INVALID_ARGUMENT, "codes and scales must be 16-byte aligned device pointers");
+  return NSA_OK;
+}
+
+static nsa_status kv4_error_word(nsa::Kv4Params* p) {
+  p->err = nsa::device_error_word();
+  return p->err ? NSA_OK : fail(NSA_ERR_CUDA, "cannot resolve the device error word on this device");
+}
+
+// Whether rows (b, i) of `width` elements at b * bstride + i * ld overlap one another (two rows of a result
+// must not share memory).
+static bool rows_overlap(int B, int L, int64_t ld, int64_t bstride, int64_t width) {
+  if (L > 1 && ld < width) return true;
+  if (B > 1 && bstride < (int64_t)(L - 1) * ld + width && !(bstride >= width && ld >= (int64_t)(B - 1) * bstride + width))
+    return true;
+  return false;
+}
+
+nsa_status nsa_kv4_append(const nsa_kv4_append_desc* d, const nsa_kv4_cache* cache, const nsa_kv4_batch* batch,
+                          const void* qkv, const float* q_norm_w, const float* k_norm_w, const float* cs, void* q_out,
+                          void* stream) {
+  if (!d) return fail(NSA_ERR_INVALID_ARGUMENT, "desc is NULL");
+  nsa::Kv4AppendParams p{};
+  bool empty = false;
+  nsa_status st = kv4_params(cache, batch, &p.kv, &empty);
+  if (st != NSA_OK) return st;
+  if (d->Hq < 1 || d->Hq % cache->Hkv) return fail(NSA_ERR_INVALID_ARGUMENT, "Hq must be a positive multiple of Hkv");
+  if (d->in_dtype != NSA_F32 && d->in_dtype != NSA_BF16) return fail(NSA_ERR_INVALID_ARGUMENT, "bad input dtype");
+  if ((d->ld | d->bstride | d->qOff | d->kOff | d->vOff) % 4 || d->ld < 0 || d->bstride < 0 || d->qOff < 0 ||
+      d->kOff < 0 || d->vOff < 0)
+    return fail(NSA_ERR_INVALID_ARGUMENT, "ld, bstride and the q/k/v offsets must be multiples of 4, >= 0");
+  if (!(d->eps >= 0.f)) return fail(NSA_ERR_INVALID_ARGUMENT, "eps must be >= 0");
+  if (cs && (d->rope_rows < 1 || d->sinOff < 0 || d->sinOff % 4))
+    return fail(NSA_ERR_INVALID_ARGUMENT, "cs needs rope_rows >= 1 and sinOff a multiple of 4");
+  if (empty) return NSA_OK;
+  if (!qkv || !aligned16(qkv)) return fail(NSA_ERR_INVALID_ARGUMENT, "qkv must be a 16-byte aligned device pointer");
+  if (!q_norm_w || !k_norm_w || !aligned16(q_norm_w) || !aligned16(k_norm_w) || (cs && !aligned16(cs)))
+    return fail(NSA_ERR_INVALID_ARGUMENT, "the q/k norm weights (required) and cs must be 16-byte aligned");
+  if (!q_out || !aligned16(q_out) || (d->qo_ld | d->qo_bstride) % 8)
+    return fail(NSA_ERR_INVALID_ARGUMENT, "q_out must be 16-byte aligned with pitches that are multiples of 8");
+  if (rows_overlap(batch->B, batch->L, d->qo_ld, d->qo_bstride, (int64_t)d->Hq * cache->D))
+    return fail(NSA_ERR_INVALID_ARGUMENT, "q_out rows must not overlap");
+  {
+    const int64_t cols = std::max({d->qOff + (int64_t)d->Hq * cache->D, d->kOff + (int64_t)cache->Hkv * cache->D,
+                                   d->vOff + (int64_t)cache->Hkv * cache->D});
+    const uintptr_t x0 = reinterpret_cast<uintptr_t>(qkv), o0 = reinterpret_cast<uintptr_t>(q_out);
+    const uintptr_t x1 = x0 + (uintptr_t)(((int64_t)(batch->B - 1) * d->bstride + (int64_t)(batch->L - 1) * d->ld + cols) *
+                                          (d->in_dtype == NSA_F32 ? 4 : 2));
+    const uintptr_t o1 = o0 + (uintptr_t)(((int64_t)(batch->B - 1) * d->qo_bstride + (int64_t)(batch->L - 1) * d->qo_ld +
+                                           (int64_t)d->Hq * cache->D) * 2);
+    if (x0 < o1 && o0 < x1) return fail(NSA_ERR_INVALID_ARGUMENT, "qkv and q_out must not overlap");
+  }
+  if ((st = kv4_error_word(&p.kv)) != NSA_OK) return st;
+  p.qkv = qkv;
+  p.in_f32 = d->in_dtype == NSA_F32;
+  p.Hq = d->Hq;
+  p.ld = d->ld;
+  p.bstride = d->bstride;
+  p.q_off = d->qOff;
+  p.k_off = d->kOff;
+  p.v_off = d->vOff;
+  p.q_w = q_norm_w;
+  p.k_w = k_norm_w;
+  p.cs = cs;
+  p.sin_off = d->sinOff;
+  p.rope_rows = d->rope_rows;
+  p.eps = d->eps;
+  p.q_out = static_cast<__nv_bfloat16*>(q_out);
+  p.qo_ld = d->qo_ld;
+  p.qo_bstride = d->qo_bstride;
+  const cudaStream_t strm = static_cast<cudaStream_t>(stream);
+  const double bytes = (double)batch->B * batch->L * cache->D *
+                       ((d->Hq + 2.0 * cache->Hkv) * (p.in_f32 ? 4 : 2) + 2.0 * d->Hq + 2.0 * cache->Hkv * 0.5625);
+  cudaError_t e = profiled("kv4_append", 0.0, bytes, strm, [&] { return nsa::launch_kv4_append(p, strm); });
+  if (e != cudaSuccess) return cuda_fail(e, "kv4_append launch");
+  return NSA_OK;
+}
+
+nsa_status nsa_kv4_read(const nsa_kv4_cache* cache, const nsa_kv4_batch* batch, void* out, int64_t ldo, int64_t bstride,
+                        void* stream) {
+  nsa::Kv4Params p{};
+  bool empty = false;
+  nsa_status st = kv4_params(cache, batch, &p, &empty);
+  if (st != NSA_OK) return st;
+  if (empty) return NSA_OK;
+  const int64_t width = 2 * (int64_t)cache->Hkv * cache->D;
+  if (!out || !aligned16(out) || (ldo | bstride) % 8)
+    return fail(NSA_ERR_INVALID_ARGUMENT, "out must be 16-byte aligned with pitches that are multiples of 8");
+  if (rows_overlap(batch->B, batch->L, ldo, bstride, width)) return fail(NSA_ERR_INVALID_ARGUMENT, "out rows must not overlap");
+  if ((st = kv4_error_word(&p)) != NSA_OK) return st;
+  const cudaStream_t strm = static_cast<cudaStream_t>(stream);
+  cudaError_t e = profiled("kv4_read", 0.0, (double)batch->B * batch->L * width * 2.5625, strm, [&] {
+    return nsa::launch_kv4_read(p, static_cast<__nv_bfloat16*>(out), ldo, bstride, strm);
+  });
+  if (e != cudaSuccess) return cuda_fail(e, "kv4_read launch");
+  return NSA_OK;
+}
+
+// Checks shared by nsa_kv4_attention and its workspace size.
+static nsa_status kv4_attention_params(const nsa_kv4_attention_desc* d, const nsa_kv4_cache* cache,
+                                       const nsa_kv4_batch* batch, nsa::Kv4AttnParams* p, bool* empty) {
+  if (!d) return fail(NSA_ERR_INVALID_ARGUMENT, "desc is NULL");
+  const nsa_status st = kv4_params(cache, batch, &p->kv, empty);
+  if (st != NSA_OK) return st;
+  if (d->Hq < 1 || d->Hq % cache->Hkv) return fail(NSA_ERR_INVALID_ARGUMENT, "Hq must be a positive multiple of Hkv");
+  if (d->window < 0 || d->sinks < 0) return fail(NSA_ERR_INVALID_ARGUMENT, "window and sinks must be >= 0");
+  if (d->sinks > 0 && d->window == 0) return fail(NSA_ERR_INVALID_ARGUMENT, "sinks needs a window");
+  if (!(d->scale >= 0.f) || d->scale > 3.0e38f) return fail(NSA_ERR_INVALID_ARGUMENT, "scale must be finite and >= 0");
+  if ((d->q_ld | d->q_bstride | d->o_ld | d->o_bstride) % 8 || d->q_ld < 0 || d->q_bstride < 0)
+    return fail(NSA_ERR_INVALID_ARGUMENT, "the q and out pitches must be multiples of 8, >= 0");
+  p->Hq = d->Hq;
+  p->window = d->window;
+  p->sinks = d->sinks;
+  p->scale_log2 = (d->scale > 0.f ? d->scale : 1.f / std::sqrt((float)cache->D)) * 1.4426950408889634f;
+  p->q_ld = d->q_ld;
+  p->q_bstride = d->q_bstride;
+  p->o_ld = d->o_ld;
+  p->o_bstride = d->o_bstride;
+  return NSA_OK;
+}
+
+size_t nsa_kv4_attention_workspace_size(const nsa_kv4_attention_desc* d, const nsa_kv4_cache* cache,
+                                        const nsa_kv4_batch* batch) {
+  nsa::Kv4AttnParams p{};
+  bool empty = false;
+  if (kv4_attention_params(d, cache, batch, &p, &empty) != NSA_OK || empty) return 0;
+  return nsa::kv4_attention_workspace(p);
+}
+
+nsa_status nsa_kv4_attention(const nsa_kv4_attention_desc* d, const nsa_kv4_cache* cache, const nsa_kv4_batch* batch,
+                             const void* q, void* out, void* workspace, size_t workspace_bytes, void* stream) {
+  nsa::Kv4AttnParams p{};
+  bool empty = false;
+  nsa_status st = kv4_attention_params(d, cache, batch, &p, &empty);
+  if (st != NSA_OK) return st;
+  if (empty) return NSA_OK;
+  if (!q || !out || !aligned16(q) || !aligned16(out))
+    return fail(NSA_ERR_INVALID_ARGUMENT, "q and out must be 16-byte aligned device pointers");
+  const int64_t width = (int64_t)d->Hq * cache->D;
+  if (rows_overlap(batch->B, batch->L, d->o_ld, d->o_bstride, width))
+    return fail(NSA_ERR_INVALID_ARGUMENT, "out rows must not overlap");
+  const uintptr_t q0 = reinterpret_cast<uintptr_t>(q), o0 = reinterpret_cast<uintptr_t>(out);
+  const auto span = [&](int64_t ld, int64_t bs) {
+    return (uintptr_t)(((int64_t)(batch->B - 1) * bs + (int64_t)(batch->L - 1) * ld + width) * 2);
+  };
+  if (q0 < o0 + span(d->o_ld, d->o_bstride) && o0 < q0 + span(d->q_ld, d->q_bstride))
+    return fail(NSA_ERR_INVALID_ARGUMENT, "q and out must not overlap");
+  const size_t need = nsa::kv4_attention_workspace(p);
+  if (need && (!workspace || workspace_bytes < need || !aligned16(workspace)))
+    return fail(NSA_ERR_WORKSPACE, "a 16-byte aligned workspace of " + std::to_string(need) + " bytes required, got " +
+                                       std::to_string(workspace ? workspace_bytes : 0));
+  if ((st = kv4_error_word(&p.kv)) != NSA_OK) return st;
+  p.q = static_cast<const __nv_bfloat16*>(q);
+  p.out = static_cast<__nv_bfloat16*>(out);
+  const cudaStream_t strm = static_cast<cudaStream_t>(stream);
+  cudaError_t e = profiled("kv4_attention", 0.0, 0.0, strm, [&] { return nsa::launch_kv4_attention(p, workspace, strm); });
+  if (e != cudaSuccess) return cuda_fail(e, "kv4_attention launch");
   return NSA_OK;
 }
 

@@ -277,6 +277,73 @@ cudaError_t launch_glu(const GluParams& p, cudaStream_t stream);
 // Gate/up row interleave per 128-row tile for the linear's fused GLU (glu.cu); row_bytes a multiple of 4.
 cudaError_t launch_glu_interleave(const void* src, void* dst, int I, int64_t row_bytes, cudaStream_t stream);
 
+// Linears with 4-bit weights and group scales (linear4.cu; the format is in q4.cuh): the quantiser and the
+// expansion back to bf16, and C[m][n] (=|+=) sum_k A[m][k] W[n][k] (+ bias[n]) for few rows.
+struct Quant4Params {
+  int N, K, G;
+  int Nt, Kc;             // row tiles of 16, chunks of 128
+  const void* w;          // [N][ldw] fp32 (in_f32) or bf16
+  int64_t ldw;
+  int in_f32;
+  uint8_t* codes;         // [Nt][Kc][16][64]
+  __nv_bfloat16* scales;  // [Nt][Kc][16][128 / G]
+};
+cudaError_t launch_quantize4(const Quant4Params& p, cudaStream_t stream);
+cudaError_t launch_expand4(const Quant4Params& p, __nv_bfloat16* out, int64_t ldo, cudaStream_t stream);
+struct Linear4Params {
+  int M, N, K, G;
+  int Nt, Kc;
+  const __nv_bfloat16* x;   // [M][ldx], rows 16-byte aligned, K a multiple of 8
+  int64_t ldx;
+  const uint8_t* codes;
+  const __nv_bfloat16* scales;
+  const float* bias;        // [N] or null
+  void* c;                  // [M][ldc] fp32, or bf16 (out_bf16)
+  int64_t ldc;
+  int out_bf16, resid;
+};
+cudaError_t launch_linear4(const Linear4Params& p, cudaStream_t stream);
+
+// 4-bit paged key/value cache (kv4.cu).
+struct Kv4Params {
+  int n_pages, P, Hkv, D;
+  uint8_t* codes;           // [n_pages][2][Hkv][P][D / 2]
+  __nv_bfloat16* scales;    // [n_pages][2][Hkv][P][D / 32]
+  int B, L, max_pages;      // sequences, rows of new tokens per sequence, page table width
+  const int* table;         // [B][table_ld]
+  int64_t table_ld;
+  const int* start;         // [B] tokens stored before this step
+  const int* count;         // [B] new tokens, or null (L)
+  int* err;
+};
+struct Kv4AppendParams {
+  Kv4Params kv;
+  const void* qkv;          // row (b, i) at b * bstride + i * ld; fp32 (in_f32) or bf16
+  int in_f32, Hq;
+  int64_t ld, bstride, q_off, k_off, v_off;
+  const float* q_w;
+  const float* k_w;
+  const float* cs;          // RoPE table (cos [rope_rows][D / 2], sin at sin_off) or null
+  int64_t sin_off;
+  int rope_rows;
+  float eps;
+  __nv_bfloat16* q_out;     // row (b, i) at b * qo_bstride + i * qo_ld
+  int64_t qo_ld, qo_bstride;
+};
+cudaError_t launch_kv4_append(const Kv4AppendParams& p, cudaStream_t stream);
+cudaError_t launch_kv4_read(const Kv4Params& p, __nv_bfloat16* out, int64_t ldo, int64_t bstride, cudaStream_t stream);
+struct Kv4AttnParams {
+  Kv4Params kv;
+  int Hq, window, sinks;
+  float scale_log2;         // softmax scale * log2(e)
+  const __nv_bfloat16* q;
+  int64_t q_ld, q_bstride;
+  __nv_bfloat16* out;
+  int64_t o_ld, o_bstride;
+};
+size_t kv4_attention_workspace(const Kv4AttnParams& p);   // bytes; 0: none needed
+cudaError_t launch_kv4_attention(const Kv4AttnParams& p, void* workspace, cudaStream_t stream);
+
 // Returns cudaErrorInvalidValue for unsupported head dims.
 cudaError_t launch_attention(const AttnParams& p, int D, const CUtensorMap& tmQ, const CUtensorMap& tmK,
                              const CUtensorMap& tmV, const CUtensorMap& tmVd, cudaStream_t stream);

@@ -73,6 +73,8 @@ enum : int {
   kErrTimeoutSoftmax = 0x103,  // softmax warps waited too long for scores / output
   kErrTimeoutProjection = 0x105,  // projection GEMM roles waited too long for a stage / accumulator
   kErrAborted = 0x1FF,         // another role of the CTA gave up first
+  kErrKvPage = 0x201,          // a page table entry outside the cache's pool
+  kErrKvPosition = 0x202,      // a token position outside the page table or the RoPE table
 };
 
 // Wait until the phase with `parity` of `bar` has completed.  Gives up (returns false) when the
