@@ -340,9 +340,13 @@ struct Kv4AttnParams {
   int64_t q_ld, q_bstride;
   __nv_bfloat16* out;
   int64_t o_ld, o_bstride;
+  // set by the launch
+  int row_tiles, splits;    // tiles of 8 query rows per kv head; CTAs that share a tile's keys
+  float* part_o;            // [units][splits][8][D] unnormalised outputs (units: sequence, kv head, row tile)
+  float* part_ml;           // [units][splits][8][2] maximum (base 2) and sum
 };
-size_t kv4_attention_workspace(const Kv4AttnParams& p);   // bytes; 0: none needed
-cudaError_t launch_kv4_attention(const Kv4AttnParams& p, void* workspace, cudaStream_t stream);
+size_t kv4_attention_workspace(Kv4AttnParams p);   // bytes; 0: none needed
+cudaError_t launch_kv4_attention(Kv4AttnParams p, void* workspace, cudaStream_t stream);
 
 // Returns cudaErrorInvalidValue for unsupported head dims.
 cudaError_t launch_attention(const AttnParams& p, int D, const CUtensorMap& tmQ, const CUtensorMap& tmK,
