@@ -301,8 +301,9 @@ struct Linear4Params {
   void* c;                  // [M][ldc] fp32, or bf16 (out_bf16)
   int64_t ldc;
   int out_bf16, resid;
+  int WK;                   // warps that share a row tile's chunks (set by the launch)
 };
-cudaError_t launch_linear4(const Linear4Params& p, cudaStream_t stream);
+cudaError_t launch_linear4(Linear4Params p, cudaStream_t stream);
 
 // 4-bit paged key/value cache (kv4.cu).
 struct Kv4Params {

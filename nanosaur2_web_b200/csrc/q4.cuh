@@ -75,4 +75,13 @@ __device__ __forceinline__ float q4_value(uint32_t w, int p, float s) {
 // holds the neighbours 2p and 2p + 1 in its two halves.
 __host__ __device__ constexpr int q4_nibble(int e) { return (e & 1) ? 4 + e / 2 : e / 2; }
 
+// C[16][8] += A[16][16] B[16][8], bf16 operands, fp32 sums; lane (r, c) = (lane / 4, lane % 4) holds A's rows r
+// (a0, a2) and r + 8 (a1, a3), its k pairs 2c (a0, a1) and 2c + 8 (a2, a3), B's column r at the same k pairs (b0,
+// b1), and C's rows r (c0, c1) and r + 8 (c2, c3) at columns 2c and 2c + 1.
+__device__ __forceinline__ void mma_bf16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
 }  // namespace nsa
