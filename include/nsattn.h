@@ -454,10 +454,10 @@ nsa_status nsa_expand4(const nsa_weight4* w, void* out, int64_t ldo, void* strea
 
 /* nsa_linear4: ops.linear (app/gpu/ops.js:50-66) with a 4-bit weight, for decode steps:
  *   C[m*ldc + n] = r, or += r with resid, where r = sum_k A[m][k] W[n][k] (+ bias[n]).
- * A bf16 [M][lda]; K and lda multiples of 8, A 16-byte aligned; C fp32 or (store form) bf16, at its
+ * A bf16 [M][lda]; K and lda multiples of 8, K at most 98304 (NSA_ERR_UNSUPPORTED), A 16-byte aligned; C fp32 or (store form) bf16, at its
  * element alignment; C must not overlap A.  The products are exact and sums are kept in fp32, so the result
- * is the fp32 linear's.  Any M runs; the weights are read once per 32 rows of A, so from a few hundred rows
- * on nsa_linear over the nsa_expand4 copy is faster. */
+ * is the fp32 linear's.  Any M runs; the weights are read once per 32 rows of A (fewer where 32 rows of K do not
+ * fit shared memory), so for hundreds of rows nsa_linear over the nsa_expand4 copy is faster. */
 typedef struct nsa_linear4_desc {
   int32_t M;
   int64_t lda;           /* A row pitch in elements (0: K) */

@@ -1633,6 +1633,7 @@ nsa_status nsa_linear4(const nsa_linear4_desc* d, const nsa_weight4* w, const vo
   if (st != NSA_OK) return st;
   if (d->M < 0) return fail(NSA_ERR_INVALID_ARGUMENT, "M must be >= 0");
   if (w->K % 8) return fail(NSA_ERR_INVALID_ARGUMENT, "K must be a multiple of 8");
+  if (w->K > nsa::kLinear4MaxK) return fail(NSA_ERR_UNSUPPORTED, "nsa_linear4 takes K up to " + std::to_string(nsa::kLinear4MaxK));
   const int64_t lda = d->lda ? d->lda : w->K, ldc = d->ldc ? d->ldc : w->N;
   if (lda < w->K || lda % 8) return fail(NSA_ERR_INVALID_ARGUMENT, "lda must be >= K and a multiple of 8");
   if (ldc < w->N) return fail(NSA_ERR_INVALID_ARGUMENT, "ldc must be >= N");

@@ -5,6 +5,8 @@
 // Layout (made once, at load): rows in tiles of 16, K in chunks of 128, zero padded; a tile's chunk is
 // 1024 contiguous bytes [16 rows][64], its scales [16 rows][128 / G] bf16.  Of a row's 64 bytes, the word
 // at 16 c + 4 i holds the values 32 i + 8 c .. + 7 (nibble order: q4_nibble).
+#include <algorithm>
+
 #include "nsa_internal.h"
 #include "q4.cuh"
 
@@ -83,10 +85,13 @@ __global__ void __launch_bounds__(256) expand4_kernel(const Quant4Params p, __nv
 // (q4_nibble), so X's own 16 bytes of values 32 i + 8 c .. + 7 are the B fragments.  A nibble n set into a bf16
 // mantissa is 128 + n; minus 136 it is the code, exactly.
 //
-// A tile's chunks are one contiguous stream, shared by WK warps of the CTA (chunk k to warp k % WK) and joined
-// in shared memory; each warp keeps kStages chunks in flight.
+// One CTA of 16 warps per SM takes TN = 16 / WK tiles at a time, the WK warps of a tile its chunks in turn, each
+// with kStages chunks in flight across tile ends, and joins them in shared memory.  The rows of X that the pass
+// covers are staged once per CTA, in the fragments' order.
 
 constexpr int kStages = 4;
+constexpr int kWarps = 16;
+constexpr int kSmemMax = 227 * 1024;
 
 // Scales of a row's chunk: 128 / G bf16 in one load.
 template <int G>
@@ -122,48 +127,71 @@ __device__ __forceinline__ uint32_t code_pair(uint32_t w) {
 
 // NT: tiles of eight rows of X.
 template <int G, int NT>
-__global__ void __launch_bounds__(256) linear4_kernel(const Linear4Params p) {
-  __shared__ float red[8][16 * 8 * NT];
+__global__ void __launch_bounds__(kWarps * 32) linear4_kernel(const Linear4Params p) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  constexpr int kOut = 16 * 8 * NT;                              // values of a tile
+  float* red = reinterpret_cast<float*>(smem);                   // [kWarps][m][16]
+  uint4* xs = reinterpret_cast<uint4*>(smem + kWarps * kOut * 4);   // [Kc][4 words i][rows][4 pieces c]
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, r = lane / 4, c = lane % 4;
-  const int wk = warp % p.WK, tile = blockIdx.x * (8 / p.WK) + warp / p.WK;
-  const int m0 = blockIdx.y * 8 * NT;
+  const int wk = warp % p.WK, tn = warp / p.WK, TN = kWarps / p.WK;
+  const int m0 = blockIdx.y * p.rows, rows = min(p.rows, p.M - m0);
+  const int steps = (p.Kc + p.WK - 1) / p.WK;                     // chunks of a tile per warp
+  const int stride = gridDim.x * TN;
+  const int tiles = (p.Nt - (int)blockIdx.x * TN + stride - 1) / stride;   // rounds of this CTA (>= 1)
+
+  uint4 qa[kStages], qb[kStages];
+  ChunkScales<G> sa[kStages], sb[kStages];
+  int f_tile = blockIdx.x * TN + tn, f_ch = wk, f_left = tiles * steps;   // what the next fetch takes
+  int f_step = 0;
+  const auto fetch = [&](int st) {
+    if (f_left-- > 0 && f_tile < p.Nt && f_ch < p.Kc) {
+      const int64_t at = (int64_t)f_tile * p.Kc + f_ch;
+      const uint4* codes = reinterpret_cast<const uint4*>(p.codes) + at * 64 + r * 4 + c;
+      const __nv_bfloat16* scales = p.scales + (at * 16 + r) * (kChunk / G);
+      qa[st] = __ldg(codes);
+      qb[st] = __ldg(codes + 32);
+      sa[st].load(scales);
+      sb[st].load(scales + 8 * (kChunk / G));
+    }
+    f_ch += p.WK;
+    if (++f_step == steps) {
+      f_step = 0;
+      f_ch = wk;
+      f_tile += stride;
+    }
+  };
+#pragma unroll
+  for (int st = 0; st < kStages; ++st) fetch(st);
+
+  for (int e = threadIdx.x; e < p.Kc * 16 * rows; e += kWarps * 32) {
+    const int w = e / rows, m = e % rows;                         // word w of row m: value 8 w
+    const int ch = w / 16, i = w % 16 / 4, cc = w % 4;
+    xs[((ch * 4 + i) * rows + m) * 4 + cc] =
+        w * 8 < p.K ? __ldg(reinterpret_cast<const uint4*>(p.x + (int64_t)(m0 + m) * p.ldx + w * 8)) : make_uint4(0u, 0u, 0u, 0u);
+  }
+  __syncthreads();
+
+  // columns past the pass's rows repeat its last row; they are not stored
+  const uint4* xt[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) xt[t] = xs + min(8 * t + r, rows - 1) * 4 + c;
   float y[NT][4];
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
     for (int j = 0; j < 4; ++j) y[t][j] = 0.f;
-  if (tile < p.Nt) {
-    const uint4* codes = reinterpret_cast<const uint4*>(p.codes) + ((int64_t)tile * p.Kc * 16 + r) * 4 + c;
-    const __nv_bfloat16* scales = p.scales + ((int64_t)tile * p.Kc * 16 + r) * (kChunk / G);
-    uint4 qa[kStages], qb[kStages];
-    ChunkScales<G> sa[kStages], sb[kStages];
-    const auto fetch = [&](int st, int ch) {
-      if (ch >= p.Kc) return;
-      qa[st] = __ldg(codes + (int64_t)ch * 64);
-      qb[st] = __ldg(codes + (int64_t)ch * 64 + 32);
-      sa[st].load(scales + (int64_t)ch * (16 * kChunk / G));
-      sb[st].load(scales + (int64_t)ch * (16 * kChunk / G) + 8 * (kChunk / G));
-    };
+  int tile0 = blockIdx.x * TN, step = 0;
+  const int total = tiles * steps;
+  for (int f = 0; f < total; f += kStages) {
 #pragma unroll
-    for (int st = 0; st < kStages; ++st) fetch(st, wk + st * p.WK);
-    for (int base = wk; base < p.Kc; base += kStages * p.WK) {
-#pragma unroll
-      for (int st = 0; st < kStages; ++st) {
-        const int ch = base + st * p.WK;
-        if (ch >= p.Kc) break;
+    for (int st = 0; st < kStages; ++st) {
+      if (f + st >= total) break;
+      const int ch = wk + step * p.WK;
+      if (ch < p.Kc && tile0 + tn < p.Nt) {
         const uint32_t wa[4] = {qa[st].x, qa[st].y, qa[st].z, qa[st].w}, wb[4] = {qb[st].x, qb[st].y, qb[st].z, qb[st].w};
-        const ChunkScales<G> ca = sa[st], cb = sb[st];
-        fetch(st, ch + kStages * p.WK);
         float acc[NT][4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int k = ch * kChunk + 32 * i + 8 * c;
-          uint4 x[NT];
-#pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            const int m = m0 + 8 * t + r;
-            x[t] = m < p.M && k < p.K ? __ldg(reinterpret_cast<const uint4*>(p.x + m * p.ldx + k)) : make_uint4(0u, 0u, 0u, 0u);
-          }
           if (32 * i % G == 0) {
 #pragma unroll
             for (int t = 0; t < NT; ++t)
@@ -174,11 +202,12 @@ __global__ void __launch_bounds__(256) linear4_kernel(const Linear4Params p) {
           const uint32_t a4 = code_pair<2>(wa[i]), a5 = code_pair<2>(wb[i]), a6 = code_pair<3>(wa[i]), a7 = code_pair<3>(wb[i]);
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
-            mma_bf16(acc[t], a0, a1, a2, a3, x[t].x, x[t].y);
-            mma_bf16(acc[t], a4, a5, a6, a7, x[t].z, x[t].w);
+            const uint4 x = xt[t][(ch * 4 + i) * rows * 4];
+            mma_bf16(acc[t], a0, a1, a2, a3, x.x, x.y);
+            mma_bf16(acc[t], a4, a5, a6, a7, x.z, x.w);
           }
           if (32 * (i + 1) % G == 0) {
-            const float fa = ca.get(32 * i / G), fb = cb.get(32 * i / G);
+            const float fa = sa[st].get(32 * i / G), fb = sb[st].get(32 * i / G);
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
               y[t][0] = fmaf(fa, acc[t][0], y[t][0]);
@@ -189,44 +218,60 @@ __global__ void __launch_bounds__(256) linear4_kernel(const Linear4Params p) {
           }
         }
       }
-    }
-  }
-  // red[warp][m][n]
+      fetch(st);
+      if (++step < steps) continue;
+      // the round's tiles are done: join their warps
+      step = 0;
+      __syncthreads();   // the previous round's sums have been read
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    float* d = red[warp] + (8 * t + 2 * c) * 16 + r;
-    d[0] = y[t][0];
-    d[16] = y[t][1];
-    d[8] = y[t][2];
-    d[24] = y[t][3];
-  }
-  __syncthreads();
-  for (int e = threadIdx.x; e < (8 / p.WK) * 16 * 8 * NT; e += 256) {
-    const int g = e / (16 * 8 * NT), at = e % (16 * 8 * NT);
-    const int m = m0 + at / 16, n = (blockIdx.x * (8 / p.WK) + g) * 16 + at % 16;
-    if (m >= p.M || n >= p.N) continue;
-    float v = 0.f;
-    for (int w = 0; w < p.WK; ++w) v += red[g * p.WK + w][at];
-    if (p.bias) v += p.bias[n];
-    const int64_t o = m * p.ldc + n;
-    if (p.out_bf16) static_cast<__nv_bfloat16*>(p.c)[o] = __float2bfloat16_rn(v);
-    else if (p.resid) static_cast<float*>(p.c)[o] += v;
-    else static_cast<float*>(p.c)[o] = v;
+      for (int t = 0; t < NT; ++t) {
+        float* d = red + warp * kOut + (8 * t + 2 * c) * 16 + r;
+        d[0] = y[t][0];
+        d[16] = y[t][1];
+        d[8] = y[t][2];
+        d[24] = y[t][3];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[t][j] = 0.f;
+      }
+      __syncthreads();
+      for (int e = threadIdx.x; e < TN * 16 * rows; e += kWarps * 32) {
+        const int g = e / (16 * rows), at = e % (16 * rows);
+        const int m = m0 + at / 16, n = (tile0 + g) * 16 + at % 16;
+        if (n >= p.N) continue;
+        float v = 0.f;
+        for (int w = 0; w < p.WK; ++w) v += red[(g * p.WK + w) * kOut + at];
+        if (p.bias) v += p.bias[n];
+        const int64_t o = m * p.ldc + n;
+        if (p.out_bf16) static_cast<__nv_bfloat16*>(p.c)[o] = __float2bfloat16_rn(v);
+        else if (p.resid) static_cast<float*>(p.c)[o] += v;
+        else static_cast<float*>(p.c)[o] = v;
+      }
+      tile0 += stride;
+    }
   }
 }
 
-template <int G>
-cudaError_t launch_linear_g(const Linear4Params& p, cudaStream_t stream) {
-  const int nt = p.M >= 32 ? 4 : (p.M + 7) / 8;
-  const dim3 grid((unsigned)((p.Nt + 8 / p.WK - 1) / (8 / p.WK)), (unsigned)((p.M + 8 * nt - 1) / (8 * nt)));
-  if (grid.y > 65535) return cudaErrorInvalidValue;
-  switch (nt) {
-    case 1: linear4_kernel<G, 1><<<grid, 256, 0, stream>>>(p); break;
-    case 2: linear4_kernel<G, 2><<<grid, 256, 0, stream>>>(p); break;
-    case 3: linear4_kernel<G, 3><<<grid, 256, 0, stream>>>(p); break;
-    default: linear4_kernel<G, 4><<<grid, 256, 0, stream>>>(p); break;
-  }
+template <int G, int NT>
+cudaError_t launch_linear_gn(const Linear4Params& p, dim3 grid, size_t bytes, cudaStream_t stream) {
+  static DeviceOnce once;
+  const cudaError_t e = once_per_device(once, [] {
+    return cudaFuncSetAttribute(linear4_kernel<G, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax);
+  });
+  if (e != cudaSuccess) return e;
+  linear4_kernel<G, NT><<<grid, kWarps * 32, bytes, stream>>>(p);
   return cudaGetLastError();
+}
+
+template <int G>
+cudaError_t launch_linear_g(const Linear4Params& p, dim3 grid, cudaStream_t stream) {
+  const int nt = (p.rows + 7) / 8;
+  const size_t bytes = (size_t)kWarps * 16 * 8 * nt * 4 + (size_t)p.rows * p.Kc * kChunk * 2;
+  switch (nt) {
+    case 1: return launch_linear_gn<G, 1>(p, grid, bytes, stream);
+    case 2: return launch_linear_gn<G, 2>(p, grid, bytes, stream);
+    case 3: return launch_linear_gn<G, 3>(p, grid, bytes, stream);
+    default: return launch_linear_gn<G, 4>(p, grid, bytes, stream);
+  }
 }
 
 template <typename T>
@@ -254,15 +299,29 @@ cudaError_t launch_expand4(const Quant4Params& p, __nv_bfloat16* out, int64_t ld
   return cudaGetLastError();
 }
 
-// Warps per tile: as few as give every SM 16 warps (a warp's own stream is longer and its join cheaper), but
-// no more than a tile has chunks.
+// Rows of X per pass: up to 32, as many as shared memory holds beside the joins, evenly over the passes.
+// Warps per tile: the number with the fewest steps of a warp (rounds of tiles times chunks per warp); of equal
+// ones the largest, whose joins are the fewest tiles at a time.
 cudaError_t launch_linear4(Linear4Params p, cudaStream_t stream) {
-  p.WK = 1;
-  while (p.WK < 8 && (int64_t)p.Nt * p.WK < 16 * 148 && 2 * p.WK <= p.Kc) p.WK *= 2;
+  if (p.Kc > kLinear4MaxK / kChunk) return cudaErrorInvalidValue;
+  const int sms = device_sm_count();
+  int rows = 32;
+  while (rows > 1 && (size_t)kWarps * 16 * 4 * ((rows + 7) / 8 * 8) + (size_t)rows * p.Kc * kChunk * 2 > kSmemMax) --rows;
+  const int passes = (p.M + rows - 1) / rows;
+  if (passes > 65535) return cudaErrorInvalidValue;
+  p.rows = (p.M + passes - 1) / passes;
+  int64_t best = INT64_MAX;
+  for (int wk = kWarps; wk >= 1; wk /= 2) {
+    const int64_t tn = kWarps / wk;
+    const int64_t steps = (p.Nt + tn * sms - 1) / (tn * sms) * ((p.Kc + wk - 1) / wk);
+    if (steps < best) best = steps, p.WK = wk;
+  }
+  const int tn = kWarps / p.WK;
+  const dim3 grid((unsigned)std::min((p.Nt + tn - 1) / tn, sms), (unsigned)passes);
   switch (p.G) {
-    case 32: return launch_linear_g<32>(p, stream);
-    case 64: return launch_linear_g<64>(p, stream);
-    default: return launch_linear_g<128>(p, stream);
+    case 32: return launch_linear_g<32>(p, grid, stream);
+    case 64: return launch_linear_g<64>(p, grid, stream);
+    default: return launch_linear_g<128>(p, grid, stream);
   }
 }
 

@@ -301,8 +301,11 @@ struct Linear4Params {
   void* c;                  // [M][ldc] fp32, or bf16 (out_bf16)
   int64_t ldc;
   int out_bf16, resid;
-  int WK;                   // warps that share a row tile's chunks (set by the launch)
+  // set by the launch
+  int WK;                   // warps that share a row tile's chunks
+  int rows;                 // rows of X a pass covers
 };
+constexpr int kLinear4MaxK = 98304;   // one row of X in shared memory beside the joins
 cudaError_t launch_linear4(Linear4Params p, cudaStream_t stream);
 
 // 4-bit paged key/value cache (kv4.cu).

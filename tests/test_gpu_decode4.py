@@ -136,7 +136,8 @@ def test_linear4_rows(M, N, K, group):
 
 
 @pytest.mark.parametrize("M,N,K,group", [(1, 640, 1024, 32), (3, 4096, 640, 64), (20, 640, 2048, 128), (1, 20000, 4096, 128),
-                                         (5, 16, 20000, 32), (2, 1, 8, 32), (33, 1536, 640, 32)])
+                                         (5, 16, 20000, 32), (2, 1, 8, 32), (33, 1536, 640, 32),
+                                         (1, 5, 98304, 128), (2, 24, 60000, 64), (30, 4800, 256, 32)])
 def test_linear4_shapes(M, N, K, group):
     from nanosaur2_web_b200.ops import linear4
     rng = np.random.default_rng(M + N + K)
