@@ -407,28 +407,22 @@ def _invalid(message: str) -> NsaError:
     return NsaError(_lib.NSA_ERR_INVALID_ARGUMENT, message)
 
 
-def _one_device(*ts) -> torch.device:
-    """The CUDA device that all given tensors (None skipped) live on."""
-    dev = None
-    for t in ts:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise _invalid("tensors must live on a CUDA device")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise _invalid(f"tensors live on {dev} and {t.device}: one device is wanted")
-    return dev
+def _native():
+    """The C++ binding of the decode operators (csrc/binding.cpp): a step is a few microseconds of GPU work, and
+    through ctypes a call would cost several times that on the host."""
+    global _native_module
+    if _native_module is None:
+        lib()   # libnsattn.so, or the message that it has to be built
+        try:
+            from . import _native as module
+        except ImportError as e:
+            raise RuntimeError("the Python binding of the decode operators is missing: build it first "
+                               f"(python -m nanosaur2_web_b200.build); this package has no fallback ({e})") from e
+        _native_module = module
+    return _native_module
 
 
-def _launch(dev: torch.device, fn, *args) -> None:
-    """check(fn(*args, stream)) on dev's current stream, with dev current."""
-    if torch.cuda.current_device() == dev.index:
-        check(fn(*args, stream_handle(dev)))
-    else:
-        with torch.cuda.device(dev):
-            check(fn(*args, stream_handle(dev)))
+_native_module = None
 
 
 @dataclass
@@ -442,51 +436,32 @@ class Weight4:
     K: int
     group: int
 
-    def _desc(self) -> "_lib.Weight4Desc":
-        c, s = self.codes, self.scales
-        if self.group not in (32, 64, 128):
-            raise _invalid("group must be 32, 64 or 128")
-        t, k = (self.N + 15) // 16, (self.K + 127) // 128
-        if c.dtype != torch.uint8 or s.dtype != torch.bfloat16 or c.shape != (t, k, 16, 64) or \
-                s.shape != (t, k, 16, 128 // self.group) or not c.is_contiguous() or not s.is_contiguous():
-            raise _invalid(f"a {self.group}-group weight [{self.N}, {self.K}] has contiguous codes uint8 [{t}, {k}, 16, 64] "
-                           f"and scales bfloat16 [{t}, {k}, 16, {128 // self.group}]")
-        return _lib.Weight4Desc(self.N, self.K, self.group, c.data_ptr(), s.data_ptr())
-
 
 def quantize4(W: torch.Tensor, group: int = 32, out: Optional[Weight4] = None) -> Weight4:
     """W [N, K] fp32 or bf16 (unit inner stride) -> its 4-bit form with a scale per ``group`` (32, 64 or 128)
     values along K: per group the smallest five-bit scale >= max|w| / 7, codes rounded to nearest, ties to
     even.  Made once, at load time (nsa_quantize4); ``out`` of the same N, K and group is overwritten."""
-    if W.dim() != 2 or W.stride(1) != 1 or W.shape[0] < 1 or W.shape[1] < 1:
+    if W.dim() != 2 or not W.numel():
         raise _invalid("W must be a non-empty [N, K] tensor with unit inner stride")
     N, K = W.shape
     if group not in (32, 64, 128):
         raise _invalid("group must be 32, 64 or 128")
     if out is None:
-        dev = _one_device(W)
         t, k = (N + 15) // 16, (K + 127) // 128
-        out = Weight4(torch.empty((t, k, 16, 64), dtype=torch.uint8, device=dev),
-                      torch.empty((t, k, 16, 128 // group), dtype=torch.bfloat16, device=dev), N, K, group)
+        out = Weight4(W.new_empty((t, k, 16, 64), dtype=torch.uint8),
+                      W.new_empty((t, k, 16, 128 // group), dtype=torch.bfloat16), N, K, group)
     elif (out.N, out.K, out.group) != (N, K, group):
         raise _invalid(f"out is [{out.N}, {out.K}] in groups of {out.group}, W [{N}, {K}] in groups of {group}")
-    dev = _one_device(W, out.codes, out.scales)
-    d = out._desc()
-    _launch(dev, lib().nsa_quantize4, ctypes.byref(d), W.data_ptr(), dtype_code(W), max(W.stride(0), K))
+    _native().quantize4(W, out.codes, out.scales, group)
     return out
 
 
 def expand4(W: Weight4, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """A 4-bit weight's values as bf16 [N, K] (nsa_expand4; exact for ``quantize4``'s scales): the weight
     ``linear`` takes when a prompt brings many rows."""
-    dev = _one_device(W.codes, W.scales, out)
     if out is None:
-        out = torch.empty((W.N, W.K), dtype=torch.bfloat16, device=dev)
-    if out.dtype != torch.bfloat16 or tuple(out.shape) != (W.N, W.K) or out.stride(1) != 1 or \
-            (W.N > 1 and out.stride(0) < W.K):
-        raise _invalid("out must be a bfloat16 [N, K] tensor with unit inner stride")
-    d = W._desc()
-    _launch(dev, lib().nsa_expand4, ctypes.byref(d), out.data_ptr(), max(out.stride(0), W.K))
+        out = W.scales.new_empty((W.N, W.K))
+    _native().expand4(W.codes, W.scales, W.N, W.K, W.group, out)
     return out
 
 
@@ -497,25 +472,7 @@ def linear4(x: torch.Tensor, W: Weight4, *, bias: Optional[torch.Tensor] = None,
     float32 or (store form) bfloat16 with unit inner stride, allocated (``out_dtype``, default float32) when not
     given.  Products are exact and sums in fp32.  Any M runs; the weight is read once per 32 rows, so for
     hundreds of rows ``linear`` over ``expand4(W)`` is faster."""
-    dev = _one_device(x, W.codes, W.scales, bias, out)
-    if x.dim() != 2 or x.dtype != torch.bfloat16 or x.shape[1] != W.K or x.stride(1) != 1:
-        raise _invalid(f"x must be [M, {W.K}] bf16 with unit inner stride")
-    M = x.shape[0]
-    if bias is not None and (bias.dtype != torch.float32 or bias.shape != (W.N,) or not bias.is_contiguous()):
-        raise _invalid(f"bias must be a contiguous float32 [{W.N}] tensor")
-    if out is None:
-        if resid:
-            raise _invalid("resid needs out")
-        out = torch.empty((M, W.N), dtype=out_dtype or torch.float32, device=dev)
-    elif out.dim() != 2 or out.shape[0] != M or out.shape[1] != W.N or (W.N > 1 and out.stride(1) != 1):
-        raise _invalid(f"out must be [{M}, {W.N}] with unit inner stride")
-    if M > 1 and (x.stride(0) < W.K or out.stride(0) < W.N):
-        raise _invalid("the rows of x and out must not overlap")
-    w = W._desc()
-    d = _lib.Linear4Desc(M, x.stride(0) if M > 1 else W.K, out.stride(0) if M > 1 else W.N, int(bool(resid)),
-                         dtype_code(out))
-    _launch(dev, lib().nsa_linear4, ctypes.byref(d), ctypes.byref(w), x.data_ptr(), _ptr(bias), out.data_ptr())
-    return out
+    return _native().linear4(x, W.codes, W.scales, W.N, W.K, W.group, bias, out, resid, out_dtype)
 
 
 @dataclass
@@ -539,14 +496,6 @@ class Kv4Cache:
     def D(self) -> int:
         return 2 * self.codes.shape[4]
 
-    def _desc(self) -> "_lib.Kv4CacheDesc":
-        c, s = self.codes, self.scales
-        if c.dim() != 5 or c.dtype != torch.uint8 or s.dtype != torch.bfloat16 or c.shape[1] != 2 or \
-                s.shape != c.shape[:4] + (c.shape[4] // 16,) or not c.is_contiguous() or not s.is_contiguous():
-            raise _invalid("the cache has contiguous codes uint8 [n_pages, 2, Hkv, P, D/2] and scales bfloat16 "
-                           "[n_pages, 2, Hkv, P, D/32]")
-        return _lib.Kv4CacheDesc(c.shape[0], c.shape[3], c.shape[2], 2 * c.shape[4], c.data_ptr(), s.data_ptr())
-
 
 def kv4_cache(n_pages: int, Hkv: int, D: int, page: int = 64, device=None) -> Kv4Cache:
     """An empty pool of ``n_pages`` pages of ``page`` tokens (a multiple of 16, at most 1024) for Hkv heads of
@@ -560,31 +509,6 @@ def kv4_cache(n_pages: int, Hkv: int, D: int, page: int = 64, device=None) -> Kv
                     torch.empty((n_pages, 2, Hkv, page, D // 32), dtype=torch.bfloat16, device=device))
 
 
-def _kv4_batch(B: int, L: int, table: torch.Tensor, start: torch.Tensor, count: Optional[torch.Tensor]):
-    if table.dim() != 2 or table.dtype != torch.int32 or table.shape[0] != B or (table.shape[1] > 1 and table.stride(1) != 1):
-        raise _invalid(f"table must be an int32 [{B}, max_pages] tensor with unit inner stride")
-    for t, name in ((start, "start"), (count, "count")):
-        if t is not None and (t.dtype != torch.int32 or t.shape != (B,) or (B > 1 and t.stride(0) != 1)):
-            raise _invalid(f"{name} must be a contiguous int32 [{B}] tensor")
-    if B > 1 and table.stride(0) < table.shape[1]:
-        table = table.contiguous()   # a broadcast table (every sequence on the same pages)
-    return _lib.Kv4Batch(B, L, table.shape[1], max(table.stride(0), table.shape[1]), table.data_ptr(), start.data_ptr(),
-                         _ptr(count)), table
-
-
-def _rows3(t: torch.Tensor, name: str, width: Optional[int] = None, dtype: Optional[torch.dtype] = None) -> None:
-    if t.dim() != 3 or (t.shape[2] > 1 and t.stride(2) != 1) or (width is not None and t.shape[2] != width) or \
-            (dtype is not None and t.dtype != dtype):
-        raise _invalid(f"{name} must be [B, L, {width or 'columns'}]{'' if dtype is None else ' ' + str(dtype)} with unit "
-                       "inner stride")
-
-
-def _pitches(t: torch.Tensor):
-    """Row and batch pitches of a [B, L, columns] tensor, those of axes of length 1 as if it were contiguous."""
-    ld = t.stride(1) if t.shape[1] > 1 else t.shape[2]
-    return ld, t.stride(0) if t.shape[0] > 1 else t.shape[1] * ld
-
-
 def kv4_append(qkv: torch.Tensor, cache: Kv4Cache, table: torch.Tensor, start: torch.Tensor, *, Hq: int,
                q_norm: torch.Tensor, k_norm: torch.Tensor, cs: Optional[RopeTable], count: Optional[torch.Tensor] = None,
                eps: float = 1e-6, qOff: int = 0, kOff: Optional[int] = None, vOff: Optional[int] = None,
@@ -595,35 +519,9 @@ def kv4_append(qkv: torch.Tensor, cache: Kv4Cache, table: torch.Tensor, start: t
     position (``cs``, None for no rotation); k and v are stored in 4 bits in the pages of ``table``, and q comes back
     as bf16 [B, L, Hq*D] (``out``), ``kv4_attention``'s operand.  start and count are device int32 [B]; rows past
     count[b] are neither read nor written."""
-    dev = _one_device(qkv, cache.codes, cache.scales, table, start, count, q_norm, k_norm, out,
-                      None if cs is None else cs.buf)
-    c = cache._desc()
-    D = c.D
-    _rows3(qkv, "qkv")
-    B, L, cols = qkv.shape
-    kOff = qOff + Hq * D if kOff is None else kOff
-    vOff = kOff + c.Hkv * D if vOff is None else vOff
-    if Hq < 1 or min(qOff, kOff, vOff) < 0 or max(qOff + Hq * D, kOff + c.Hkv * D, vOff + c.Hkv * D) > cols:
-        raise _invalid("the q, k and v heads must lie inside qkv's columns")
-    for w in (q_norm, k_norm):
-        if w.dtype != torch.float32 or w.shape != (D,) or not w.is_contiguous():
-            raise _invalid(f"q_norm and k_norm must be contiguous float32 [{D}] tensors")
-    if cs is not None and (cs.D != D or cs.buf.dtype != torch.float32 or not cs.buf.is_contiguous() or
-                           cs.L * (D // 2) > cs.buf.numel() - cs.sinOff or cs.L * (D // 2) > cs.buf.numel()):
-        raise _invalid(f"cs must be a float32 table of head dim {D}")
-    if out is None:
-        out = torch.empty((B, L, Hq * D), dtype=torch.bfloat16, device=dev)
-    _rows3(out, "out", Hq * D, torch.bfloat16)
-    if out.shape[:2] != qkv.shape[:2]:
-        raise _invalid("out must have qkv's B and L")
-    batch, table = _kv4_batch(B, L, table, start, count)
-    ld, bs = _pitches(qkv)
-    old, obs = _pitches(out)
-    d = _lib.Kv4AppendDesc(Hq, dtype_code(qkv), ld, bs, qOff, kOff, vOff, old, obs, 0 if cs is None else cs.sinOff,
-                           0 if cs is None else cs.L, eps)
-    _launch(dev, lib().nsa_kv4_append, ctypes.byref(d), ctypes.byref(c), ctypes.byref(batch), qkv.data_ptr(),
-            q_norm.data_ptr(), k_norm.data_ptr(), None if cs is None else cs.buf.data_ptr(), out.data_ptr())
-    return out
+    buf, rows, dim, sin_off = (None, 0, 0, 0) if cs is None else (cs.buf, cs.L, cs.D, cs.sinOff)
+    return _native().kv4_append(qkv, cache.codes, cache.scales, table, start, count, Hq, q_norm, k_norm, buf, rows, dim,
+                                sin_off, eps, qOff, kOff, vOff, out)
 
 
 def kv4_read(cache: Kv4Cache, table: torch.Tensor, start: torch.Tensor, L: int, *, count: Optional[torch.Tensor] = None,
@@ -631,20 +529,7 @@ def kv4_read(cache: Kv4Cache, table: torch.Tensor, start: torch.Tensor, L: int, 
     """Positions start[b] .. start[b] + L - 1 of every sequence back as bf16 rows [B, L, 2*Hkv*D], key heads then
     value heads (nsa_kv4_read; exact): what ``attention`` takes as k and v.  Rows past count[b] are left as they
     were (zeros when ``out`` is not given)."""
-    dev = _one_device(cache.codes, cache.scales, table, start, count, out)
-    c = cache._desc()
-    B, width = table.shape[0], 2 * c.Hkv * c.D
-    if L < 0:
-        raise _invalid("L must be >= 0")
-    if out is None:
-        out = torch.zeros((B, L, width), dtype=torch.bfloat16, device=dev)
-    _rows3(out, "out", width, torch.bfloat16)
-    if out.shape[:2] != (B, L):
-        raise _invalid(f"out must be [{B}, {L}, {width}]")
-    batch, table = _kv4_batch(B, L, table, start, count)
-    ld, bs = _pitches(out)
-    _launch(dev, lib().nsa_kv4_read, ctypes.byref(c), ctypes.byref(batch), out.data_ptr(), ld, bs)
-    return out
+    return _native().kv4_read(cache.codes, cache.scales, table, start, L, count, out)
 
 
 def kv4_attention(q: torch.Tensor, cache: Kv4Cache, table: torch.Tensor, start: torch.Tensor, *,
@@ -657,27 +542,4 @@ def kv4_attention(q: torch.Tensor, cache: Kv4Cache, table: torch.Tensor, start: 
     were (``out`` not given: uninitialised).  scale 0 means 1/sqrt(D).  ``workspace``: a uint8 tensor to
     reuse, as large as the C call asks (nsa_kv4_attention_workspace_size; the error names the size), allocated per
     call when not given; calls that overlap on the GPU need one each."""
-    dev = _one_device(q, cache.codes, cache.scales, table, start, count, out, workspace)
-    c = cache._desc()
-    _rows3(q, "q", None, torch.bfloat16)
-    B, L, width = q.shape
-    if width % c.D or width < c.D:
-        raise _invalid(f"q must have whole heads of {c.D}")
-    if out is None:
-        out = torch.empty((B, L, width), dtype=torch.bfloat16, device=dev)
-    _rows3(out, "out", width, torch.bfloat16)
-    if out.shape != q.shape:
-        raise _invalid("out must have q's shape")
-    batch, table = _kv4_batch(B, L, table, start, count)
-    qld, qbs = _pitches(q)
-    old, obs = _pitches(out)
-    d = _lib.Kv4AttentionDesc(width // c.D, qld, qbs, old, obs, window, sinks, scale)
-    fn = lib()
-    need = fn.nsa_kv4_attention_workspace_size(ctypes.byref(d), ctypes.byref(c), ctypes.byref(batch))
-    if workspace is None and need:
-        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-    if workspace is not None and (workspace.dtype != torch.uint8 or not workspace.is_contiguous()):
-        raise _invalid("workspace must be a contiguous uint8 tensor")
-    _launch(dev, fn.nsa_kv4_attention, ctypes.byref(d), ctypes.byref(c), ctypes.byref(batch), q.data_ptr(),
-            out.data_ptr(), _ptr(workspace), 0 if workspace is None else workspace.numel())
-    return out
+    return _native().kv4_attention(q, cache.codes, cache.scales, table, start, count, window, sinks, scale, out, workspace)
