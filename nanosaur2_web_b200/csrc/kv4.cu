@@ -46,179 +46,153 @@ __device__ __forceinline__ int new_tokens(const Kv4Params& p, int b) {
   return p.count ? min(max(p.count[b], 0), p.L) : p.L;
 }
 
-// N (1, 2 or 4) consecutive inputs.
-template <int N>
-__device__ __forceinline__ void load_n(const float* src, float* x) {
-  if constexpr (N == 4) {
-    const float4 v = *reinterpret_cast<const float4*>(src);
-    x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
-  } else if constexpr (N == 2) {
-    const float2 v = *reinterpret_cast<const float2*>(src);
-    x[0] = v.x; x[1] = v.y;
-  } else {
-    x[0] = *src;
-  }
+// Four consecutive inputs.
+__device__ __forceinline__ void load4(const float* src, float* x) {
+  const float4 v = __ldg(reinterpret_cast<const float4*>(src));
+  x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
 }
-template <int N>
-__device__ __forceinline__ void load_n(const __nv_bfloat16* src, float* x) {
-  if constexpr (N == 4) {
-    const uint2 v = *reinterpret_cast<const uint2*>(src);
-    x[0] = __uint_as_float(v.x << 16); x[1] = __uint_as_float(v.x & 0xFFFF0000u);
-    x[2] = __uint_as_float(v.y << 16); x[3] = __uint_as_float(v.y & 0xFFFF0000u);
-  } else if constexpr (N == 2) {
-    const uint32_t v = *reinterpret_cast<const uint32_t*>(src);
-    x[0] = __uint_as_float(v << 16); x[1] = __uint_as_float(v & 0xFFFF0000u);
-  } else {
-    x[0] = __bfloat162float(*src);
-  }
+__device__ __forceinline__ void load4(const __nv_bfloat16* src, float* x) {
+  const uint2 v = __ldg(reinterpret_cast<const uint2*>(src));
+  x[0] = __uint_as_float(v.x << 16); x[1] = __uint_as_float(v.x & 0xFFFF0000u);
+  x[2] = __uint_as_float(v.y << 16); x[3] = __uint_as_float(v.y & 0xFFFF0000u);
 }
 
-template <typename T>
-__device__ __forceinline__ T warp_sum_t(T v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-
-// RMSNorm times w and the rotation of pairs (i, i + D/2) of one head held by a warp: a[j], b[j] are
-// elements i = lane * HN + j and D/2 + i.
-template <typename T, int HN>
-__device__ __forceinline__ void norm_rope(T* a, T* b, const Kv4AppendParams& p, const float* w, int pos, int lane) {
-  constexpr int half = 32 * HN;
+// RMSNorm and rotation of one head held by LANES lanes: x[0..3] are elements 4 hl .. of the first half, x[4..7] their
+// partners in the second; w the weights alike; c, s the cosines and sines of the four pairs.
+template <typename T, int LANES>
+__device__ __forceinline__ void norm_rope(const float* x, const float* w, const float* c, const float* s, bool rope, float eps,
+                                          T* out) {
   T ss = 0;
 #pragma unroll
-  for (int j = 0; j < HN; ++j) ss += a[j] * a[j] + b[j] * b[j];
-  ss = warp_sum_t(ss);
+  for (int e = 0; e < 8; ++e) ss += (T)x[e] * (T)x[e];
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
   T r;
   if constexpr (sizeof(T) == 8)
-    r = 1.0 / sqrt(ss / (2 * half) + (double)p.eps);
+    r = rsqrt(ss * (1.0 / (8 * LANES)) + (double)eps);
   else
-    r = rsqrtf(ss / (float)(2 * half) + p.eps);
-  float wa[HN], wb[HN], c[HN], s[HN];
-  load_n<HN>(w + lane * HN, wa);
-  load_n<HN>(w + half + lane * HN, wb);
-  if (p.cs) {
-    load_n<HN>(p.cs + (int64_t)pos * half + lane * HN, c);
-    load_n<HN>(p.cs + p.sin_off + (int64_t)pos * half + lane * HN, s);
-  }
+    r = rsqrtf(ss * (1.f / (8 * LANES)) + eps);
 #pragma unroll
-  for (int j = 0; j < HN; ++j) {
-    const T y1 = a[j] * r * (T)wa[j], y2 = b[j] * r * (T)wb[j];
-    a[j] = p.cs ? y1 * (T)c[j] - y2 * (T)s[j] : y1;
-    b[j] = p.cs ? y2 * (T)c[j] + y1 * (T)s[j] : y2;
+  for (int e = 0; e < 8; ++e) out[e] = (T)x[e] * r * (T)w[e];
+  if (rope) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const T a = out[e], b = out[4 + e];
+      out[e] = a * (T)c[e] - b * (T)s[e];
+      out[4 + e] = b * (T)c[e] + a * (T)s[e];
+    }
   }
 }
 
-// HN consecutive elements per lane, one half of a head: scale over the 32 / HN lanes of a group, codes
-// packed into bytes and stored at dst (this half's codes), scales at sc.
-template <typename T, int HN>
-__device__ __forceinline__ void store_half(const T* x, uint8_t* dst, __nv_bfloat16* sc, int lane) {
-  T am = 0;
+// A lane's four values of each half of a head's row of the cache (the group of 32 is eight lanes): even lanes store the
+// pair's word of the first half, odd lanes that of the second.
+template <bool SHORT, typename T>
+__device__ __forceinline__ void store_codes(const T* x, uint8_t* codes, __nv_bfloat16* scales, int hl, int half, bool live) {
+  float s[2];
+  uint32_t bits[2];
 #pragma unroll
-  for (int j = 0; j < HN; ++j) am = amax2(fabs(x[j]), am);
+  for (int k = 0; k < 2; ++k) {
+    T am = 0;
 #pragma unroll
-  for (int o = 1; o < 32 / HN; o <<= 1) am = amax2(__shfl_xor_sync(0xffffffffu, am, o), am);
-  const float s = q4_scale(am);
-  uint32_t bits = 0x8888u >> (16 - 4 * HN);
-  if (s > 0.f) {
-    const T inv = (T)1 / (T)s;
-    bits = 0;
+    for (int e = 0; e < 4; ++e) am = amax2((T)fabs(x[4 * k + e]), am);
 #pragma unroll
-    for (int j = 0; j < HN; ++j) bits |= q4_code(x[j], (T)s, inv) << (4 * j);
+    for (int o = 1; o < 8; o <<= 1) am = amax2(__shfl_xor_sync(0xffffffffu, am, o), am);
+    s[k] = q4_scale(am);
+    bits[k] = s[k] > 0.f ? q4_bits<4, q4_in_order, SHORT>(x + 4 * k, s[k], am) : 0x8888u;
   }
-  if constexpr (HN == 4) {
-    reinterpret_cast<uint16_t*>(dst)[lane] = (uint16_t)bits;
-  } else if constexpr (HN == 2) {
-    dst[lane] = (uint8_t)bits;
-  } else {
-    const uint32_t up = __shfl_down_sync(0xffffffffu, bits, 1);
-    if (lane % 2 == 0) dst[lane / 2] = (uint8_t)(bits | (up << 4));
-  }
-  if (lane % (32 / HN) == 0) sc[lane / (32 / HN)] = __float2bfloat16_rn(s);
+  const bool odd = hl & 1;
+  const uint32_t got = __shfl_xor_sync(0xffffffffu, odd ? bits[0] : bits[1], 1);
+  if (!live) return;
+  const uint32_t word = odd ? got | (bits[1] << 16) : bits[0] | (got << 16);
+  *reinterpret_cast<uint32_t*>(codes + (odd ? half / 2 : 0) + hl / 2 * 4) = word;
+  if (hl % 8 < 2) scales[(odd ? half / kKvGroup : 0) + hl / 8] = __float2bfloat16_rn(odd ? s[1] : s[0]);
 }
 
-// One warp per (token, head) of q | k | v.  Keys are computed in fp64: the code of a value next to the
-// border of two codes is decided by the last bits, and the fp32 order of sums would decide it by chance.
-template <typename T, int HN>
-__global__ void __launch_bounds__(256) kv4_append_kernel(const Kv4AppendParams p) {
-  constexpr int D = 64 * HN, half = D / 2;
+// A CTA per token; a warp takes 256 / D heads of one kind (q, k or v) at a time, eight values a lane.  Bound by the
+// bytes of q | k | v.  Keys are computed in fp64: the code of a value next to the border of two codes is
+// decided by the last bits, and the fp32 order of sums would decide it by chance.
+template <typename T, int D>
+__global__ void __launch_bounds__(256, 3) kv4_append_kernel(const Kv4AppendParams p) {
+  constexpr int LANES = D / 8, HPW = 32 / LANES, half = D / 2;
   const Kv4Params& kv = p.kv;
-  const int lane = threadIdx.x % 32;
-  const int heads = p.Hq + 2 * kv.Hkv;
-  const int64_t unit = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
-  if (unit >= (int64_t)kv.B * kv.L * heads) return;
-  const int h = (int)(unit % heads);
-  const int64_t row = unit / heads;
-  const int b = (int)(row / kv.L), i = (int)(row % kv.L);
+  const int lane = threadIdx.x % 32, hl = lane % LANES;
+  const int q_slots = (p.Hq + HPW - 1) / HPW, kv_slots = (kv.Hkv + HPW - 1) / HPW;
+  const int b = blockIdx.x / kv.L, i = blockIdx.x % kv.L;
   if (i >= new_tokens(kv, b)) return;
   const int pos = position(kv, b, i);
   if (pos < 0) return;
   if (p.cs && pos >= p.rope_rows) {
-    if (lane == 0) atomicCAS(kv.err, 0, kErrKvPosition);
+    if (threadIdx.x == 0) atomicCAS(kv.err, 0, kErrKvPosition);
     return;
   }
-  const bool is_q = h < p.Hq, is_k = !is_q && h < p.Hq + kv.Hkv;
-  const int hh = is_q ? h : (is_k ? h - p.Hq : h - p.Hq - kv.Hkv);
-  const int64_t off = is_q ? p.q_off : (is_k ? p.k_off : p.v_off);
-  const T* src = static_cast<const T*>(p.qkv) + b * p.bstride + i * p.ld + off + (int64_t)hh * D;
-  float a[HN], c[HN];
-  load_n<HN>(src + lane * HN, a);
-  load_n<HN>(src + half + lane * HN, c);
-  if (is_q) {
-    norm_rope<float, HN>(a, c, p, p.q_w, pos, lane);
-    __nv_bfloat16* dst = p.q_out + b * p.qo_bstride + i * p.qo_ld + (int64_t)hh * D;
-#pragma unroll
-    for (int j = 0; j < HN; ++j) {
-      dst[lane * HN + j] = __float2bfloat16_rn(a[j]);
-      dst[half + lane * HN + j] = __float2bfloat16_rn(c[j]);
+  const T* row = static_cast<const T*>(p.qkv) + b * p.bstride + i * p.ld;
+  for (int slot = threadIdx.x / 32; slot < q_slots + 2 * kv_slots; slot += blockDim.x / 32) {
+    const int kind = slot < q_slots ? 0 : slot < q_slots + kv_slots ? 1 : 2;
+    const int heads = kind == 0 ? p.Hq : kv.Hkv;
+    const int h = (kind == 0 ? slot : slot - q_slots - (kind - 1) * kv_slots) * HPW + lane / LANES;
+    const bool live = h < heads;                                   // lanes past the last head repeat it, storing nothing
+    const int hh = live ? h : heads - 1;
+    const T* src = row + (kind == 0 ? p.q_off : kind == 1 ? p.k_off : p.v_off) + (int64_t)hh * D + hl * 4;
+    float x[8], w[8], c[4], s[4];
+    load4(src, x);
+    load4(src + half, x + 4);
+    if (kind < 2) {
+      const float* wt = (kind == 0 ? p.q_w : p.k_w) + hl * 4;
+      load4(wt, w);
+      load4(wt + half, w + 4);
+      if (p.cs) {
+        const float* t = p.cs + (int64_t)pos * half + hl * 4;
+        load4(t, c);
+        load4(t + p.sin_off, s);
+      }
     }
-    return;
-  }
-  const int page = page_of(kv, b, pos);
-  if (page < 0) return;
-  const int64_t tok = cache_row(kv, page, is_k ? 0 : 1, hh, pos);
-  uint8_t* codes = kv.codes + tok * (D / 2);
-  __nv_bfloat16* scales = kv.scales + tok * (D / kKvGroup);
-  if (is_k) {
-    double ad[HN], cd[HN];
-#pragma unroll
-    for (int j = 0; j < HN; ++j) ad[j] = a[j], cd[j] = c[j];
-    norm_rope<double, HN>(ad, cd, p, p.k_w, pos, lane);
-    store_half<double, HN>(ad, codes, scales, lane);
-    store_half<double, HN>(cd, codes + half / 2, scales + half / kKvGroup, lane);
-  } else {
-    store_half<float, HN>(a, codes, scales, lane);
-    store_half<float, HN>(c, codes + half / 2, scales + half / kKvGroup, lane);
+    if (kind == 0) {
+      float o[8];
+      norm_rope<float, LANES>(x, w, c, s, p.cs != nullptr, p.eps, o);
+      if (live) {
+        __nv_bfloat16* dst = p.q_out + b * p.qo_bstride + i * p.qo_ld + (int64_t)hh * D + hl * 4;
+        *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]));
+        *reinterpret_cast<uint2*>(dst + half) = make_uint2(pack_bf16x2(o[4], o[5]), pack_bf16x2(o[6], o[7]));
+      }
+      continue;
+    }
+    const int page = page_of(kv, b, pos);
+    if (page < 0) return;
+    const int64_t tok = cache_row(kv, page, kind - 1, hh, pos);
+    uint8_t* codes = kv.codes + tok * (D / 2);
+    __nv_bfloat16* scales = kv.scales + tok * (D / kKvGroup);
+    if (kind == 1) {
+      double o[8];
+      norm_rope<double, LANES>(x, w, c, s, p.cs != nullptr, p.eps, o);
+      store_codes<false>(o, codes, scales, hl, half, live);
+    } else {
+      store_codes<sizeof(T) == 2>(x, codes, scales, hl, half, live);
+    }
   }
 }
 
-// One thread per word (8 values) of a read-back row.
+// A CTA per row, a thread per word (8 values).
 __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4Params p, __nv_bfloat16* __restrict__ out, int64_t ldo,
                                                        int64_t bstride) {
-  const int words = p.D / 8;
-  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int w = (int)(idx % words);
-  int64_t r = idx / words;
-  const int h = (int)(r % p.Hkv);
-  r /= p.Hkv;
-  const int which = (int)(r % 2);
-  r /= 2;
-  const int i = (int)(r % p.L);
-  const int64_t b = r / p.L;
-  if (b >= p.B || i >= new_tokens(p, (int)b)) return;
-  const int pos = position(p, (int)b, i);
+  const int b = blockIdx.x / p.L, i = blockIdx.x % p.L;
+  if (i >= new_tokens(p, b)) return;
+  const int pos = position(p, b, i);
   if (pos < 0) return;
-  const int page = page_of(p, (int)b, pos);
+  const int page = page_of(p, b, pos);
   if (page < 0) return;
-  const int64_t tok = cache_row(p, page, which, h, pos);
-  const uint32_t v = reinterpret_cast<const uint32_t*>(p.codes + tok * (p.D / 2))[w];
-  const float s = __bfloat162float(p.scales[tok * (p.D / kKvGroup) + w * 8 / kKvGroup]);
-  uint4 o;
-  o.x = pack_bf16x2(q4_value(v, 0, s), q4_value(v, 1, s));
-  o.y = pack_bf16x2(q4_value(v, 2, s), q4_value(v, 3, s));
-  o.z = pack_bf16x2(q4_value(v, 4, s), q4_value(v, 5, s));
-  o.w = pack_bf16x2(q4_value(v, 6, s), q4_value(v, 7, s));
-  reinterpret_cast<uint4*>(out + b * bstride + i * ldo + ((int64_t)which * p.Hkv + h) * p.D)[w] = o;
+  const int words = p.D / 8;
+  for (int e = threadIdx.x; e < 2 * p.Hkv * words; e += blockDim.x) {
+    const int w = e % words, h = e / words;                        // h: key heads, then value heads
+    const int64_t tok = cache_row(p, page, 0, h, pos);             // heads of both halves follow one another
+    const uint32_t v = __ldg(reinterpret_cast<const uint32_t*>(p.codes + tok * (p.D / 2)) + w);
+    const float s = __bfloat162float(p.scales[tok * (p.D / kKvGroup) + w * 8 / kKvGroup]);
+    uint4 o;
+    o.x = pack_bf16x2(q4_value(v, 0, s), q4_value(v, 1, s));
+    o.y = pack_bf16x2(q4_value(v, 2, s), q4_value(v, 3, s));
+    o.z = pack_bf16x2(q4_value(v, 4, s), q4_value(v, 5, s));
+    o.w = pack_bf16x2(q4_value(v, 6, s), q4_value(v, 7, s));
+    reinterpret_cast<uint4*>(out + b * bstride + i * ldo)[e] = o;
+  }
 }
 
 // ------------------------------------------------------------------------------------ attention
@@ -621,11 +595,14 @@ __global__ void kv4_join_kernel(const Kv4AttnParams p) {
 }
 
 template <typename T>
-cudaError_t launch_append_t(const Kv4AppendParams& p, unsigned blocks, cudaStream_t stream) {
+cudaError_t launch_append_t(const Kv4AppendParams& p, unsigned rows, cudaStream_t stream) {
+  const int hpw = 256 / p.kv.D;
+  const int slots = (p.Hq + hpw - 1) / hpw + 2 * ((p.kv.Hkv + hpw - 1) / hpw);
+  const int threads = 32 * std::min(slots, 8);
   switch (p.kv.D) {
-    case 64: kv4_append_kernel<T, 1><<<blocks, 256, 0, stream>>>(p); break;
-    case 128: kv4_append_kernel<T, 2><<<blocks, 256, 0, stream>>>(p); break;
-    case 256: kv4_append_kernel<T, 4><<<blocks, 256, 0, stream>>>(p); break;
+    case 64: kv4_append_kernel<T, 64><<<rows, threads, 0, stream>>>(p); break;
+    case 128: kv4_append_kernel<T, 128><<<rows, threads, 0, stream>>>(p); break;
+    case 256: kv4_append_kernel<T, 256><<<rows, threads, 0, stream>>>(p); break;
     default: return cudaErrorInvalidValue;
   }
   return cudaGetLastError();
@@ -634,16 +611,17 @@ cudaError_t launch_append_t(const Kv4AppendParams& p, unsigned blocks, cudaStrea
 }  // namespace
 
 cudaError_t launch_kv4_append(const Kv4AppendParams& p, cudaStream_t stream) {
-  const int64_t blocks = ((int64_t)p.kv.B * p.kv.L * (p.Hq + 2 * p.kv.Hkv) + 7) / 8;
-  if (blocks > 0x7FFFFFFFLL) return cudaErrorInvalidValue;
-  return p.in_f32 ? launch_append_t<float>(p, (unsigned)blocks, stream)
-                  : launch_append_t<__nv_bfloat16>(p, (unsigned)blocks, stream);
+  const int64_t rows = (int64_t)p.kv.B * p.kv.L;
+  if (rows > 0x7FFFFFFFLL) return cudaErrorInvalidValue;
+  return p.in_f32 ? launch_append_t<float>(p, (unsigned)rows, stream)
+                  : launch_append_t<__nv_bfloat16>(p, (unsigned)rows, stream);
 }
 
 cudaError_t launch_kv4_read(const Kv4Params& p, __nv_bfloat16* out, int64_t ldo, int64_t bstride, cudaStream_t stream) {
-  const int64_t blocks = ((int64_t)p.B * p.L * 2 * p.Hkv * (p.D / 8) + 255) / 256;
-  if (blocks > 0x7FFFFFFFLL) return cudaErrorInvalidValue;
-  kv4_read_kernel<<<(unsigned)blocks, 256, 0, stream>>>(p, out, ldo, bstride);
+  const int64_t rows = (int64_t)p.B * p.L;
+  if (rows > 0x7FFFFFFFLL) return cudaErrorInvalidValue;
+  const int threads = std::min(256, (2 * p.Hkv * (p.D / 8) + 31) / 32 * 32);
+  kv4_read_kernel<<<(unsigned)rows, threads, 0, stream>>>(p, out, ldo, bstride);
   return cudaGetLastError();
 }
 

@@ -8,6 +8,7 @@
 #include <algorithm>
 
 #include "nsa_internal.h"
+#include "ptx.cuh"
 #include "q4.cuh"
 
 namespace nsa {
@@ -19,59 +20,84 @@ constexpr int kRowTile = 16, kChunk = 128;
 // byte offset of logical word lw (8 values, 0..15) in a row's 64 bytes of a chunk
 __device__ __forceinline__ int word_at(int lw) { return 16 * (lw & 3) + 4 * (lw >> 2); }
 
-template <typename T>
-__device__ __forceinline__ float load1(const void* p, int64_t i);
-template <>
-__device__ __forceinline__ float load1<float>(const void* p, int64_t i) { return static_cast<const float*>(p)[i]; }
-template <>
-__device__ __forceinline__ float load1<__nv_bfloat16>(const void* p, int64_t i) {
-  return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+// Eight values of a row from k on (zeros past K): one or two 16-byte loads where rows are 16-byte aligned.
+template <bool VEC>
+__device__ __forceinline__ void load8(const float* row, int k, int K, float* x) {
+  if (VEC && k + 8 <= K) {
+    const float4 a = __ldg(reinterpret_cast<const float4*>(row + k)), b = __ldg(reinterpret_cast<const float4*>(row + k) + 1);
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = k + e < K ? row[k + e] : 0.f;
+  }
+}
+template <bool VEC>
+__device__ __forceinline__ void load8(const __nv_bfloat16* row, int k, int K, float* x) {
+  if (VEC && k + 8 <= K) {
+    const uint4 v = __ldg(reinterpret_cast<const uint4*>(row + k));
+    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      x[2 * e] = __uint_as_float(u[e] << 16);
+      x[2 * e + 1] = __uint_as_float(u[e] & 0xFFFF0000u);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = k + e < K ? __bfloat162float(row[k + e]) : 0.f;
+  }
 }
 
-// One thread per word (8 values of one row); the 4, 8 or 16 neighbouring threads of a group share its
-// largest magnitude by shuffles.
-template <typename T, int G>
+// One CTA per tile chunk, one thread per word (8 values of one row); the 4, 8 or 16 neighbouring threads of a group
+// share its largest magnitude by shuffles.  Bound by the weight's bytes.
+template <typename T, int G, bool VEC>
 __global__ void __launch_bounds__(256) quantize4_kernel(const Quant4Params p) {
-  const int64_t words = (int64_t)p.Kc * 16;
-  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;   // grid covers Nt * 16 rows x words exactly
-  const int64_t row = idx / words;
-  const int w = (int)(idx % words);
-  if (row >= (int64_t)p.Nt * kRowTile) return;                   // whole warps: words is a multiple of 16 and rows of 16
+  const int tile = blockIdx.x / p.Kc, ch = blockIdx.x % p.Kc;
+  const int r = threadIdx.x / 16, w = threadIdx.x % 16;
+  const int64_t row = (int64_t)tile * kRowTile + r;
   float x[8];
+  if (row < p.N) {
+    load8<VEC>(static_cast<const T*>(p.w) + row * p.ldw, ch * kChunk + w * 8, p.K, x);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = 0.f;
+  }
   float am = 0.f;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const int k = w * 8 + e;
-    x[e] = (row < p.N && k < p.K) ? load1<T>(p.w, row * p.ldw + k) : 0.f;
-    am = amax2(fabsf(x[e]), am);
-  }
+  for (int e = 0; e < 8; ++e) am = amax2(fabsf(x[e]), am);
 #pragma unroll
   for (int o = 1; o < G / 8; o <<= 1) am = amax2(__shfl_xor_sync(0xffffffffu, am, o), am);
   const float s = q4_scale(am);
-  uint32_t out = 0x88888888u;
-  if (s > 0.f) {
-    const float inv = __fdiv_rn(1.f, s);
-    out = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) out |= q4_code(x[e], s, inv) << (4 * q4_nibble(e));
-  }
-  const int64_t tr = ((row / kRowTile) * p.Kc + w / 16) * kRowTile + row % kRowTile;   // row of the tiled order
-  *reinterpret_cast<uint32_t*>(p.codes + tr * 64 + word_at(w % 16)) = out;
-  if (w % (G / 8) == 0) p.scales[tr * (kChunk / G) + (w % 16) / (G / 8)] = __float2bfloat16_rn(s);
+  const uint32_t out = s > 0.f ? q4_bits<8, q4_nibble, sizeof(T) == 2>(x, s, am) : 0x88888888u;
+  const int64_t tr = (int64_t)blockIdx.x * kRowTile + r;   // row of the tiled order
+  *reinterpret_cast<uint32_t*>(p.codes + tr * 64 + word_at(w)) = out;
+  if (w % (G / 8) == 0) p.scales[tr * (kChunk / G) + w / (G / 8)] = __float2bfloat16_rn(s);
 }
 
+// The same shape backwards: a thread per word, one 16-byte store where the rows of out are 16-byte aligned.
+template <bool VEC>
 __global__ void __launch_bounds__(256) expand4_kernel(const Quant4Params p, __nv_bfloat16* __restrict__ out, int64_t ldo) {
-  const int64_t words = (p.K + 7) / 8;
-  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t row = idx / words;
-  const int w = (int)(idx % words);
-  if (row >= p.N) return;
-  const int64_t tr = ((row / kRowTile) * p.Kc + w / 16) * kRowTile + row % kRowTile;
-  const uint32_t v = *reinterpret_cast<const uint32_t*>(p.codes + tr * 64 + word_at(w % 16));
-  const int per = kChunk / p.G;
-  const float s = __bfloat162float(p.scales[tr * per + (w % 16) * 8 / p.G]);
-  for (int e = 0; e < 8 && w * 8 + e < p.K; ++e)
-    out[row * ldo + w * 8 + e] = __float2bfloat16_rn(q4_value(v, q4_nibble(e), s));
+  const int tile = blockIdx.x / p.Kc, ch = blockIdx.x % p.Kc;
+  const int r = threadIdx.x / 16, w = threadIdx.x % 16;
+  const int64_t row = (int64_t)tile * kRowTile + r;
+  const int k = ch * kChunk + w * 8;
+  if (row >= p.N || k >= p.K) return;
+  const int64_t tr = (int64_t)blockIdx.x * kRowTile + r;
+  const uint32_t v = __ldg(reinterpret_cast<const uint32_t*>(p.codes + tr * 64 + word_at(w)));
+  const float s = __bfloat162float(p.scales[tr * (kChunk / p.G) + w * 8 / p.G]);
+  __nv_bfloat16* dst = out + row * ldo + k;
+  if (VEC && k + 8 <= p.K) {
+    uint4 o;
+    o.x = pack_bf16x2(q4_value(v, q4_nibble(0), s), q4_value(v, q4_nibble(1), s));
+    o.y = pack_bf16x2(q4_value(v, q4_nibble(2), s), q4_value(v, q4_nibble(3), s));
+    o.z = pack_bf16x2(q4_value(v, q4_nibble(4), s), q4_value(v, q4_nibble(5), s));
+    o.w = pack_bf16x2(q4_value(v, q4_nibble(6), s), q4_value(v, q4_nibble(7), s));
+    *reinterpret_cast<uint4*>(dst) = o;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (k + e < p.K) dst[e] = __float2bfloat16_rn(q4_value(v, q4_nibble(e), s));
+  }
 }
 
 // ------------------------------------------------------------------------------------ the linear
@@ -274,14 +300,12 @@ cudaError_t launch_linear_g(const Linear4Params& p, dim3 grid, cudaStream_t stre
   }
 }
 
-template <typename T>
-cudaError_t launch_quantize_t(const Quant4Params& p, cudaStream_t stream) {
-  const int64_t blocks = (int64_t)p.Nt * p.Kc;   // 16 rows x 16 words = 256 threads per tile chunk
-  if (blocks > 0x7FFFFFFFLL) return cudaErrorInvalidValue;
+template <typename T, bool VEC>
+cudaError_t launch_quantize_t(const Quant4Params& p, unsigned blocks, cudaStream_t stream) {
   switch (p.G) {
-    case 32: quantize4_kernel<T, 32><<<(unsigned)blocks, 256, 0, stream>>>(p); break;
-    case 64: quantize4_kernel<T, 64><<<(unsigned)blocks, 256, 0, stream>>>(p); break;
-    default: quantize4_kernel<T, 128><<<(unsigned)blocks, 256, 0, stream>>>(p); break;
+    case 32: quantize4_kernel<T, 32, VEC><<<blocks, 256, 0, stream>>>(p); break;
+    case 64: quantize4_kernel<T, 64, VEC><<<blocks, 256, 0, stream>>>(p); break;
+    default: quantize4_kernel<T, 128, VEC><<<blocks, 256, 0, stream>>>(p); break;
   }
   return cudaGetLastError();
 }
@@ -289,13 +313,21 @@ cudaError_t launch_quantize_t(const Quant4Params& p, cudaStream_t stream) {
 }  // namespace
 
 cudaError_t launch_quantize4(const Quant4Params& p, cudaStream_t stream) {
-  return p.in_f32 ? launch_quantize_t<float>(p, stream) : launch_quantize_t<__nv_bfloat16>(p, stream);
+  const int64_t blocks = (int64_t)p.Nt * p.Kc;
+  if (blocks > 0x7FFFFFFFLL) return cudaErrorInvalidValue;
+  const bool vec = (reinterpret_cast<uintptr_t>(p.w) | (uintptr_t)(p.ldw * (p.in_f32 ? 4 : 2))) % 16 == 0;
+  const unsigned n = (unsigned)blocks;
+  if (p.in_f32) return vec ? launch_quantize_t<float, true>(p, n, stream) : launch_quantize_t<float, false>(p, n, stream);
+  return vec ? launch_quantize_t<__nv_bfloat16, true>(p, n, stream) : launch_quantize_t<__nv_bfloat16, false>(p, n, stream);
 }
 
 cudaError_t launch_expand4(const Quant4Params& p, __nv_bfloat16* out, int64_t ldo, cudaStream_t stream) {
-  const int64_t blocks = ((int64_t)p.N * ((p.K + 7) / 8) + 255) / 256;
+  const int64_t blocks = (int64_t)p.Nt * p.Kc;
   if (blocks > 0x7FFFFFFFLL) return cudaErrorInvalidValue;
-  expand4_kernel<<<(unsigned)blocks, 256, 0, stream>>>(p, out, ldo);
+  if ((reinterpret_cast<uintptr_t>(out) | (uintptr_t)(ldo * 2)) % 16 == 0)
+    expand4_kernel<true><<<(unsigned)blocks, 256, 0, stream>>>(p, out, ldo);
+  else
+    expand4_kernel<false><<<(unsigned)blocks, 256, 0, stream>>>(p, out, ldo);
   return cudaGetLastError();
 }
 

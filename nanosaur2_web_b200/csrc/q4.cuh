@@ -11,10 +11,12 @@
 // and 24 s, the dequantiser's factors, stay finite), and a group holding an infinity or a NaN gets
 // s = NaN: every value of it reads back as NaN.
 //
-// Both roundings are decided exactly.  7 s needs eight bits, so 7 s >= amax is an exact comparison that
-// corrects amax / 7 for its own rounding; and r = 2 x - 2 c s is exact in the type of x for the nearest
-// codes (c s needs eight bits, and r's magnitude is at most about 2 s, near the lowest bit of both), so
-// comparing it with s finds the nearest code and its ties whatever x * (1 / s) rounded to.
+// Both roundings are decided exactly.  7 s needs eight bits, so 7 s >= amax is an exact comparison, whatever
+// amax * (1 / 7) rounded to.  A code is x * inv rounded to an integer, once with inv a little below 1 / s and once a
+// little above: where the two agree, so does x / s; where they differ, x / s is next to k + 1/2.  An input of at
+// most eight bits (bf16) is then exactly k + 1/2, and the even neighbour is the code; for others the remainder
+// x - c s against s / 2 decides, exact because c s needs eight bits and no bit of the remainder, at most about s,
+// lies below the lowest of x and c s.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -24,46 +26,23 @@ namespace nsa {
 
 constexpr int kKvGroup = 32;   // values per scale of the cache, along the head dim
 
-__device__ __forceinline__ float q4_scale(float amax) {
-  if (amax < 0x1p-110f) return 0.f;
-  if (!(amax <= 3.4028235e38f)) return __uint_as_float(0x7FC00000u);
-  amax = fminf(amax, 0x1p120f);
-  const uint32_t lo = __float_as_uint(__fdiv_rn(amax, 7.f)) & 0xFFF80000u;   // four bits after the leading one
-  return 7.f * __uint_as_float(lo) >= amax ? __uint_as_float(lo) : __uint_as_float(lo + 0x00080000u);
+template <typename T>
+__device__ __forceinline__ float q4_scale(T amax) {
+  if (amax < (T)0x1p-110) return 0.f;
+  if (!isfinite(amax)) return __uint_as_float(0x7FC00000u);
+  const T top = amax < (T)0x1p120 ? amax : (T)0x1p120;
+  uint32_t lo = __float_as_uint((float)top * 0.14285715f) & 0xFFF80000u;   // four bits after the leading one
+  if ((T)7 * (T)__uint_as_float(lo) < top) lo += 0x00080000u;
+  if ((T)7 * (T)__uint_as_float(lo) < top) lo += 0x00080000u;
+  return __uint_as_float(lo);
 }
 
-__device__ __forceinline__ float q4_scale(double amax) {
-  if (amax < 0x1p-110) return 0.f;
-  if (!(amax <= 1.7976931348623157e308)) return __uint_as_float(0x7FC00000u);
-  amax = fmin(amax, 0x1p120);
-  const unsigned long long lo = (unsigned long long)__double_as_longlong(amax / 7.0) & 0xFFFF000000000000ull;
-  const double s = __longlong_as_double((long long)lo);
-  return (float)(7.0 * s >= amax ? s : __longlong_as_double((long long)(lo + 0x0001000000000000ull)));
+// Larger of two magnitudes, a NaN kept.
+__device__ __forceinline__ float amax2(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
 }
-
-// Stored code (c + 8) of x for scale s > 0; inv is about 1 / s.
-__device__ __forceinline__ uint32_t q4_code(float x, float s, float inv) {
-  x = fminf(fmaxf(x, -0x1p120f), 0x1p120f);
-  float c = rintf(x * inv);
-  const float r = fmaf(-2.f * c, s, 2.f * x);
-  const bool odd = ((int)c & 1) != 0;
-  if (r > s || (r == s && odd)) c += 1.f;
-  else if (r < -s || (r == -s && odd)) c -= 1.f;
-  return (uint32_t)((int)fminf(fmaxf(c, -7.f), 7.f) + 8);
-}
-
-__device__ __forceinline__ uint32_t q4_code(double x, double s, double inv) {
-  x = fmin(fmax(x, -0x1p120), 0x1p120);
-  double c = rint(x * inv);
-  const double r = fma(-2.0 * c, s, 2.0 * x);
-  const bool odd = ((int)c & 1) != 0;
-  if (r > s || (r == s && odd)) c += 1.0;
-  else if (r < -s || (r == -s && odd)) c -= 1.0;
-  return (uint32_t)((int)fmin(fmax(c, -7.0), 7.0) + 8);
-}
-
-// Largest magnitude of two, keeping a NaN (fmaxf drops it).
-__device__ __forceinline__ float amax2(float a, float b) { return (a >= b || a != a) ? a : b; }
 __device__ __forceinline__ double amax2(double a, double b) { return (a >= b || a != a) ? a : b; }
 
 // Value of nibble p (bits 4p .. 4p+3) of a word times its scale; exact.
@@ -74,6 +53,56 @@ __device__ __forceinline__ float q4_value(uint32_t w, int p, float s) {
 // Weight words: value e (0..7) of a word sits in nibble q4_nibble(e), so that (w >> 4p) & 0x000F000F
 // holds the neighbours 2p and 2p + 1 in its two halves.
 __host__ __device__ constexpr int q4_nibble(int e) { return (e & 1) ? 4 + e / 2 : e / 2; }
+// Cache words: value e in nibble e.
+__host__ __device__ constexpr int q4_in_order(int e) { return e; }
+
+// Rounding by adding 1.5 * 2^23 (fp64: 1.5 * 2^52) + 8: the low bits of the sum then are c + 8.
+__device__ __forceinline__ uint32_t q4_round(float x, float inv) { return __float_as_uint(fmaf(x, inv, 12582920.f)); }
+__device__ __forceinline__ uint32_t q4_round(double x, double inv) {
+  return (uint32_t)__double2loint(fma(x, inv, 6755399441055752.0));
+}
+
+// N (4 or 8) stored codes for scale s > 0, value e in nibble NIBBLE(e).  SHORT: every x has at most eight bits.  The
+// nibbles are gathered by adding the sums' low words times powers of 16; what fp32 sums have above the nibbles adds
+// up to a constant modulo 2^32.
+template <int N, int (*NIBBLE)(int), bool SHORT, typename T>
+__device__ __forceinline__ uint32_t q4_bits(const T* in, float s, T amax) {
+  const float inv = __fdividef(1.f, s);
+  const T lo = (T)inv * (T)(1 - 0x1p-20), hi = (T)inv * (T)(1 + 0x1p-20);
+  constexpr uint32_t above = sizeof(T) == 4 ? 0x4B400000u * (N == 8 ? 0x11111111u : 0x1111u) : 0u;
+  T x[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) x[e] = in[e];
+  if (amax > (T)0x1p120) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) x[e] = x[e] > (T)0x1p120 ? (T)0x1p120 : x[e] < (T)-0x1p120 ? (T)-0x1p120 : x[e];
+  }
+  uint32_t w = 0, differ = 0;
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    const uint32_t a = q4_round(x[e], lo), b = q4_round(x[e], hi);
+    uint32_t n = a;
+    if constexpr (SHORT) {
+      n = min(a, b);
+      n += n & (a ^ b) & 1u;
+    } else {
+      differ |= a ^ b;
+    }
+    w += n * (1u << (4 * NIBBLE(e)));
+  }
+  if (!SHORT && differ) {
+    w = 0;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      uint32_t n = q4_round(x[e], lo);
+      const T c = (T)((int)(n & 15u) - 8);
+      const T r = fma(-c, (T)s, x[e]), half = (T)0.5 * (T)s;
+      if (fabs(r) > half || (fabs(r) == half && (n & 1u))) n += r > (T)0 ? 1u : 0xFFFFFFFFu;
+      w += n * (1u << (4 * NIBBLE(e)));
+    }
+  }
+  return w - above;
+}
 
 // C[16][8] += A[16][16] B[16][8], bf16 operands, fp32 sums; lane (r, c) = (lane / 4, lane % 4) holds A's rows r
 // (a0, a2) and r + 8 (a1, a3), its k pairs 2c (a0, a1) and 2c + 8 (a2, a3), B's column r at the same k pairs (b0,
