@@ -92,13 +92,30 @@ __device__ __forceinline__ void store_codes(const T* x, uint8_t* codes, __nv_bfl
   uint32_t bits[2];
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
-    T am = 0;
+    float xf[4], am = 0.f;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) am = amax2((T)fabs(x[4 * k + e]), am);
+    for (int e = 0; e < 4; ++e) {
+      xf[e] = (float)x[4 * k + e];
+      am = amax2(fabsf(xf[e]), am);
+    }
 #pragma unroll
     for (int o = 1; o < 8; o <<= 1) am = amax2(__shfl_xor_sync(0xffffffffu, am, o), am);
     s[k] = q4_scale(am);
-    bits[k] = s[k] > 0.f ? q4_bits<4, q4_in_order, SHORT>(x + 4 * k, s[k], am) : 0x8888u;
+    if constexpr (sizeof(T) == 8) {
+      // fp64: where the rounded largest magnitude lies next to a border of two scales, the exact one decides (the
+      // eight lanes of a group agree on it)
+      const float below = __uint_as_float(__float_as_uint(s[k]) - 0x00080000u), near = am * 0x1p-22f;
+      if (fabsf(7.f * s[k] - am) <= near || fabsf(7.f * below - am) <= near || fabsf(am - 0x1p-110f) <= near || !isfinite(am)) {
+        const unsigned lanes = 0xFFu << (threadIdx.x & 24);
+        double exact = 0.0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) exact = amax2(fabs((double)x[4 * k + e]), exact);
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) exact = amax2(__shfl_xor_sync(lanes, exact, o), exact);
+        s[k] = q4_scale(exact);
+      }
+    }
+    bits[k] = s[k] > 0.f ? q4_bits<4, q4_in_order, SHORT>(x + 4 * k, xf, s[k], am) : 0x8888u;
   }
   const bool odd = hl & 1;
   const uint32_t got = __shfl_xor_sync(0xffffffffu, odd ? bits[0] : bits[1], 1);
@@ -185,12 +202,16 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4Params p, __nv_b
     const int w = e % words, h = e / words;                        // h: key heads, then value heads
     const int64_t tok = cache_row(p, page, 0, h, pos);             // heads of both halves follow one another
     const uint32_t v = __ldg(reinterpret_cast<const uint32_t*>(p.codes + tok * (p.D / 2)) + w);
-    const float s = __bfloat162float(p.scales[tok * (p.D / kKvGroup) + w * 8 / kKvGroup]);
+    const uint16_t sc = __ldg(reinterpret_cast<const uint16_t*>(p.scales) + tok * (p.D / kKvGroup) + w * 8 / kKvGroup);
+    uint32_t s2;
+    asm("mov.b32 %0, {%1, %1};" : "=r"(s2) : "h"(sc));
+    const uint32_t v04 = mul_bf16x2(code_pair<0>(v), s2), v15 = mul_bf16x2(code_pair<1>(v), s2);
+    const uint32_t v26 = mul_bf16x2(code_pair<2>(v), s2), v37 = mul_bf16x2(code_pair<3>(v), s2);
     uint4 o;
-    o.x = pack_bf16x2(q4_value(v, 0, s), q4_value(v, 1, s));
-    o.y = pack_bf16x2(q4_value(v, 2, s), q4_value(v, 3, s));
-    o.z = pack_bf16x2(q4_value(v, 4, s), q4_value(v, 5, s));
-    o.w = pack_bf16x2(q4_value(v, 6, s), q4_value(v, 7, s));
+    o.x = __byte_perm(v04, v15, 0x5410);
+    o.y = __byte_perm(v26, v37, 0x5410);
+    o.z = __byte_perm(v04, v15, 0x7632);
+    o.w = __byte_perm(v26, v37, 0x7632);
     reinterpret_cast<uint4*>(out + b * bstride + i * ldo)[e] = o;
   }
 }
@@ -232,12 +253,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
 __device__ __forceinline__ uint32_t fma_bf16x2(uint32_t a, uint32_t b, uint32_t c) {
   uint32_t d;
   asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
-  return d;
-}
-
-__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
-  uint32_t d;
-  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
 }
 

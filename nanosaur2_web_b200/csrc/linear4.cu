@@ -68,7 +68,7 @@ __global__ void __launch_bounds__(256) quantize4_kernel(const Quant4Params p) {
 #pragma unroll
   for (int o = 1; o < G / 8; o <<= 1) am = amax2(__shfl_xor_sync(0xffffffffu, am, o), am);
   const float s = q4_scale(am);
-  const uint32_t out = s > 0.f ? q4_bits<8, q4_nibble, sizeof(T) == 2>(x, s, am) : 0x88888888u;
+  const uint32_t out = s > 0.f ? q4_bits<8, q4_nibble, sizeof(T) == 2>(x, x, s, am) : 0x88888888u;
   const int64_t tr = (int64_t)blockIdx.x * kRowTile + r;   // row of the tiled order
   *reinterpret_cast<uint32_t*>(p.codes + tr * 64 + word_at(w)) = out;
   if (w % (G / 8) == 0) p.scales[tr * (kChunk / G) + w / (G / 8)] = __float2bfloat16_rn(s);
@@ -84,19 +84,21 @@ __global__ void __launch_bounds__(256) expand4_kernel(const Quant4Params p, __nv
   if (row >= p.N || k >= p.K) return;
   const int64_t tr = (int64_t)blockIdx.x * kRowTile + r;
   const uint32_t v = __ldg(reinterpret_cast<const uint32_t*>(p.codes + tr * 64 + word_at(w)));
-  const float s = __bfloat162float(p.scales[tr * (kChunk / p.G) + w * 8 / p.G]);
+  const uint16_t sc = __ldg(reinterpret_cast<const uint16_t*>(p.scales) + tr * (kChunk / p.G) + w * 8 / p.G);
   __nv_bfloat16* dst = out + row * ldo + k;
   if (VEC && k + 8 <= p.K) {
-    uint4 o;
-    o.x = pack_bf16x2(q4_value(v, q4_nibble(0), s), q4_value(v, q4_nibble(1), s));
-    o.y = pack_bf16x2(q4_value(v, q4_nibble(2), s), q4_value(v, q4_nibble(3), s));
-    o.z = pack_bf16x2(q4_value(v, q4_nibble(4), s), q4_value(v, q4_nibble(5), s));
-    o.w = pack_bf16x2(q4_value(v, q4_nibble(6), s), q4_value(v, q4_nibble(7), s));
+    uint32_t s2;
+    asm("mov.b32 %0, {%1, %1};" : "=r"(s2) : "h"(sc));
+    uint4 o;   // code * scale, rounded once
+    o.x = mul_bf16x2(code_pair<0>(v), s2);
+    o.y = mul_bf16x2(code_pair<1>(v), s2);
+    o.z = mul_bf16x2(code_pair<2>(v), s2);
+    o.w = mul_bf16x2(code_pair<3>(v), s2);
     *reinterpret_cast<uint4*>(dst) = o;
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      if (k + e < p.K) dst[e] = __float2bfloat16_rn(q4_value(v, q4_nibble(e), s));
+      if (k + e < p.K) dst[e] = __float2bfloat16_rn(q4_value(v, q4_nibble(e), __uint_as_float((uint32_t)sc << 16)));
   }
 }
 
@@ -143,13 +145,6 @@ struct ChunkScales<128> {
   __device__ __forceinline__ void load(const __nv_bfloat16* p) { v = __ldg(reinterpret_cast<const uint16_t*>(p)); }
   __device__ __forceinline__ float get(int) const { return __uint_as_float((uint32_t)v << 16); }
 };
-
-template <int P>
-__device__ __forceinline__ uint32_t code_pair(uint32_t w) {
-  uint32_t d;
-  asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(((w >> (4 * P)) & 0x000F000Fu) | 0x43004300u), "r"(0xC308C308u));
-  return d;
-}
 
 // NT: tiles of eight rows of X.
 template <int G, int NT>

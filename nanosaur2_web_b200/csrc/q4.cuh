@@ -62,46 +62,58 @@ __device__ __forceinline__ uint32_t q4_round(double x, double inv) {
   return (uint32_t)__double2loint(fma(x, inv, 6755399441055752.0));
 }
 
-// N (4 or 8) stored codes for scale s > 0, value e in nibble NIBBLE(e).  SHORT: every x has at most eight bits.  The
-// nibbles are gathered by adding the sums' low words times powers of 16; what fp32 sums have above the nibbles adds
-// up to a constant modulo 2^32.
-template <int N, int (*NIBBLE)(int), bool SHORT, typename T>
-__device__ __forceinline__ uint32_t q4_bits(const T* in, float s, T amax) {
-  const float inv = __fdividef(1.f, s);
-  const T lo = (T)inv * (T)(1 - 0x1p-20), hi = (T)inv * (T)(1 + 0x1p-20);
-  constexpr uint32_t above = sizeof(T) == 4 ? 0x4B400000u * (N == 8 ? 0x11111111u : 0x1111u) : 0u;
-  T x[N];
-#pragma unroll
-  for (int e = 0; e < N; ++e) x[e] = in[e];
-  if (amax > (T)0x1p120) {
-#pragma unroll
-    for (int e = 0; e < N; ++e) x[e] = x[e] > (T)0x1p120 ? (T)0x1p120 : x[e] < (T)-0x1p120 ? (T)-0x1p120 : x[e];
-  }
-  uint32_t w = 0, differ = 0;
+// The slow, exact decision: saturation, and the remainder of x.
+template <int N, int (*NIBBLE)(int), typename T>
+__device__ __forceinline__ uint32_t q4_bits_exact(const T* x, float s) {
+  const T inv = (T)__fdividef(1.f, s), half = (T)0.5 * (T)s;
+  uint32_t w = 0;
 #pragma unroll
   for (int e = 0; e < N; ++e) {
-    const uint32_t a = q4_round(x[e], lo), b = q4_round(x[e], hi);
+    const T v = x[e] > (T)0x1p120 ? (T)0x1p120 : x[e] < (T)-0x1p120 ? (T)-0x1p120 : x[e];
+    uint32_t n = q4_round(v, inv) & 15u;
+    const T r = fma((T)(8 - (int)n), (T)s, v);
+    if (fabs(r) > half || (fabs(r) == half && (n & 1u))) n += r > (T)0 ? 1u : 0xFFFFFFFFu;
+    w += n << (4 * NIBBLE(e));
+  }
+  return w;
+}
+
+// N (4 or 8) stored codes for scale s > 0, value e in nibble NIBBLE(e), from x or, where T is fp64, from its fp32
+// roundings xf as far as they decide.  SHORT: every x has at most eight bits.  The nibbles are gathered by adding the
+// sums' words times powers of 16; what the sums have above the nibbles adds up to a constant modulo 2^32.
+template <int N, int (*NIBBLE)(int), bool SHORT, typename T>
+__device__ __forceinline__ uint32_t q4_bits(const T* x, const float* xf, float s, float amax) {
+  const float inv = __fdividef(1.f, s), lo = inv * (1.f - 0x1p-20f), hi = inv * (1.f + 0x1p-20f);
+  uint32_t w = 0u - 0x4B400000u * (N == 8 ? 0x11111111u : 0x1111u);
+  bool slow = !(amax <= 0x1p120f);
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    const uint32_t a = q4_round(xf[e], lo), b = q4_round(xf[e], hi);
     uint32_t n = a;
     if constexpr (SHORT) {
       n = min(a, b);
       n += n & (a ^ b) & 1u;
     } else {
-      differ |= a ^ b;
+      slow |= a != b;
     }
     w += n * (1u << (4 * NIBBLE(e)));
   }
-  if (!SHORT && differ) {
-    w = 0;
-#pragma unroll
-    for (int e = 0; e < N; ++e) {
-      uint32_t n = q4_round(x[e], lo);
-      const T c = (T)((int)(n & 15u) - 8);
-      const T r = fma(-c, (T)s, x[e]), half = (T)0.5 * (T)s;
-      if (fabs(r) > half || (fabs(r) == half && (n & 1u))) n += r > (T)0 ? 1u : 0xFFFFFFFFu;
-      w += n * (1u << (4 * NIBBLE(e)));
-    }
-  }
-  return w - above;
+  if (slow) w = q4_bits_exact<N, NIBBLE>(x, s);
+  return w;
+}
+
+// Codes of nibbles P and P + 4 of a word as a bf16 pair, exactly: a nibble n in a bf16 mantissa is 128 + n.
+template <int P>
+__device__ __forceinline__ uint32_t code_pair(uint32_t w) {
+  uint32_t d;
+  asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(((w >> (4 * P)) & 0x000F000Fu) | 0x43004300u), "r"(0xC308C308u));
+  return d;
+}
+
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
 }
 
 // C[16][8] += A[16][16] B[16][8], bf16 operands, fp32 sums; lane (r, c) = (lane / 4, lane % 4) holds A's rows r
