@@ -1815,8 +1815,11 @@ static nsa_status kv4_attention_params(const nsa_kv4_attention_desc* d, const ns
   if ((d->q_ld | d->q_bstride | d->o_ld | d->o_bstride) % 8 || d->q_ld < 0 || d->q_bstride < 0)
     return fail(NSA_ERR_INVALID_ARGUMENT, "the q and out pitches must be multiples of 8, >= 0");
   p->Hq = d->Hq;
+  if ((int64_t)batch->L * (d->Hq / cache->Hkv) > 0x7FFFFFF0LL) return fail(NSA_ERR_UNSUPPORTED, "problem too large for one launch");
+  p->Hq = d->Hq;
   p->window = d->window;
   p->sinks = d->sinks;
+  if (!nsa::kv4_attention_fits(*p)) return fail(NSA_ERR_UNSUPPORTED, "problem too large for one launch");
   p->scale_log2 = (d->scale > 0.f ? d->scale : 1.f / std::sqrt((float)cache->D)) * 1.4426950408889634f;
   p->q_ld = d->q_ld;
   p->q_bstride = d->q_bstride;

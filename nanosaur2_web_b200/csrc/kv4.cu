@@ -218,17 +218,19 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4Params p, __nv_b
 
 // ------------------------------------------------------------------------------------ attention
 //
-// A CTA takes eight query rows that share a key/value head (row R of sequence b is new token R / group, query
-// head R % group of the head's group) and a share of the keys; each of its warps walks its own blocks of 16
-// tokens (a block never straddles pages) with its own running maximum, sum and output, joined in shared memory
-// at the end and, when the keys are split over CTAs, by a second kernel.
+// A unit is 8 or 16 query rows that share a key/value head (row R of sequence b is new token R / group, query head
+// R % group of the head's group) over the blocks of 16 tokens that they see (a block never straddles pages).  The
+// blocks of all units in a row are dealt out evenly to one wave of CTAs, whatever the sequences' lengths, so a CTA works
+// on the end of one unit, some whole ones and the beginning of another.  Within a CTA each warp walks its own blocks
+// with its own running maximum, sum and output, joined in shared memory; what CTAs have of a shared unit is joined
+// by a second kernel.
 //
 // Both products run on mma.m16n8k16 with the cached operand as A, so that the eight query rows fill N = 8 and
 // only the cache's bytes are converted:
 //   S^T [16 tokens][8 rows] = K [16 tokens][D] Q^T,   O^T [D][8 rows] += V^T [D][16 tokens] P^T.
 // A tcgen05 tile would need the converted operand in shared memory (4 times the cache's bytes written and
-// read again there); here each lane loads 4-bit words straight from global memory in the A fragment's own
-// order, converts them in registers and multiplies.  The contraction index of a product may be permuted, so
+// read again there); here the blocks themselves are brought there, a few ahead of their use, and each lane reads its
+// 4-bit words in the A fragment's own order, converts them in registers and multiplies.  The contraction index of a product may be permuted, so
 // lane (r, c) = (lane / 4, lane % 4) takes, of token r, the 16-byte pieces c of the row: nibbles p and p + 4
 // of a word are one bf16 pair, and Q is staged in the matching order.  For V the lane takes piece r of the
 // tokens 2c, 2c + 1, 2c + 8, 2c + 9 (what its B fragment of P^T holds) and pairs the tokens' words by byte
@@ -242,11 +244,12 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4Params p, __nv_b
 // range without a reduction over lanes per block.
 
 constexpr int kAttnWarps = 4;
+constexpr int kMaxShares = 1024;   // CTAs of the attention: at most so many share one unit
 constexpr float kMaxSlack = 8.f;   // exp2 of a score may reach 2^8 before the maximum is moved
 
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   uint32_t d;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
   return d;
 }
 
@@ -269,344 +272,573 @@ __device__ __forceinline__ ScalePair scale_pair(uint32_t lo, uint32_t hi) {
 template <int P>
 __device__ __forceinline__ uint32_t dequant(uint32_t x, ScalePair s) {
   const uint32_t m = P == 0 ? x << 3 : x >> (4 * P - 3);
-  return fma_bf16x2((m & 0x00780078u) | 0x3F803F80u, s.s16, s.m24);
+  return fma_bf16x2(mask_or(m, 0x00780078u, 0x3F803F80u), s.s16, s.m24);
 }
 
-// N 32-bit words (1, 2 or 4 aligned, 8 as two pieces 64 bytes apart).
+// N 32-bit words from shared memory (1, 2 or 4 aligned).
 template <int N>
 __device__ __forceinline__ void load_words(const uint8_t* src, uint32_t* w) {
   if constexpr (N == 1) {
-    w[0] = __ldg(reinterpret_cast<const uint32_t*>(src));
+    w[0] = *reinterpret_cast<const uint32_t*>(src);
   } else if constexpr (N == 2) {
-    const uint2 v = __ldg(reinterpret_cast<const uint2*>(src));
+    const uint2 v = *reinterpret_cast<const uint2*>(src);
     w[0] = v.x; w[1] = v.y;
-  } else if constexpr (N == 4) {
-    const uint4 v = __ldg(reinterpret_cast<const uint4*>(src));
-    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
   } else {
-    load_words<4>(src, w);
-    load_words<4>(src + 64, w + 4);
+    const uint4 v = *reinterpret_cast<const uint4*>(src);
+    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
   }
 }
 
-// Which 16-token blocks the rows of a tile see: [0, sink_blocks), then from first on; n in all.
+__device__ __forceinline__ void copy16_async(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {   // all but the N latest groups of this lane are done
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Which 16-token blocks the rows at positions pmin .. pmax see: [0, sink_blocks), then from first on; n in all.
 struct Blocks {
   int sink_blocks, first, n;
 };
 __device__ __forceinline__ Blocks blocks_of(int pmin, int pmax, int window, int sinks) {
-  if (pmax < 0) return {0, 0, 0};
   const int lo = window > 0 ? max(0, pmin - window + 1) : 0;
   const int first = lo / 16;
   const int ns = min((min(sinks, lo) + 15) / 16, first);
   return {ns, first, ns + pmax / 16 - first + 1};
 }
 
+// The rows of row tile rt of sequence b: new tokens i_first .. i_last (none: i_last < i_first) at positions pmin .. pmax;
+// outside: some of them lie outside the table and see nothing.
+struct Tile {
+  int row0, rows, i_first, i_last, pmin, pmax;
+  bool outside;
+  Blocks bl;
+};
+__device__ __forceinline__ Tile tile_of(const Kv4AttnParams& p, int b, int rt, int rows_per_tile, int group) {
+  const Kv4Params& kv = p.kv;
+  Tile t;
+  t.row0 = rt * rows_per_tile;
+  t.rows = min(rows_per_tile, kv.L * group - t.row0);
+  t.i_first = t.row0 / group;
+  t.i_last = min((t.row0 + t.rows - 1) / group, new_tokens(kv, b) - 1);
+  const int64_t start = kv.start[b], cap = (int64_t)kv.max_pages * kv.P;
+  t.outside = t.i_last >= t.i_first && (start < 0 || start + t.i_last >= cap);
+  t.pmin = (int)(start + t.i_first);
+  t.pmax = (int)min(start + t.i_last, cap - 1);
+  t.bl = {0, 0, 0};
+  if (t.i_last >= t.i_first && start >= 0 && start + t.i_first < cap && kv.n_pages > 0)
+    t.bl = blocks_of(t.pmin, t.pmax, p.window, p.sinks);
+  return t;
+}
+// Blocks of a unit of the tile; a unit that sees nothing but has rows to write counts one.
+__device__ __forceinline__ int unit_blocks(const Tile& t) { return t.i_last < t.i_first ? 0 : max(t.bl.n, 1); }
+
+// A block of 16 tokens in shared memory: keys, values (8 D bytes each), key scales, value scales (D bytes each).  The
+// 16-byte pieces of the codes are moved within each 128 bytes so that neither the keys' reads (all pieces of eight
+// tokens) nor the values' (one piece of every other token) meet on a bank.
 template <int D>
-struct AttnSmem {
-  static constexpr size_t q = (size_t)D / 16 * 32 * 8;                       // Q^T fragments
-  static constexpr size_t o = (size_t)kAttnWarps * 8 * (D + 4) * 4;          // warps' outputs, rows padded
-  static constexpr size_t bytes = (q > o ? q : o) + kAttnWarps * 8 * 2 * 4;  // ... and their (m, l); below 48 KB
+struct Stage {
+  static constexpr int values = 8 * D, scales = 16 * D, bytes = 18 * D;
+  static constexpr int copies = D / 64;   // pieces of the keys (and of the values) per lane
+  // place of piece q of token t
+  static __device__ __forceinline__ int at(int t, int q) {
+    constexpr int per = D / 32;           // pieces per token
+    const int e = t * per + q, row = e / 8, x = e % 8;
+    const int f = D == 256 ? ((row >> 1) & 3) * 2 ^ (row & 1) * 4 : D == 128 ? (row & 3) * 2 : (row & 1) * 2;
+    return row * 128 + (x ^ f) * 16;
+  }
 };
 
-template <int D>
-__global__ void __launch_bounds__(kAttnWarps * 32, D == 256 ? 3 : 4) kv4_attention_kernel(const Kv4AttnParams p) {
+template <int D, int NT>
+struct AttnSmem {
+  static constexpr int stages = D == 256 ? 3 : 4;
+  static constexpr size_t q = (size_t)D / 16 * NT * 32 * 8;                         // Q^T fragments
+  static constexpr size_t ring = (size_t)kAttnWarps * stages * Stage<D>::bytes;
+  static constexpr size_t o = (size_t)kAttnWarps * 8 * NT * (D + 4) * 4;            // warps' outputs, rows padded
+  static constexpr size_t ml = (size_t)kAttnWarps * 8 * NT * 2 * 4;                 // ... and their (m, l)
+  static constexpr size_t bytes = (q + ring > o ? q + ring : o) + ml;
+};
+
+constexpr int ctas_per_sm(int D, int NT) { return NT == 1 ? (D == 256 ? 3 : 4) : (D == 256 ? 2 : 3); }
+
+// NT: tiles of eight query rows.
+template <int D, int NT>
+__global__ void __launch_bounds__(kAttnWarps * 32, ctas_per_sm(D, NT)) kv4_attention_kernel(const Kv4AttnParams p) {
   constexpr int KW = D / 32;   // words of a token's keys per lane
   constexpr int VW = D / 64;   // words of a token's values per lane
   constexpr int KG = D == 256 ? 2 : 1;
+  constexpr int ROWS = 8 * NT, STAGES = AttnSmem<D, NT>::stages;
   extern __shared__ __align__(16) uint8_t smem[];
   const Kv4Params& kv = p.kv;
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, r = lane / 4, c = lane % 4;
+  const int lane = threadIdx.x % 32, r = lane / 4, c = lane % 4;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0);   // known to be the same in all lanes
   const int group = p.Hq / kv.Hkv;
-  const int split = blockIdx.x % p.splits;
-  int u = blockIdx.x / p.splits;
-  const int unit = u;
-  const int rt = u % p.row_tiles;
-  u /= p.row_tiles;
-  const int hk = u % kv.Hkv, b = u / kv.Hkv;
-  const int rows = min(8, kv.L * group - rt * 8);
-  const int cnt = new_tokens(kv, b);
-  // positions of the tile's rows (-1: not a row of this step, or outside the table)
-  int pos0 = -1, pos1 = -1, pmin = 0x7FFFFFFF, pmax = -1;
-  bool outside = false;
-  for (int k = 0; k < rows; ++k) {
-    const int i = (rt * 8 + k) / group;
-    if (i >= cnt) break;
-    const int pos = position(kv, b, i);
-    if (pos >= 0) pmin = min(pmin, pos);
-    else outside = true;
-    pmax = max(pmax, pos);
-    if (k == 2 * c) pos0 = pos;
-    if (k == 2 * c + 1) pos1 = pos;
+
+  // this CTA's blocks [g0, g1) of all units' (units: sequence, row tile, kv head), and the (sequence, tile) of the first
+  const int tiles = kv.B * p.row_tiles;
+  const auto blocks_at = [&](int e) {
+    return e < tiles ? kv.Hkv * unit_blocks(tile_of(p, e / p.row_tiles, e % p.row_tiles, ROWS, group)) : 0;
+  };
+  int own = blocks_at(lane), total = __reduce_add_sync(0xffffffffu, own);
+  for (int e0 = 32; e0 < tiles; e0 += 32) total += __reduce_add_sync(0xffffffffu, blocks_at(e0 + lane));
+  const int per = max((total - 1) / (int)gridDim.x + 1, kAttnWarps);
+  const int g0 = (int)min((int64_t)blockIdx.x * per, (int64_t)total), g1 = min(g0 + per, total);
+  asm volatile("griddepcontrol.launch_dependents;");
+  if (threadIdx.x == 0) p.part_head[blockIdx.x] = make_int2(-1, 0);
+  if (g0 >= g1) return;
+  int entry = 0, before = 0;   // before: blocks of the entries before
+  for (int e0 = 0;; e0 += 32) {
+    if (e0 > 0) own = blocks_at(e0 + lane);
+    int upto = own;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, upto, d);
+      if (lane >= d) upto += x;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, before + upto > g0);
+    if (hit) {
+      const int src = __ffs(hit) - 1;
+      entry = e0 + src;
+      before += __shfl_sync(0xffffffffu, upto - own, src);
+      break;
+    }
+    before += __shfl_sync(0xffffffffu, upto, 31);
   }
-  const Blocks bl = blocks_of(pmin, pmax, p.window, p.sinks);
-  const int share = (bl.n + p.splits - 1) / p.splits;
-  const int t1 = min(bl.n, (split + 1) * share);
-  int t = split * share + warp;
+
+  // Where blocks are: 16 tokens of a head are 8 D bytes of codes and D of scales, so a 32-bit index of blocks and one
+  // wide multiply-add give every address.  A lane copies pieces lane, lane + 32, .. of the codes; of the scales, the
+  // first D / 16 lanes the keys' and the next D / 16 the values'.
+  const uint32_t ppb = kv.P / 16, to_values = kv.Hkv * ppb;
+  const uint8_t* codes = kv.codes + lane * 16;
+  const bool copies_scales = lane < D / 8, value_scales = lane >= D / 16;
+  const uint8_t* scales = reinterpret_cast<const uint8_t*>(kv.scales) + (value_scales ? (uint64_t)to_values * D : 0) + lane % (D / 16) * 16;
+  uint8_t* ring = smem + AttnSmem<D, NT>::q + warp * STAGES * Stage<D>::bytes;
+  const uint32_t ring_at = smem_u32(ring);
+  uint32_t code_at[Stage<D>::copies];
+#pragma unroll
+  for (int x = 0; x < Stage<D>::copies; ++x) {
+    const int e = lane + 32 * x;
+    code_at[x] = Stage<D>::at(e / (D / 32), e % (D / 32));
+  }
+  const uint32_t scale_at = Stage<D>::scales + (value_scales ? D : 0) + lane % (D / 16) * 16;
+  // what the lane reads of a stage: its key words of tokens r and r + 8, value words of tokens 2c, 2c + 1, 2c + 8, 2c + 9
+  int k_at[2][KW > 4 ? 2 : 1], v_at[4];
+#pragma unroll
+  for (int x = 0; x < 2; ++x)
+#pragma unroll
+    for (int y = 0; y < (KW > 4 ? 2 : 1); ++y)
+      k_at[x][y] = D == 64 ? Stage<D>::at(r + 8 * x, c / 2) + c % 2 * 8 : Stage<D>::at(r + 8 * x, c + 4 * y);
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    const int t = 2 * c + (x & 1) + 8 * (x >> 1);
+    v_at[x] = Stage<D>::values + (D == 256 ? Stage<D>::at(t, r) : D == 128 ? Stage<D>::at(t, r / 2) + r % 2 * 8 : Stage<D>::at(t, r / 4) + r % 4 * 4);
+  }
+  const int ks_at = Stage<D>::scales + r * (D / 16) + 2 * (D == 64 ? c / 2 : c);
+  const int vs_at = Stage<D>::scales + D + 2 * c * (D / 16) + r * VW / 4 * 2;
+
+  for (int g = g0; g < g1;) {
+  const int b = entry / p.row_tiles, rt = entry % p.row_tiles;
+  const Tile tl = tile_of(p, b, rt, ROWS, group);
+  const Blocks bl = tl.bl;
+  const int n = unit_blocks(tl);
+  if (g - before >= kv.Hkv * n) {   // on to the next tile with rows
+    before += kv.Hkv * n;
+    ++entry;
+    continue;
+  }
+  const int hk = (g - before) / n, first = g - before - hk * n;
+  const int last = min(n, first + (g1 - g));   // this CTA's blocks of the unit: [first, last)
+  const int row0 = tl.row0, rows = tl.rows, i_last = tl.i_last, pmin = tl.pmin, pmax = tl.pmax;
+  if (threadIdx.x == 0 && first == 0 && hk == 0) {
+    if (tl.outside) atomicCAS(kv.err, 0, kErrKvPosition);
+    else if (kv.n_pages == 0) atomicCAS(kv.err, 0, kErrKvPage);
+  }
+  // this warp's blocks
+  const int each = (last - first + kAttnWarps - 1) / kAttnWarps;
+  const int ta = min(first + warp * each, last), tb = bl.n > 0 ? min(ta + each, last) : ta;
+  const int* table = kv.table + (int64_t)b * kv.table_ld;
+
+  // Walks the warp's blocks, STAGES - 1 ahead of their use: `at` and `left` are the next block's index and the blocks
+  // until another page (or the jump from the first tokens to the window).  A missing page stands on page 0, masked
+  // (`absent`, one bit per stage).  The ids of the two pages ahead are loaded early.
+  int w_t, left, id1, id2;
+  uint32_t at, w_page, absent;
+  bool missing;
+  const auto id_of = [&](uint32_t page) { return page < (uint32_t)kv.max_pages ? __ldg(table + page) : -1; };
+  const auto enter = [&](int id, uint32_t slot) {   // page w_page from its block `slot` on
+    missing = id < 0 || id >= kv.n_pages;
+    if (missing && lane == 0) atomicCAS(kv.err, 0, kErrKvPage);
+    at = ((uint32_t)(missing ? 0 : id) * 2 * kv.Hkv + hk) * ppb + slot;
+    left = (int)(ppb - slot);
+    if (w_t < bl.sink_blocks) left = min(left, bl.sink_blocks - w_t);
+  };
+  const auto jump = [&] {   // to block w_t, wherever it is
+    const uint32_t blk = w_t < bl.sink_blocks ? w_t : bl.first + w_t - bl.sink_blocks;
+    w_page = blk / ppb;
+    const int id = id_of(w_page);
+    id1 = id_of(w_page + 1);
+    id2 = id_of(w_page + 2);
+    enter(id, blk - w_page * ppb);
+  };
+  const auto fetch = [&](int st) {   // block w_t into stage st, then on to the next
+    if (w_t < tb) {
+      if (left == 0) {
+        if (w_t == ta || w_t == bl.sink_blocks) {
+          jump();
+        } else {
+          ++w_page;
+          const int id = id1;
+          id1 = id2;
+          id2 = id_of(w_page + 2);
+          enter(id, 0);
+        }
+      }
+      const uint32_t to = ring_at + st * Stage<D>::bytes;
+      const uint8_t* k = codes + (uint64_t)at * (8 * D);
+      const uint8_t* v = codes + (uint64_t)(at + to_values) * (8 * D);
+#pragma unroll
+      for (int x = 0; x < Stage<D>::copies; ++x) copy16_async(to + code_at[x], k + 512 * x);
+      if (copies_scales) copy16_async(to + scale_at, scales + (uint64_t)at * D);
+#pragma unroll
+      for (int x = 0; x < Stage<D>::copies; ++x) copy16_async(to + Stage<D>::values + code_at[x], v + 512 * x);
+      absent = (absent & ~(1u << st)) | ((uint32_t)missing << st);
+      ++w_t;
+      ++at;
+      --left;
+    }
+    copy_commit();
+  };
+  const auto begin = [&] {
+    w_t = ta;
+    left = 0;
+    absent = 0;
+#pragma unroll
+    for (int st = 0; st < STAGES - 1; ++st) fetch(st);
+  };
+  begin();
+
+  int pos[NT][2];
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int k = 8 * t + 2 * c + j, i = (row0 + k) / group;
+      pos[t][j] = k < rows && i <= i_last && bl.n > 0 && pmin + (i - tl.i_first) <= pmax ? pmin + (i - tl.i_first) : -1;
+    }
+  // blocks whose every token every row sees start in [whole_from, whole_to], or before `sinks` - 15
+  const int whole_to = tl.outside ? -1 : pmin - 15, whole_from = p.window > 0 ? pmax - p.window + 1 : 0;
 
   // Q^T fragments: for k-step 2w + s of lane (r, c), words of row r's dims in the order of the lane's key words
   uint2* qs = reinterpret_cast<uint2*>(smem);
-  for (int e = threadIdx.x; e < D / 16 * 32; e += kAttnWarps * 32) {
-    const int ks = e / 32, ln = e % 32, rr = ln / 4, cc = ln % 4, w = ks / 2, s2 = ks % 2;
+  for (int e = threadIdx.x; e < D / 16 * NT * 32; e += kAttnWarps * 32) {
+    const int ln = e % 32, t = e / 32 % NT, ks = e / 32 / NT, rr = 8 * t + ln / 4, cc = ln % 4, w = ks / 2;
     const int word = D == 256 ? 4 * (cc + 4 * (w / 4)) + w % 4 : KW * cc + w;
     uint2 f = make_uint2(0u, 0u);
-    const int i = (rt * 8 + rr) / group;
-    if (rr < rows && i < cnt) {
+    const int i = (row0 + rr) / group;
+    if (rr < rows && i <= i_last) {
       const uint4 v = *reinterpret_cast<const uint4*>(p.q + b * p.q_bstride + i * p.q_ld +
-                                                      (int64_t)(hk * group + (rt * 8 + rr) % group) * D + word * 8);
-      // pairs (e, e + 4): e = 2 s2 and 2 s2 + 1
-      const uint32_t lo = s2 ? v.y : v.x, hi = s2 ? v.w : v.z;
+                                                      (int64_t)(hk * group + row0 + rr - i * group) * D + word * 8);
+      // pairs (e, e + 4): e = 2 s and 2 s + 1
+      const uint32_t lo = ks % 2 ? v.y : v.x, hi = ks % 2 ? v.w : v.z;
       f = make_uint2(__byte_perm(lo, hi, 0x5410), __byte_perm(lo, hi, 0x7632));
     }
     qs[e] = f;
   }
   __syncthreads();
 
-  float o[VW * 4][4];
+  // m: the largest raw score so far; lim: what a score may reach before m moves; z: the scaled maximum subtracted (0
+  // while there is none)
+  const float slack = kMaxSlack / p.scale_log2;
+  float o[NT][VW * 4][4], m[NT][2], lim[NT][2], z[NT][2], l[NT][2];
+  // The second pass, only after an output that is not a number: see `careful` below.
+  for (bool careful = false;; careful = true) {
+    if (careful) begin();
 #pragma unroll
-  for (int x = 0; x < VW * 4; ++x)
+    for (int t = 0; t < NT; ++t) {
 #pragma unroll
-    for (int y = 0; y < 4; ++y) o[x][y] = 0.f;
-  float m0 = -INFINITY, m1 = -INFINITY, z0 = 0.f, z1 = 0.f, l0 = 0.f, l1 = 0.f;   // z: the maximum subtracted (0 while none)
-
-  uint32_t kw[2][KW], vw[4][VW];
-  uint32_t ks[2][KG], vs[4];
-  const int* table = kv.table + (int64_t)b * kv.table_ld;
-  const int64_t head = (int64_t)hk * kv.P, page_rows = (int64_t)2 * kv.Hkv * kv.P;
-  const auto block_at = [&](int tt) { return tt < bl.sink_blocks ? tt : bl.first + tt - bl.sink_blocks; };
-  // row of the block's first token in the key half of its page, or -1
-  const auto row_of = [&](int tt) -> int64_t {
-    if (tt >= t1) return -1;
-    const int j = block_at(tt) * 16;
-    const int id = __ldg(table + j / kv.P);
-    if (id < 0 || id >= kv.n_pages) {
-      if (lane == 0) atomicCAS(kv.err, 0, kErrKvPage);
-      return -1;
+      for (int x = 0; x < VW * 4; ++x)
+#pragma unroll
+        for (int y = 0; y < 4; ++y) o[t][x][y] = 0.f;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) m[t][j] = lim[t][j] = -INFINITY, z[t][j] = 0.f, l[t][j] = 0.f;
     }
-    return id * page_rows + head + j % kv.P;
-  };
-  const auto load_k = [&](int64_t row) {
+    int j_now = 16 * (ta < bl.sink_blocks ? ta : bl.first + ta - bl.sink_blocks) - 16, stage = 0;
+    for (int tt = ta; tt < tb; ++tt) {
+      j_now = tt == bl.sink_blocks ? 16 * bl.first : j_now + 16;
+      copy_wait<STAGES - 2>();
+      __syncwarp();   // the block is there for all lanes, and all lanes are done with the stage that is filled next
+      fetch(stage == 0 ? STAGES - 1 : stage - 1);
+      const uint8_t* blk = ring + stage * Stage<D>::bytes;
+      const bool gone = absent >> stage & 1;
+      stage = stage == STAGES - 1 ? 0 : stage + 1;
+      uint32_t kw[2][KW], ks[2][KG];
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      if (row < 0) {
+      for (int x = 0; x < 2; ++x) {
+        load_words<(KW > 4 ? 4 : KW)>(blk + k_at[x][0], kw[x]);
+        if constexpr (KW > 4) load_words<4>(blk + k_at[x][1], kw[x] + 4);
 #pragma unroll
-        for (int y = 0; y < KW; ++y) kw[x][y] = 0;
-#pragma unroll
-        for (int y = 0; y < KG; ++y) ks[x][y] = 0;
-        continue;
+        for (int y = 0; y < KG; ++y) ks[x][y] = *reinterpret_cast<const uint16_t*>(blk + ks_at + x * (D / 2) + 8 * y);
       }
-      const int64_t tok = row + r + 8 * x;
-      load_words<KW>(kv.codes + tok * (D / 2) + (D == 256 ? 16 : KW * 4) * c, kw[x]);
-      const uint16_t* sc = reinterpret_cast<const uint16_t*>(kv.scales) + tok * (D / 32);
+      float s[NT][2][4];
 #pragma unroll
-      for (int y = 0; y < KG; ++y) ks[x][y] = __ldg(sc + (D == 64 ? c / 2 : c + 4 * y));
-    }
-  };
-  const auto load_v = [&](int64_t row) {
+      for (int w = 0; w < KW; ++w) {
+        const int g2 = KG == 2 ? w / 4 : 0;
+        const ScalePair sa = scale_pair(ks[0][g2], ks[0][g2]), sb = scale_pair(ks[1][g2], ks[1][g2]);
+        const uint32_t a0 = dequant<0>(kw[0][w], sa), a1 = dequant<0>(kw[1][w], sb), a2 = dequant<1>(kw[0][w], sa),
+                       a3 = dequant<1>(kw[1][w], sb), a4 = dequant<2>(kw[0][w], sa), a5 = dequant<2>(kw[1][w], sb),
+                       a6 = dequant<3>(kw[0][w], sa), a7 = dequant<3>(kw[1][w], sb);
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      if (row < 0) {
-#pragma unroll
-        for (int y = 0; y < VW; ++y) vw[x][y] = 0;
-        vs[x] = 0;
-        continue;
-      }
-      const int64_t tok = row + (int64_t)kv.Hkv * kv.P + 2 * c + (x & 1) + 8 * (x >> 1);
-      load_words<VW>(kv.codes + tok * (D / 2) + VW * 4 * r, vw[x]);
-      vs[x] = __ldg(reinterpret_cast<const uint16_t*>(kv.scales) + tok * (D / 32) + r * VW / 4);
-    }
-  };
-
-  int64_t row = row_of(t);
-  if (t < t1) {
-    load_k(row);
-    load_v(row);
-  }
-  int64_t next = row_of(t + kAttnWarps);
-  for (; t < t1; t += kAttnWarps) {
-    float s[2][4] = {};
-#pragma unroll
-    for (int w = 0; w < KW; ++w) {
-      const int g = KG == 2 ? w / 4 : 0;
-      const ScalePair sa = scale_pair(ks[0][g], ks[0][g]), sb = scale_pair(ks[1][g], ks[1][g]);
-      const uint2 q0 = qs[(2 * w) * 32 + lane], q1 = qs[(2 * w + 1) * 32 + lane];
-      mma_bf16(s[0], dequant<0>(kw[0][w], sa), dequant<0>(kw[1][w], sb), dequant<1>(kw[0][w], sa), dequant<1>(kw[1][w], sb), q0.x, q0.y);
-      mma_bf16(s[1], dequant<2>(kw[0][w], sa), dequant<2>(kw[1][w], sb), dequant<3>(kw[0][w], sa), dequant<3>(kw[1][w], sb), q1.x, q1.y);
-    }
-    const int j0 = block_at(t) * 16;
-    const bool missing = row < 0;
-    if (t + kAttnWarps < t1) load_k(next);
-    float x0 = (s[0][0] + s[1][0]) * p.scale_log2, x1 = (s[0][1] + s[1][1]) * p.scale_log2;
-    float x2 = (s[0][2] + s[1][2]) * p.scale_log2, x3 = (s[0][3] + s[1][3]) * p.scale_log2;
-    const bool whole = !missing && !outside && j0 + 15 <= pmin && (p.window == 0 || j0 > pmax - p.window || j0 + 15 < p.sinks);
-    if (!whole) {
-      const auto see = [&](int pos, int j) {
-        return !missing && j <= pos && (p.window == 0 || j > pos - p.window || j < p.sinks);
-      };
-      if (!see(pos0, j0 + r)) x0 = -INFINITY;
-      if (!see(pos1, j0 + r)) x1 = -INFINITY;
-      if (!see(pos0, j0 + r + 8)) x2 = -INFINITY;
-      if (!see(pos1, j0 + r + 8)) x3 = -INFINITY;
-      // tokens no row sees may hold anything: their values become zeros
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const int j = j0 + 2 * c + (x & 1) + 8 * (x >> 1);
-        if (missing || j > pmax || (p.window > 0 && j <= pmin - p.window && j >= p.sinks)) vs[x] = 0;
-      }
-    }
-    const bool up = x0 > m0 + kMaxSlack || x2 > m0 + kMaxSlack || x1 > m1 + kMaxSlack || x3 > m1 + kMaxSlack;
-    if (__any_sync(0xffffffffu, up)) {
-      float n0 = fmaxf(x0, x2), n1 = fmaxf(x1, x3);
-#pragma unroll
-      for (int d = 4; d < 32; d <<= 1) {
-        n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, d));
-        n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, d));
-      }
-      n0 = fmaxf(n0, m0);
-      n1 = fmaxf(n1, m1);
-      const float y0 = n0 == -INFINITY ? 0.f : n0, y1 = n1 == -INFINITY ? 0.f : n1;
-      const float f0 = exp2f(m0 - y0), f1 = exp2f(m1 - y1);
-      m0 = n0; m1 = n1; z0 = y0; z1 = y1;
-      l0 *= f0;
-      l1 *= f1;
-#pragma unroll
-      for (int x = 0; x < VW * 4; ++x) {
-        o[x][0] *= f0; o[x][1] *= f1;
-        o[x][2] *= f0; o[x][3] *= f1;
-      }
-    }
-    x0 = exp2f(x0 - z0); x1 = exp2f(x1 - z1);
-    x2 = exp2f(x2 - z0); x3 = exp2f(x3 - z1);
-    l0 += x0 + x2;
-    l1 += x1 + x3;
-    const uint32_t h0 = pack_bf16x2(x0, x1), h1 = pack_bf16x2(x2, x3);
-    const uint32_t e0 = pack_bf16x2(x0 - __uint_as_float(h0 << 16), x1 - __uint_as_float(h0 & 0xFFFF0000u));
-    const uint32_t e1 = pack_bf16x2(x2 - __uint_as_float(h1 << 16), x3 - __uint_as_float(h1 & 0xFFFF0000u));
-    const uint32_t ph0 = transpose8x8(h0), ph1 = transpose8x8(h1), pl0 = transpose8x8(e0), pl1 = transpose8x8(e1);
-    // A value group with an infinity or a NaN is NaN in the outputs of the rows that see it; as a factor it
-    // would reach the others too (0 * NaN), so it leaves the product and is added to its rows here.
-    bool odd = false;
-#pragma unroll
-    for (int x = 0; x < 4; ++x) odd |= (vs[x] & 0x7F80u) == 0x7F80u;
-    if (__any_sync(0xffffffffu, odd)) {
-      for (int k = 0; k < 16; ++k) {
-        const int x = (k & 1) + 2 * (k >> 3), src = r * 4 + (k % 8) / 2;
-        const uint32_t sk = __shfl_sync(0xffffffffu, x == 0 ? vs[0] : x == 1 ? vs[1] : x == 2 ? vs[2] : vs[3], src);
-        if ((sk & 0x7F80u) != 0x7F80u) continue;
-        const int j = j0 + k;
-        const auto see = [&](int pos) { return j <= pos && (p.window == 0 || j > pos - p.window || j < p.sinks); };
-        const float nan = __uint_as_float(0x7FC00000u);
-#pragma unroll
-        for (int y = 0; y < VW * 4; ++y) {
-          if (see(pos0)) o[y][0] = nan, o[y][2] = nan;
-          if (see(pos1)) o[y][1] = nan, o[y][3] = nan;
+        for (int t = 0; t < NT; ++t) {
+          const uint2 q0 = qs[(2 * w * NT + t) * 32 + lane], q1 = qs[((2 * w + 1) * NT + t) * 32 + lane];
+          if (w == 0) {
+            mma_bf16_zero(s[t][0], a0, a1, a2, a3, q0.x, q0.y);
+            mma_bf16_zero(s[t][1], a4, a5, a6, a7, q1.x, q1.y);
+          } else {
+            mma_bf16(s[t][0], a0, a1, a2, a3, q0.x, q0.y);
+            mma_bf16(s[t][1], a4, a5, a6, a7, q1.x, q1.y);
+          }
         }
       }
+      uint32_t vw[4][VW], vs[4];
 #pragma unroll
-      for (int x = 0; x < 4; ++x)
-        if ((vs[x] & 0x7F80u) == 0x7F80u) vs[x] = 0;
-    }
-    const ScalePair va = scale_pair(vs[0], vs[1]), vb = scale_pair(vs[2], vs[3]);
-#pragma unroll
-    for (int w = 0; w < VW; ++w) {
-      const uint32_t xa = __byte_perm(vw[0][w], vw[1][w], 0x5410), ya = __byte_perm(vw[0][w], vw[1][w], 0x7632);
-      const uint32_t xb = __byte_perm(vw[2][w], vw[3][w], 0x5410), yb = __byte_perm(vw[2][w], vw[3][w], 0x7632);
-      const auto tile = [&](float* acc, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
-        mma_bf16(acc, a0, a1, a2, a3, ph0, ph1);
-        mma_bf16(acc, a0, a1, a2, a3, pl0, pl1);
+      for (int x = 0; x < 4; ++x) {
+        load_words<VW>(blk + v_at[x], vw[x]);
+        vs[x] = *reinterpret_cast<const uint16_t*>(blk + vs_at + ((x & 1) + 8 * (x >> 1)) * (D / 16));
+      }
+      const auto see = [&](int ps, int j) {
+        return !gone && j <= ps && (p.window == 0 || j > ps - p.window || j < p.sinks);
       };
-      tile(o[4 * w + 0], dequant<0>(xa, va), dequant<0>(ya, va), dequant<0>(xb, vb), dequant<0>(yb, vb));
-      tile(o[4 * w + 1], dequant<1>(xa, va), dequant<1>(ya, va), dequant<1>(xb, vb), dequant<1>(yb, vb));
-      tile(o[4 * w + 2], dequant<2>(xa, va), dequant<2>(ya, va), dequant<2>(xb, vb), dequant<2>(yb, vb));
-      tile(o[4 * w + 3], dequant<3>(xa, va), dequant<3>(ya, va), dequant<3>(xb, vb), dequant<3>(yb, vb));
+      float x[NT][4];
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int y = 0; y < 4; ++y) x[t][y] = s[t][0][y] + s[t][1][y];
+      if (__any_sync(0xffffffffu, gone || j_now > whole_to || (j_now < whole_from && j_now + 15 >= p.sinks))) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int y = 0; y < 4; ++y)
+            if (!see(pos[t][y & 1], j_now + r + 8 * (y >> 1))) x[t][y] = -INFINITY;
+        // tokens no row sees may hold anything: their values become zeros
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          const int j = j_now + 2 * c + (y & 1) + 8 * (y >> 1);
+          if (gone || j > pmax || (p.window > 0 && j <= pmin - p.window && j >= p.sinks)) vs[y] = 0;
+        }
+      }
+      bool up = false;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) up |= fmaxf(x[t][0], x[t][2]) > lim[t][0] || fmaxf(x[t][1], x[t][3]) > lim[t][1];
+      if (__any_sync(0xffffffffu, up)) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          float f[2];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            float n2 = fmaxf(x[t][j], x[t][j + 2]);
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) n2 = fmaxf(n2, __shfl_xor_sync(0xffffffffu, n2, d));
+            n2 = fmaxf(n2, m[t][j]);
+            z[t][j] = n2 == -INFINITY ? 0.f : n2 * p.scale_log2;
+            f[j] = ex2(m[t][j] * p.scale_log2 - z[t][j]);
+            m[t][j] = n2;
+            lim[t][j] = n2 == -INFINITY ? n2 : n2 + slack;
+            l[t][j] *= f[j];
+          }
+#pragma unroll
+          for (int y = 0; y < VW * 4; ++y) {
+            o[t][y][0] *= f[0]; o[t][y][1] *= f[1];
+            o[t][y][2] *= f[0]; o[t][y][3] *= f[1];
+          }
+        }
+      }
+      uint32_t ph[NT][2], pl[NT][2];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+#pragma unroll
+        for (int y = 0; y < 4; ++y) x[t][y] = ex2(fmaf(x[t][y], p.scale_log2, -z[t][y & 1]));
+        l[t][0] += x[t][0] + x[t][2];
+        l[t][1] += x[t][1] + x[t][3];
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          const uint32_t h = pack_bf16x2(x[t][2 * y], x[t][2 * y + 1]);
+          const uint32_t e = pack_bf16x2(x[t][2 * y] - __uint_as_float(h << 16), x[t][2 * y + 1] - __uint_as_float(h & 0xFFFF0000u));
+          ph[t][y] = transpose8x8(h);
+          pl[t][y] = transpose8x8(e);
+        }
+      }
+      // A value group with an infinity or a NaN is NaN in the outputs of the rows that see it; as a factor it
+      // reaches the others of the tile too (0 * NaN).  Where an output came out as no number the blocks are walked
+      // again with such groups taken out of the product and added to their rows here.
+      if (careful) {
+        for (int k = 0; k < 16; ++k) {
+          const int y = (k & 1) + 2 * (k >> 3), src = r * 4 + (k % 8) / 2;
+          const uint32_t sk = __shfl_sync(0xffffffffu, y == 0 ? vs[0] : y == 1 ? vs[1] : y == 2 ? vs[2] : vs[3], src);
+          if ((sk & 0x7F80u) != 0x7F80u) continue;
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+              if (see(pos[t][j], j_now + k)) {
+#pragma unroll
+                for (int w = 0; w < VW * 4; ++w) o[t][w][j] = o[t][w][j + 2] = __uint_as_float(0x7FC00000u);
+              }
+        }
+#pragma unroll
+        for (int y = 0; y < 4; ++y)
+          if ((vs[y] & 0x7F80u) == 0x7F80u) vs[y] = 0;
+      }
+      const ScalePair va = scale_pair(vs[0], vs[1]), vb = scale_pair(vs[2], vs[3]);
+#pragma unroll
+      for (int w = 0; w < VW; ++w) {
+        const uint32_t xa = __byte_perm(vw[0][w], vw[1][w], 0x5410), ya = __byte_perm(vw[0][w], vw[1][w], 0x7632);
+        const uint32_t xb = __byte_perm(vw[2][w], vw[3][w], 0x5410), yb = __byte_perm(vw[2][w], vw[3][w], 0x7632);
+        const auto tile = [&](int x4, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            mma_bf16(o[t][x4], a0, a1, a2, a3, ph[t][0], ph[t][1]);
+            mma_bf16(o[t][x4], a0, a1, a2, a3, pl[t][0], pl[t][1]);
+          }
+        };
+        tile(4 * w + 0, dequant<0>(xa, va), dequant<0>(ya, va), dequant<0>(xb, vb), dequant<0>(yb, vb));
+        tile(4 * w + 1, dequant<1>(xa, va), dequant<1>(ya, va), dequant<1>(xb, vb), dequant<1>(yb, vb));
+        tile(4 * w + 2, dequant<2>(xa, va), dequant<2>(ya, va), dequant<2>(xb, vb), dequant<2>(yb, vb));
+        tile(4 * w + 3, dequant<3>(xa, va), dequant<3>(ya, va), dequant<3>(xb, vb), dequant<3>(yb, vb));
+      }
     }
-    if (t + kAttnWarps < t1) load_v(next);
-    row = next;
-    next = row_of(t + 2 * kAttnWarps);
+    float sum = 0.f;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int y = 0; y < VW * 4; ++y) sum += (o[t][y][0] - o[t][y][0]) + (o[t][y][1] - o[t][y][1]) + (o[t][y][2] - o[t][y][2]) + (o[t][y][3] - o[t][y][3]);
+    if (careful || !__any_sync(0xffffffffu, sum != 0.f)) break;   // x - x is 0 unless x is infinite or no number
   }
 #pragma unroll
-  for (int d = 4; d < 32; d <<= 1) {
-    l0 += __shfl_xor_sync(0xffffffffu, l0, d);
-    l1 += __shfl_xor_sync(0xffffffffu, l1, d);
-  }
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int d = 4; d < 32; d <<= 1) l[t][j] += __shfl_xor_sync(0xffffffffu, l[t][j], d);
 
   // join the warps
-  __syncthreads();   // the fragments of Q are no longer read
+  copy_wait<0>();
+  __syncthreads();   // nothing reads the fragments of Q or the ring any more
   float* so = reinterpret_cast<float*>(smem);
-  float* sm = reinterpret_cast<float*>(smem + AttnSmem<D>::bytes - kAttnWarps * 8 * 2 * 4);
+  float* sm = reinterpret_cast<float*>(smem + AttnSmem<D, NT>::bytes - AttnSmem<D, NT>::ml);
   constexpr int LD = D + 4;
 #pragma unroll
-  for (int w = 0; w < VW; ++w)
+  for (int t = 0; t < NT; ++t) {
+    const int k = warp * ROWS + 8 * t + 2 * c;
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const int d = 8 * (VW * r + w) + x;
-      float* row0 = so + (warp * 8 + 2 * c) * LD + d;
-      row0[0] = o[4 * w + x][0];
-      row0[LD] = o[4 * w + x][1];
-      row0[4] = o[4 * w + x][2];
-      row0[LD + 4] = o[4 * w + x][3];
+    for (int w = 0; w < VW; ++w)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        float* d = so + k * LD + 8 * (VW * r + w) + x;
+        d[0] = o[t][4 * w + x][0];
+        d[LD] = o[t][4 * w + x][1];
+        d[4] = o[t][4 * w + x][2];
+        d[LD + 4] = o[t][4 * w + x][3];
+      }
+    if (r == 0) {
+      float* ml = sm + k * 2;
+      ml[0] = m[t][0] == -INFINITY ? m[t][0] : z[t][0]; ml[1] = l[t][0];
+      ml[2] = m[t][1] == -INFINITY ? m[t][1] : z[t][1]; ml[3] = l[t][1];
     }
-  if (r == 0) {
-    float* ml = sm + (warp * 8 + 2 * c) * 2;
-    ml[0] = m0; ml[1] = l0;
-    ml[2] = m1; ml[3] = l1;
   }
   __syncthreads();
   for (int e = threadIdx.x; e < rows * (D / 4); e += kAttnWarps * 32) {
     const int k = e / (D / 4), d = e % (D / 4) * 4;
-    const int i = (rt * 8 + k) / group;
-    if (i >= cnt) break;
+    const int i = (row0 + k) / group;
+    if (i > i_last) break;
     float M = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kAttnWarps; ++w) M = fmaxf(M, sm[(w * 8 + k) * 2]);
-    const float z = M == -INFINITY ? 0.f : M;
-    float l = 0.f;
+    for (int w = 0; w < kAttnWarps; ++w) M = fmaxf(M, sm[(w * ROWS + k) * 2]);
+    const float zero = M == -INFINITY ? 0.f : M;
+    float ls = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int w = 0; w < kAttnWarps; ++w) {
-      const float f = exp2f(sm[(w * 8 + k) * 2] - z);
-      const float4 v = *reinterpret_cast<const float4*>(so + (w * 8 + k) * LD + d);
-      l = fmaf(f, sm[(w * 8 + k) * 2 + 1], l);
+      const float f = ex2(sm[(w * ROWS + k) * 2] - zero);
+      const float4 v = *reinterpret_cast<const float4*>(so + (w * ROWS + k) * LD + d);
+      ls = fmaf(f, sm[(w * ROWS + k) * 2 + 1], ls);
       acc.x = fmaf(f, v.x, acc.x); acc.y = fmaf(f, v.y, acc.y);
       acc.z = fmaf(f, v.z, acc.z); acc.w = fmaf(f, v.w, acc.w);
     }
-    if (p.splits == 1) {
-      const float inv = l == 0.f ? 0.f : 1.f / l;   // no key seen: zeros
+    if (first == 0 && last == n) {
+      const float inv = ls == 0.f ? 0.f : 1.f / ls;   // no key seen: zeros
       uint2 w;
       w.x = pack_bf16x2(acc.x * inv, acc.y * inv);
       w.y = pack_bf16x2(acc.z * inv, acc.w * inv);
-      *reinterpret_cast<uint2*>(p.out + b * p.o_bstride + i * p.o_ld + (int64_t)(hk * group + (rt * 8 + k) % group) * D + d) = w;
+      *reinterpret_cast<uint2*>(p.out + b * p.o_bstride + i * p.o_ld + (int64_t)(hk * group + row0 + k - i * group) * D + d) = w;
     } else {
-      const int64_t pr = ((int64_t)unit * p.splits + split) * 8 + k;
+      // a unit shared with other CTAs: a CTA has at most two, at its first block and at its last
+      const int64_t pr = ((int64_t)blockIdx.x * 2 + (g == g0 ? 0 : 1)) * ROWS + k;
       *reinterpret_cast<float4*>(p.part_o + pr * D + d) = acc;
       if (d == 0) {
         p.part_ml[pr * 2] = M;
-        p.part_ml[pr * 2 + 1] = l;
+        p.part_ml[pr * 2 + 1] = ls;
       }
     }
   }
+  // who has the first of a shared unit's blocks names it: the entry and head, and the CTAs that share it
+  if (threadIdx.x == 0 && first == 0 && last < n)
+    p.part_head[blockIdx.x] = make_int2(entry * kv.Hkv + hk, (int)((g + n - 1) / per) - (int)blockIdx.x + 1 + (g == g0 ? 0 : 1 << 30));
+  g += last - first;
+  if (g < g1) __syncthreads();   // the next unit stages its rows where the sums were
+  }
 }
 
-// Joins the shares of a row's keys: one CTA per (unit, row), a thread per dim.
-__global__ void kv4_join_kernel(const Kv4AttnParams p) {
+// Joins a shared unit: one CTA per (CTA of the first kernel, row), exiting where that names none.
+__global__ void __launch_bounds__(256) kv4_join_kernel(const Kv4AttnParams p) {
+  __shared__ float weight[kMaxShares], red[256];
   const Kv4Params& kv = p.kv;
-  const int D = kv.D, group = p.Hq / kv.Hkv;
-  const int k = blockIdx.x % 8;
-  const int64_t unit = blockIdx.x / 8;
-  const int rt = (int)(unit % p.row_tiles), hk = (int)(unit / p.row_tiles % kv.Hkv), b = (int)(unit / p.row_tiles / kv.Hkv);
-  const int R = rt * 8 + k, i = R / group;
+  asm volatile("griddepcontrol.wait;" ::: "memory");   // launched while the first kernel runs
+  const int2 head = p.part_head[blockIdx.x];
+  if (head.x < 0) return;
+  const int D = kv.D, group = p.Hq / kv.Hkv, rows = 8 * p.row_nt, k = blockIdx.y;
+  const int hk = head.x % kv.Hkv, entry = head.x / kv.Hkv, rt = entry % p.row_tiles, b = entry / p.row_tiles;
+  const int R = rt * rows + k, i = R / group;
   if (R >= kv.L * group || i >= new_tokens(kv, b)) return;
-  const int64_t pr = unit * p.splits * 8 + k;
+  // share s: slot 0 of the CTA blockIdx.x + s, but the first may be that CTA's slot 1
+  const int shares = head.y & ((1 << 30) - 1);
+  const auto slot = [&](int s) { return ((int64_t)(blockIdx.x + s) * 2 + (s == 0 ? head.y >> 30 : 0)) * rows + k; };
   float M = -INFINITY;
-  for (int s = 0; s < p.splits; ++s) M = fmaxf(M, p.part_ml[(pr + s * 8) * 2]);
-  const float z = M == -INFINITY ? 0.f : M;
-  float l = 0.f, acc = 0.f;
-  for (int s = 0; s < p.splits; ++s) {
-    const float f = exp2f(p.part_ml[(pr + s * 8) * 2] - z);
-    l = fmaf(f, p.part_ml[(pr + s * 8) * 2 + 1], l);
-    acc = fmaf(f, p.part_o[(pr + s * 8) * D + threadIdx.x], acc);
+  for (int s = threadIdx.x; s < shares; s += 256) M = fmaxf(M, p.part_ml[slot(s) * 2]);
+  red[threadIdx.x] = M;
+  __syncthreads();
+  for (int d = 128; d > 0; d >>= 1) {
+    if (threadIdx.x < d) red[threadIdx.x] = fmaxf(red[threadIdx.x], red[threadIdx.x + d]);
+    __syncthreads();
   }
-  p.out[b * p.o_bstride + i * p.o_ld + (int64_t)(hk * group + R % group) * D + threadIdx.x] =
-      __float2bfloat16_rn(l == 0.f ? 0.f : acc / l);
+  M = red[0];
+  const float z = M == -INFINITY ? 0.f : M;
+  __syncthreads();
+  float l = 0.f;
+  for (int s = threadIdx.x; s < shares; s += 256) {
+    const float f = ex2(p.part_ml[slot(s) * 2] - z);
+    weight[s] = f;
+    l = fmaf(f, p.part_ml[slot(s) * 2 + 1], l);
+  }
+  red[threadIdx.x] = l;
+  __syncthreads();
+  for (int d = 128; d > 0; d >>= 1) {
+    if (threadIdx.x < d) red[threadIdx.x] += red[threadIdx.x + d];
+    __syncthreads();
+  }
+  l = red[0];
+  __syncthreads();
+  // a thread per dim and 256 / D threads per dim over the shares
+  const int d = threadIdx.x % D, lanes = 256 / D;
+  float acc = 0.f;
+#pragma unroll 8
+  for (int s = threadIdx.x / D; s < shares; s += lanes) acc = fmaf(weight[s], p.part_o[slot(s) * D + d], acc);
+  red[threadIdx.x] = acc;
+  __syncthreads();
+  if (threadIdx.x >= D) return;
+  for (int x = 1; x < lanes; ++x) acc += red[threadIdx.x + x * D];
+  p.out[b * p.o_bstride + i * p.o_ld + (int64_t)(hk * group + R % group) * D + d] = __float2bfloat16_rn(l == 0.f ? 0.f : acc / l);
 }
 
 template <typename T>
@@ -640,54 +872,79 @@ cudaError_t launch_kv4_read(const Kv4Params& p, __nv_bfloat16* out, int64_t ldo,
   return cudaGetLastError();
 }
 
-constexpr int kCtasWanted = 4 * 3 * 148;   // four waves of three CTAs on each of a B200's SMs
-
-// Row tiles, and how many CTAs share a tile's keys: enough for a few CTAs per SM and to even out sequences of
-// different lengths, as long as each warp keeps two blocks of 16 tokens of the longest sequence.
+// Row tiles (two tiles of eight rows at a time share the converted operand where there are more than eight rows), and the
+// CTAs: one wave, but at least a block of 16 tokens for each warp of the longest sequences.
 void kv4_attention_plan(Kv4AttnParams* p) {
   const Kv4Params& kv = p->kv;
-  p->row_tiles = (int)(((int64_t)kv.L * (p->Hq / kv.Hkv) + 7) / 8);
+  const int64_t rows = (int64_t)kv.L * (p->Hq / kv.Hkv);
+  p->row_nt = rows > 8 ? 2 : 1;
+  p->row_tiles = (int)((rows + 8 * p->row_nt - 1) / (8 * p->row_nt));
   const int64_t units = (int64_t)kv.B * kv.Hkv * p->row_tiles;
-  const int64_t cap = (int64_t)kv.max_pages * kv.P;
-  const int64_t seen = p->window > 0 ? std::min(cap, (int64_t)p->window + p->sinks + kv.L + 30) : cap;
-  const int64_t want = (kCtasWanted + units - 1) / units;
-  const int64_t most = (seen + 16 * kAttnWarps * 2 - 1) / (16 * kAttnWarps * 2);
-  p->splits = (int)std::max<int64_t>(1, std::min(want, most));
+  const int64_t cap = (int64_t)kv.max_pages * kv.P / 16;
+  const int64_t seen = p->window > 0 ? std::min(cap, ((int64_t)p->window + 8 * p->row_nt + 30) / 16 + (p->sinks + 15) / 16) : cap;
+  const int64_t most = (units * std::max<int64_t>(seen, 1) + kAttnWarps - 1) / kAttnWarps;
+  p->ctas = (int)std::min<int64_t>(most, std::min(kMaxShares, 148 * ctas_per_sm(kv.D, p->row_nt)));
 }
 
+// Blocks are counted in 32 bits.
+bool kv4_attention_fits(Kv4AttnParams p) {
+  const Kv4Params& kv = p.kv;
+  const double tiles = (double)kv.B * kv.Hkv * (((double)kv.L * (p.Hq / kv.Hkv)) / 8 + 1);
+  return tiles * ((double)kv.max_pages * kv.P / 16 + 1) < 2147480000.0;
+}
+
+// Two partial tiles per CTA (outputs, then maxima and sums), then the names of shared units.
 size_t kv4_attention_workspace(Kv4AttnParams p) {
   kv4_attention_plan(&p);
-  if (p.splits == 1) return 0;
-  return (size_t)p.kv.B * p.kv.Hkv * p.row_tiles * p.splits * 8 * (p.kv.D + 2) * 4;
+  return (size_t)p.ctas * (2 * 8 * p.row_nt * (p.kv.D + 2) * 4 + 8);
 }
 
 namespace {
 
-template <int D>
-cudaError_t launch_attention_t(const Kv4AttnParams& p, unsigned blocks, cudaStream_t stream) {
-  kv4_attention_kernel<D><<<blocks, kAttnWarps * 32, AttnSmem<D>::bytes, stream>>>(p);
+template <int D, int NT>
+cudaError_t launch_attention_t(const Kv4AttnParams& p, cudaStream_t stream) {
+  constexpr int bytes = (int)AttnSmem<D, NT>::bytes;
+  if (bytes > 48 * 1024) {
+    static DeviceOnce once;
+    const cudaError_t e = once_per_device(
+        once, [] { return cudaFuncSetAttribute(kv4_attention_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); });
+    if (e != cudaSuccess) return e;
+  }
+  kv4_attention_kernel<D, NT><<<p.ctas, kAttnWarps * 32, bytes, stream>>>(p);
   return cudaGetLastError();
+}
+
+template <int D>
+cudaError_t launch_attention_d(const Kv4AttnParams& p, cudaStream_t stream) {
+  return p.row_nt == 1 ? launch_attention_t<D, 1>(p, stream) : launch_attention_t<D, 2>(p, stream);
 }
 
 }  // namespace
 
 cudaError_t launch_kv4_attention(Kv4AttnParams p, void* workspace, cudaStream_t stream) {
   kv4_attention_plan(&p);
-  const int64_t units = (int64_t)p.kv.B * p.kv.Hkv * p.row_tiles;
-  if (units * p.splits > 0x7FFFFFFFLL || units * 8 > 0x7FFFFFFFLL) return cudaErrorInvalidValue;
+  const int64_t slots = (int64_t)p.ctas * 2 * 8 * p.row_nt;
   p.part_o = static_cast<float*>(workspace);
-  p.part_ml = p.part_o + units * p.splits * 8 * p.kv.D;
-  const unsigned blocks = (unsigned)(units * p.splits);
+  p.part_ml = p.part_o + slots * p.kv.D;
+  p.part_head = reinterpret_cast<int2*>(p.part_ml + slots * 2);
   cudaError_t e;
   switch (p.kv.D) {
-    case 64: e = launch_attention_t<64>(p, blocks, stream); break;
-    case 128: e = launch_attention_t<128>(p, blocks, stream); break;
-    case 256: e = launch_attention_t<256>(p, blocks, stream); break;
+    case 64: e = launch_attention_d<64>(p, stream); break;
+    case 128: e = launch_attention_d<128>(p, stream); break;
+    case 256: e = launch_attention_d<256>(p, stream); break;
     default: return cudaErrorInvalidValue;
   }
-  if (e != cudaSuccess || p.splits == 1) return e;
-  kv4_join_kernel<<<(unsigned)(units * 8), p.kv.D, 0, stream>>>(p);
-  return cudaGetLastError();
+  if (e != cudaSuccess || p.ctas == 1) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(p.ctas, 8 * p.row_nt);
+  cfg.blockDim = dim3(256);
+  cfg.stream = stream;
+  cudaLaunchAttribute early;   // set up while the first kernel runs; it waits for that kernel's end by itself
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kv4_join_kernel, p);
 }
 
 }  // namespace nsa

@@ -345,10 +345,13 @@ struct Kv4AttnParams {
   __nv_bfloat16* out;
   int64_t o_ld, o_bstride;
   // set by the launch
-  int row_tiles, splits;    // tiles of 8 query rows per kv head; CTAs that share a tile's keys
-  float* part_o;            // [units][splits][8][D] unnormalised outputs (units: sequence, kv head, row tile)
-  float* part_ml;           // [units][splits][8][2] maximum (base 2) and sum
+  int row_nt, row_tiles;    // 8 row_nt query rows per row tile; row tiles per sequence and kv head
+  int ctas;                 // CTAs that the blocks of 16 tokens are dealt out to
+  float* part_o;            // [ctas][2][8 row_nt][D] unnormalised outputs of units shared with other CTAs
+  float* part_ml;           // [ctas][2][8 row_nt][2] maximum (base 2) and sum
+  int2* part_head;          // [ctas] the shared unit whose first block the CTA has (-1: none), and its CTAs
 };
+bool kv4_attention_fits(Kv4AttnParams p);           // sequences x heads x table width within one launch
 size_t kv4_attention_workspace(Kv4AttnParams p);   // bytes; 0: none needed
 cudaError_t launch_kv4_attention(Kv4AttnParams p, void* workspace, cudaStream_t stream);
 

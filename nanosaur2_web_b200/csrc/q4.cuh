@@ -102,11 +102,18 @@ __device__ __forceinline__ uint32_t q4_bits(const T* x, const float* xf, float s
   return w;
 }
 
+// (v & mask) | bits in one instruction (left to the compiler, two constants make it two).
+__device__ __forceinline__ uint32_t mask_or(uint32_t v, uint32_t mask, uint32_t bits) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(v), "r"(mask), "r"(bits));
+  return d;
+}
+
 // Codes of nibbles P and P + 4 of a word as a bf16 pair, exactly: a nibble n in a bf16 mantissa is 128 + n.
 template <int P>
 __device__ __forceinline__ uint32_t code_pair(uint32_t w) {
   uint32_t d;
-  asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(((w >> (4 * P)) & 0x000F000Fu) | 0x43004300u), "r"(0xC308C308u));
+  asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(mask_or(w >> (4 * P), 0x000F000Fu, 0x43004300u)), "r"(0xC308C308u));
   return d;
 }
 
@@ -120,9 +127,16 @@ __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
 // (a0, a2) and r + 8 (a1, a3), its k pairs 2c (a0, a1) and 2c + 8 (a2, a3), B's column r at the same k pairs (b0,
 // b1), and C's rows r (c0, c1) and r + 8 (c2, c3) at columns 2c and 2c + 1.
 __device__ __forceinline__ void mma_bf16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// The same from zero.
+__device__ __forceinline__ void mma_bf16_zero(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+               : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 
 }  // namespace nsa
