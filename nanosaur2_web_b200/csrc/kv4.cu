@@ -8,6 +8,8 @@
 // recorded in the device error word and its access skipped.
 #include <algorithm>
 
+#include <cooperative_groups.h>
+
 #include "nsa_internal.h"
 #include "ptx.cuh"
 #include "q4.cuh"
@@ -223,7 +225,8 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4Params p, __nv_b
 // blocks of all units in a row are dealt out evenly to one wave of CTAs, whatever the sequences' lengths, so a CTA works
 // on the end of one unit, some whole ones and the beginning of another.  Within a CTA each warp walks its own blocks
 // with its own running maximum, sum and output, joined in shared memory; what CTAs have of a shared unit is joined
-// by a second kernel.
+// by a second kernel.  Few and short units are latency instead: a cluster of eight CTAs takes one unit and joins it
+// through its shared memories.
 //
 // Both products run on mma.m16n8k16 with the cached operand as A, so that the eight query rows fill N = 8 and
 // only the cache's bytes are converted:
@@ -244,7 +247,6 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4Params p, __nv_b
 // range without a reduction over lanes per block.
 
 constexpr int kAttnWarps = 4;
-constexpr int kMaxShares = 1024;   // CTAs of the attention: at most so many share one unit
 constexpr float kMaxSlack = 8.f;   // exp2 of a score may reach 2^8 before the maximum is moved
 
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
@@ -309,6 +311,9 @@ __device__ __forceinline__ Blocks blocks_of(int pmin, int pmax, int window, int 
   return {ns, first, ns + pmax / 16 - first + 1};
 }
 
+// New token of row R of a sequence's rows.
+__device__ __forceinline__ int token_of(const Kv4Params& kv, int R, int group) { return kv.L == 1 ? 0 : R / group; }
+
 // The rows of row tile rt of sequence b: new tokens i_first .. i_last (none: i_last < i_first) at positions pmin .. pmax;
 // outside: some of them lie outside the table and see nothing.
 struct Tile {
@@ -321,8 +326,8 @@ __device__ __forceinline__ Tile tile_of(const Kv4AttnParams& p, int b, int rt, i
   Tile t;
   t.row0 = rt * rows_per_tile;
   t.rows = min(rows_per_tile, kv.L * group - t.row0);
-  t.i_first = t.row0 / group;
-  t.i_last = min((t.row0 + t.rows - 1) / group, new_tokens(kv, b) - 1);
+  t.i_first = token_of(kv, t.row0, group);
+  t.i_last = min(token_of(kv, t.row0 + t.rows - 1, group), new_tokens(kv, b) - 1);
   const int64_t start = kv.start[b], cap = (int64_t)kv.max_pages * kv.P;
   t.outside = t.i_last >= t.i_first && (start < 0 || start + t.i_last >= cap);
   t.pmin = (int)(start + t.i_first);
@@ -363,8 +368,8 @@ struct AttnSmem {
 
 constexpr int ctas_per_sm(int D, int NT) { return NT == 1 ? (D == 256 ? 3 : 4) : (D == 256 ? 2 : 3); }
 
-// NT: tiles of eight query rows.
-template <int D, int NT>
+// NT: tiles of eight query rows.  CL: 1, or the CTAs of a cluster that takes one unit.
+template <int D, int NT, int CL>
 __global__ void __launch_bounds__(kAttnWarps * 32, ctas_per_sm(D, NT)) kv4_attention_kernel(const Kv4AttnParams p) {
   constexpr int KW = D / 32;   // words of a token's keys per lane
   constexpr int VW = D / 64;   // words of a token's values per lane
@@ -377,34 +382,39 @@ __global__ void __launch_bounds__(kAttnWarps * 32, ctas_per_sm(D, NT)) kv4_atten
   const int group = p.Hq / kv.Hkv;
 
   // this CTA's blocks [g0, g1) of all units' (units: sequence, row tile, kv head), and the (sequence, tile) of the first
-  const int tiles = kv.B * p.row_tiles;
-  const auto blocks_at = [&](int e) {
-    return e < tiles ? kv.Hkv * unit_blocks(tile_of(p, e / p.row_tiles, e % p.row_tiles, ROWS, group)) : 0;
-  };
-  int own = blocks_at(lane), total = __reduce_add_sync(0xffffffffu, own);
-  for (int e0 = 32; e0 < tiles; e0 += 32) total += __reduce_add_sync(0xffffffffu, blocks_at(e0 + lane));
-  const int per = max((total - 1) / (int)gridDim.x + 1, kAttnWarps);
-  const int g0 = (int)min((int64_t)blockIdx.x * per, (int64_t)total), g1 = min(g0 + per, total);
-  asm volatile("griddepcontrol.launch_dependents;");
-  if (threadIdx.x == 0) p.part_head[blockIdx.x] = make_int2(-1, 0);
-  if (g0 >= g1) return;
-  int entry = 0, before = 0;   // before: blocks of the entries before
-  for (int e0 = 0;; e0 += 32) {
-    if (e0 > 0) own = blocks_at(e0 + lane);
-    int upto = own;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int x = __shfl_up_sync(0xffffffffu, upto, d);
-      if (lane >= d) upto += x;
+  int g0 = 0, g1 = 1, per = 1, entry = 0, before = 0;   // before: blocks of the entries before
+  if constexpr (CL == 1) {
+    const int tiles = kv.B * p.row_tiles;
+    const auto blocks_at = [&](int e) {
+      return e < tiles ? kv.Hkv * unit_blocks(tile_of(p, e / p.row_tiles, e % p.row_tiles, ROWS, group)) : 0;
+    };
+    int own = blocks_at(lane), total = __reduce_add_sync(0xffffffffu, own);
+    for (int e0 = 32; e0 < tiles; e0 += 32) total += __reduce_add_sync(0xffffffffu, blocks_at(e0 + lane));
+    per = max((total - 1) / (int)gridDim.x + 1, kAttnWarps);
+    g0 = (int)min((int64_t)blockIdx.x * per, (int64_t)total);
+    g1 = min(g0 + per, total);
+    asm volatile("griddepcontrol.launch_dependents;");
+    if (threadIdx.x == 0) p.part_head[blockIdx.x] = make_int2(-1, 0);
+    if (g0 >= g1) return;
+    for (int e0 = 0;; e0 += 32) {
+      if (e0 > 0) own = blocks_at(e0 + lane);
+      int upto = own;
+  #pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, upto, d);
+        if (lane >= d) upto += x;
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, before + upto > g0);
+      if (hit) {
+        const int src = __ffs(hit) - 1;
+        entry = e0 + src;
+        before += __shfl_sync(0xffffffffu, upto - own, src);
+        break;
+      }
+      before += __shfl_sync(0xffffffffu, upto, 31);
     }
-    const unsigned hit = __ballot_sync(0xffffffffu, before + upto > g0);
-    if (hit) {
-      const int src = __ffs(hit) - 1;
-      entry = e0 + src;
-      before += __shfl_sync(0xffffffffu, upto - own, src);
-      break;
-    }
-    before += __shfl_sync(0xffffffffu, upto, 31);
+  } else {
+    entry = blockIdx.x / CL / kv.Hkv;
   }
 
   // Where blocks are: 16 tokens of a head are 8 D bytes of codes and D of scales, so a 32-bit index of blocks and one
@@ -443,15 +453,25 @@ __global__ void __launch_bounds__(kAttnWarps * 32, ctas_per_sm(D, NT)) kv4_atten
   const Tile tl = tile_of(p, b, rt, ROWS, group);
   const Blocks bl = tl.bl;
   const int n = unit_blocks(tl);
-  if (g - before >= kv.Hkv * n) {   // on to the next tile with rows
-    before += kv.Hkv * n;
-    ++entry;
-    continue;
+  int hk, first, last;   // this CTA's blocks of the unit: [first, last)
+  if constexpr (CL == 1) {
+    if (g - before >= kv.Hkv * n) {   // on to the next tile with rows
+      before += kv.Hkv * n;
+      ++entry;
+      continue;
+    }
+    hk = (g - before) / n;
+    first = g - before - hk * n;
+    last = min(n, first + (g1 - g));
+  } else {
+    if (n == 0) return;   // the whole cluster
+    hk = blockIdx.x / CL % kv.Hkv;
+    const int share = (n + CL - 1) / CL;
+    first = min((int)(blockIdx.x % CL) * share, n);
+    last = min(first + share, n);
   }
-  const int hk = (g - before) / n, first = g - before - hk * n;
-  const int last = min(n, first + (g1 - g));   // this CTA's blocks of the unit: [first, last)
   const int row0 = tl.row0, rows = tl.rows, i_last = tl.i_last, pmin = tl.pmin, pmax = tl.pmax;
-  if (threadIdx.x == 0 && first == 0 && hk == 0) {
+  if (threadIdx.x == 0 && first == 0 && last > 0 && hk == 0) {
     if (tl.outside) atomicCAS(kv.err, 0, kErrKvPosition);
     else if (kv.n_pages == 0) atomicCAS(kv.err, 0, kErrKvPage);
   }
@@ -524,7 +544,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, ctas_per_sm(D, NT)) kv4_atten
   for (int t = 0; t < NT; ++t)
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const int k = 8 * t + 2 * c + j, i = (row0 + k) / group;
+      const int k = 8 * t + 2 * c + j, i = token_of(kv, row0 + k, group);
       pos[t][j] = k < rows && i <= i_last && bl.n > 0 && pmin + (i - tl.i_first) <= pmax ? pmin + (i - tl.i_first) : -1;
     }
   // blocks whose every token every row sees start in [whole_from, whole_to], or before `sinks` - 15
@@ -536,7 +556,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, ctas_per_sm(D, NT)) kv4_atten
     const int ln = e % 32, t = e / 32 % NT, ks = e / 32 / NT, rr = 8 * t + ln / 4, cc = ln % 4, w = ks / 2;
     const int word = D == 256 ? 4 * (cc + 4 * (w / 4)) + w % 4 : KW * cc + w;
     uint2 f = make_uint2(0u, 0u);
-    const int i = (row0 + rr) / group;
+    const int i = token_of(kv, row0 + rr, group);
     if (rr < rows && i <= i_last) {
       const uint4 v = *reinterpret_cast<const uint4*>(p.q + b * p.q_bstride + i * p.q_ld +
                                                       (int64_t)(hk * group + row0 + rr - i * group) * D + word * 8);
@@ -747,26 +767,40 @@ __global__ void __launch_bounds__(kAttnWarps * 32, ctas_per_sm(D, NT)) kv4_atten
       ml[2] = m[t][1] == -INFINITY ? m[t][1] : z[t][1]; ml[3] = l[t][1];
     }
   }
-  __syncthreads();
-  for (int e = threadIdx.x; e < rows * (D / 4); e += kAttnWarps * 32) {
+  // every warp of the CTA, or of the cluster's CTAs
+  namespace cg = cooperative_groups;
+  if constexpr (CL > 1) cg::this_cluster().sync();
+  else __syncthreads();
+  const int from = CL > 1 ? (blockIdx.x % CL) * kAttnWarps * 32 + threadIdx.x : threadIdx.x;
+  for (int e = from; e < rows * (D / 4); e += CL * kAttnWarps * 32) {
     const int k = e / (D / 4), d = e % (D / 4) * 4;
-    const int i = (row0 + k) / group;
+    const int i = token_of(kv, row0 + k, group);
     if (i > i_last) break;
-    float M = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < kAttnWarps; ++w) M = fmaxf(M, sm[(w * ROWS + k) * 2]);
-    const float zero = M == -INFINITY ? 0.f : M;
-    float ls = 0.f;
+    float M = -INFINITY, ls = 0.f, mw[CL * kAttnWarps];
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int w = 0; w < kAttnWarps; ++w) {
-      const float f = ex2(sm[(w * ROWS + k) * 2] - zero);
-      const float4 v = *reinterpret_cast<const float4*>(so + (w * ROWS + k) * LD + d);
-      ls = fmaf(f, sm[(w * ROWS + k) * 2 + 1], ls);
+    for (int w = 0; w < CL * kAttnWarps; ++w) {
+      const float* x = sm + (w % kAttnWarps * ROWS + k) * 2;
+      if constexpr (CL > 1) x = cg::this_cluster().map_shared_rank(x, w / kAttnWarps);
+      mw[w] = x[0];
+      M = fmaxf(M, mw[w]);
+    }
+    const float zero = M == -INFINITY ? 0.f : M;
+#pragma unroll
+    for (int w = 0; w < CL * kAttnWarps; ++w) {
+      const float f = ex2(mw[w] - zero);
+      const float* x = so + (w % kAttnWarps * ROWS + k) * LD + d;
+      const float* y = sm + (w % kAttnWarps * ROWS + k) * 2 + 1;
+      if constexpr (CL > 1) {
+        x = cg::this_cluster().map_shared_rank(x, w / kAttnWarps);
+        y = cg::this_cluster().map_shared_rank(y, w / kAttnWarps);
+      }
+      const float4 v = *reinterpret_cast<const float4*>(x);
+      ls = fmaf(f, *y, ls);
       acc.x = fmaf(f, v.x, acc.x); acc.y = fmaf(f, v.y, acc.y);
       acc.z = fmaf(f, v.z, acc.z); acc.w = fmaf(f, v.w, acc.w);
     }
-    if (first == 0 && last == n) {
+    if (CL > 1 || (first == 0 && last == n)) {
       const float inv = ls == 0.f ? 0.f : 1.f / ls;   // no key seen: zeros
       uint2 w;
       w.x = pack_bf16x2(acc.x * inv, acc.y * inv);
@@ -782,6 +816,10 @@ __global__ void __launch_bounds__(kAttnWarps * 32, ctas_per_sm(D, NT)) kv4_atten
       }
     }
   }
+  if constexpr (CL > 1) {
+    cg::this_cluster().sync();   // no CTA leaves while another reads its shared memory
+    return;
+  }
   // who has the first of a shared unit's blocks names it: the entry and head, and the CTAs that share it
   if (threadIdx.x == 0 && first == 0 && last < n)
     p.part_head[blockIdx.x] = make_int2(entry * kv.Hkv + hk, (int)((g + n - 1) / per) - (int)blockIdx.x + 1 + (g == g0 ? 0 : 1 << 30));
@@ -790,55 +828,58 @@ __global__ void __launch_bounds__(kAttnWarps * 32, ctas_per_sm(D, NT)) kv4_atten
   }
 }
 
-// Joins a shared unit: one CTA per (CTA of the first kernel, row), exiting where that names none.
-__global__ void __launch_bounds__(256) kv4_join_kernel(const Kv4AttnParams p) {
-  __shared__ float weight[kMaxShares], red[256];
+// Joins a shared unit: one CTA per (CTA of the first kernel, row), exiting where that names none; a thread per dim or two.
+template <int D>
+__global__ void __launch_bounds__(128) kv4_join_kernel(const Kv4AttnParams p) {
   const Kv4Params& kv = p.kv;
   asm volatile("griddepcontrol.wait;" ::: "memory");   // launched while the first kernel runs
   const int2 head = p.part_head[blockIdx.x];
   if (head.x < 0) return;
-  const int D = kv.D, group = p.Hq / kv.Hkv, rows = 8 * p.row_nt, k = blockIdx.y;
+  const int group = p.Hq / kv.Hkv, rows = 8 * p.row_nt, k = blockIdx.y, lane = threadIdx.x % 32;
   const int hk = head.x % kv.Hkv, entry = head.x / kv.Hkv, rt = entry % p.row_tiles, b = entry / p.row_tiles;
-  const int R = rt * rows + k, i = R / group;
+  const int R = rt * rows + k, i = token_of(kv, R, group);
   if (R >= kv.L * group || i >= new_tokens(kv, b)) return;
   // share s: slot 0 of the CTA blockIdx.x + s, but the first may be that CTA's slot 1
   const int shares = head.y & ((1 << 30) - 1);
   const auto slot = [&](int s) { return ((int64_t)(blockIdx.x + s) * 2 + (s == 0 ? head.y >> 30 : 0)) * rows + k; };
   float M = -INFINITY;
-  for (int s = threadIdx.x; s < shares; s += 256) M = fmaxf(M, p.part_ml[slot(s) * 2]);
-  red[threadIdx.x] = M;
-  __syncthreads();
-  for (int d = 128; d > 0; d >>= 1) {
-    if (threadIdx.x < d) red[threadIdx.x] = fmaxf(red[threadIdx.x], red[threadIdx.x + d]);
-    __syncthreads();
-  }
-  M = red[0];
+  for (int s = lane; s < shares; s += 32) M = fmaxf(M, p.part_ml[slot(s) * 2]);
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
   const float z = M == -INFINITY ? 0.f : M;
-  __syncthreads();
-  float l = 0.f;
-  for (int s = threadIdx.x; s < shares; s += 256) {
-    const float f = ex2(p.part_ml[slot(s) * 2] - z);
-    weight[s] = f;
-    l = fmaf(f, p.part_ml[slot(s) * 2 + 1], l);
-  }
-  red[threadIdx.x] = l;
-  __syncthreads();
-  for (int d = 128; d > 0; d >>= 1) {
-    if (threadIdx.x < d) red[threadIdx.x] += red[threadIdx.x + d];
-    __syncthreads();
-  }
-  l = red[0];
-  __syncthreads();
-  // a thread per dim and 256 / D threads per dim over the shares
-  const int d = threadIdx.x % D, lanes = 256 / D;
-  float acc = 0.f;
+  constexpr int V = D == 256 ? 2 : 1;
+  float l = 0.f, acc[V] = {};
+  for (int s0 = 0; s0 < shares; s0 += 32) {
+    float f = 0.f;
+    if (s0 + lane < shares) {
+      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + slot(s0 + lane) * 2);
+      f = ex2(ml.x - z);
+      l = fmaf(f, ml.y, l);
+    }
+    const int n = min(32, shares - s0);
 #pragma unroll 8
-  for (int s = threadIdx.x / D; s < shares; s += lanes) acc = fmaf(weight[s], p.part_o[slot(s) * D + d], acc);
-  red[threadIdx.x] = acc;
-  __syncthreads();
-  if (threadIdx.x >= D) return;
-  for (int x = 1; x < lanes; ++x) acc += red[threadIdx.x + x * D];
-  p.out[b * p.o_bstride + i * p.o_ld + (int64_t)(hk * group + R % group) * D + d] = __float2bfloat16_rn(l == 0.f ? 0.f : acc / l);
+    for (int j = 0; j < n; ++j) {
+      const float w = __shfl_sync(0xffffffffu, f, j);
+      if (D < 128 && threadIdx.x >= D) continue;
+      const float* src = p.part_o + slot(s0 + j) * D + threadIdx.x * V;
+      if constexpr (V == 2) {
+        const float2 v = *reinterpret_cast<const float2*>(src);
+        acc[0] = fmaf(w, v.x, acc[0]);
+        acc[1] = fmaf(w, v.y, acc[1]);
+      } else {
+        acc[0] = fmaf(w, *src, acc[0]);
+      }
+    }
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+  if (D < 128 && threadIdx.x >= D) return;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  __nv_bfloat16* dst = p.out + b * p.o_bstride + i * p.o_ld + (int64_t)(hk * group + R - i * group) * D + threadIdx.x * V;
+  if constexpr (V == 2)
+    *reinterpret_cast<uint32_t*>(dst) = pack_bf16x2(acc[0] * inv, acc[1] * inv);
+  else
+    *dst = __float2bfloat16_rn(acc[0] * inv);
 }
 
 template <typename T>
@@ -872,8 +913,11 @@ cudaError_t launch_kv4_read(const Kv4Params& p, __nv_bfloat16* out, int64_t ldo,
   return cudaGetLastError();
 }
 
+constexpr int kCluster = 8;
+
 // Row tiles (two tiles of eight rows at a time share the converted operand where there are more than eight rows), and the
-// CTAs: one wave, but at least a block of 16 tokens for each warp of the longest sequences.
+// CTAs: a cluster per unit where these fit one wave and no unit is longer than eight blocks per warp, else one wave, but
+// at least a block of 16 tokens for each warp of the longest sequences.
 void kv4_attention_plan(Kv4AttnParams* p) {
   const Kv4Params& kv = p->kv;
   const int64_t rows = (int64_t)kv.L * (p->Hq / kv.Hkv);
@@ -882,8 +926,10 @@ void kv4_attention_plan(Kv4AttnParams* p) {
   const int64_t units = (int64_t)kv.B * kv.Hkv * p->row_tiles;
   const int64_t cap = (int64_t)kv.max_pages * kv.P / 16;
   const int64_t seen = p->window > 0 ? std::min(cap, ((int64_t)p->window + 8 * p->row_nt + 30) / 16 + (p->sinks + 15) / 16) : cap;
+  const int wave = 148 * ctas_per_sm(kv.D, p->row_nt);
+  p->cluster = units * kCluster <= wave && seen <= kCluster * kAttnWarps * 8;
   const int64_t most = (units * std::max<int64_t>(seen, 1) + kAttnWarps - 1) / kAttnWarps;
-  p->ctas = (int)std::min<int64_t>(most, std::min(kMaxShares, 148 * ctas_per_sm(kv.D, p->row_nt)));
+  p->ctas = p->cluster ? (int)units * kCluster : (int)std::min<int64_t>(most, wave);
 }
 
 // Blocks are counted in 32 bits.
@@ -896,55 +942,68 @@ bool kv4_attention_fits(Kv4AttnParams p) {
 // Two partial tiles per CTA (outputs, then maxima and sums), then the names of shared units.
 size_t kv4_attention_workspace(Kv4AttnParams p) {
   kv4_attention_plan(&p);
+  if (p.cluster) return 0;
   return (size_t)p.ctas * (2 * 8 * p.row_nt * (p.kv.D + 2) * 4 + 8);
 }
 
 namespace {
 
-template <int D, int NT>
+template <int D, int NT, int CL>
 cudaError_t launch_attention_t(const Kv4AttnParams& p, cudaStream_t stream) {
   constexpr int bytes = (int)AttnSmem<D, NT>::bytes;
   if (bytes > 48 * 1024) {
     static DeviceOnce once;
     const cudaError_t e = once_per_device(
-        once, [] { return cudaFuncSetAttribute(kv4_attention_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); });
+        once, [] { return cudaFuncSetAttribute(kv4_attention_kernel<D, NT, CL>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); });
     if (e != cudaSuccess) return e;
   }
-  kv4_attention_kernel<D, NT><<<p.ctas, kAttnWarps * 32, bytes, stream>>>(p);
-  return cudaGetLastError();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(p.ctas);
+  cfg.blockDim = dim3(kAttnWarps * 32);
+  cfg.dynamicSmemBytes = bytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute cluster;
+  cluster.id = cudaLaunchAttributeClusterDimension;
+  cluster.val.clusterDim.x = CL;
+  cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+  cfg.attrs = &cluster;
+  cfg.numAttrs = CL > 1 ? 1 : 0;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kv4_attention_kernel<D, NT, CL>, p);
+  if (e != cudaSuccess || CL > 1 || p.ctas == 1) return e;
+  cudaLaunchAttribute early;   // set up while the first kernel runs; it waits for that kernel's end by itself
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3(p.ctas, 8 * NT);
+  cfg.blockDim = dim3(128);
+  cfg.dynamicSmemBytes = 0;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kv4_join_kernel<D>, p);
 }
 
 template <int D>
 cudaError_t launch_attention_d(const Kv4AttnParams& p, cudaStream_t stream) {
-  return p.row_nt == 1 ? launch_attention_t<D, 1>(p, stream) : launch_attention_t<D, 2>(p, stream);
+  if (p.cluster)
+    return p.row_nt == 1 ? launch_attention_t<D, 1, kCluster>(p, stream) : launch_attention_t<D, 2, kCluster>(p, stream);
+  return p.row_nt == 1 ? launch_attention_t<D, 1, 1>(p, stream) : launch_attention_t<D, 2, 1>(p, stream);
 }
 
 }  // namespace
 
 cudaError_t launch_kv4_attention(Kv4AttnParams p, void* workspace, cudaStream_t stream) {
   kv4_attention_plan(&p);
-  const int64_t slots = (int64_t)p.ctas * 2 * 8 * p.row_nt;
-  p.part_o = static_cast<float*>(workspace);
-  p.part_ml = p.part_o + slots * p.kv.D;
-  p.part_head = reinterpret_cast<int2*>(p.part_ml + slots * 2);
-  cudaError_t e;
+  if (!p.cluster) {
+    const int64_t slots = (int64_t)p.ctas * 2 * 8 * p.row_nt;
+    p.part_o = static_cast<float*>(workspace);
+    p.part_ml = p.part_o + slots * p.kv.D;
+    p.part_head = reinterpret_cast<int2*>(p.part_ml + slots * 2);
+  }
   switch (p.kv.D) {
-    case 64: e = launch_attention_d<64>(p, stream); break;
-    case 128: e = launch_attention_d<128>(p, stream); break;
-    case 256: e = launch_attention_d<256>(p, stream); break;
+    case 64: return launch_attention_d<64>(p, stream);
+    case 128: return launch_attention_d<128>(p, stream);
+    case 256: return launch_attention_d<256>(p, stream);
     default: return cudaErrorInvalidValue;
   }
-  if (e != cudaSuccess || p.ctas == 1) return e;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(p.ctas, 8 * p.row_nt);
-  cfg.blockDim = dim3(256);
-  cfg.stream = stream;
-  cudaLaunchAttribute early;   // set up while the first kernel runs; it waits for that kernel's end by itself
-  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  early.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &early;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kv4_join_kernel, p);
 }
 
 }  // namespace nsa

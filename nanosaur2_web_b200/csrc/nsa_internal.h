@@ -346,6 +346,7 @@ struct Kv4AttnParams {
   int64_t o_ld, o_bstride;
   // set by the launch
   int row_nt, row_tiles;    // 8 row_nt query rows per row tile; row tiles per sequence and kv head
+  int cluster;              // 1: a cluster of CTAs per unit, joined in shared memory (no workspace)
   int ctas;                 // CTAs that the blocks of 16 tokens are dealt out to
   float* part_o;            // [ctas][2][8 row_nt][D] unnormalised outputs of units shared with other CTAs
   float* part_ml;           // [ctas][2][8 row_nt][2] maximum (base 2) and sum

@@ -270,7 +270,8 @@ def test_kv4_attention(B, L, Hq, Hkv, D, P, T, window, sinks):
     assert (np.abs(n64(got) - want) <= tol).all(), float((np.abs(n64(got) - want) / tol).max())
 
 
-@pytest.mark.parametrize("D,Hkv,P,T", [(128, 1, 64, 5000), (64, 2, 16, 3001), (256, 1, 32, 2500)])
+@pytest.mark.parametrize("D,Hkv,P,T", [(128, 1, 64, 5000), (64, 2, 16, 3001), (256, 1, 32, 2500), (256, 1, 16, 4500),
+                                      (64, 1, 48, 9000)])
 def test_kv4_attention_long_and_split(D, Hkv, P, T):
     """One sequence, long enough that its keys are shared out and joined; a scale of the caller's; large scores."""
     from nanosaur2_web_b200.ops import kv4_attention
@@ -282,6 +283,29 @@ def test_kv4_attention_long_and_split(D, Hkv, P, T):
     check_device()
     want, tol = attend_oracle(cd, n64(q), start, [2], 0, 0, np.float32(0.2))
     assert (np.abs(n64(got) - want) <= tol).all(), float((np.abs(n64(got) - want) / tol).max())
+
+
+@pytest.mark.parametrize("B,L,Hq,Hkv,D,P,T,window,sinks", [(90, 1, 4, 2, 64, 16, 60, 0, 0), (70, 3, 6, 1, 128, 16, 45, 0, 0),
+                                                           (37, 2, 4, 4, 256, 16, 40, 9, 3), (100, 1, 1, 1, 64, 16, 300, 33, 0),
+                                                           (3, 70, 3, 3, 64, 16, 90, 0, 0)])
+def test_kv4_attention_many_units(B, L, Hq, Hkv, D, P, T, window, sinks):
+    """More sequences, heads and rows than one wave takes, of very different lengths, some without new tokens: CTAs
+    hold ends, wholes and beginnings of units."""
+    from nanosaur2_web_b200.ops import kv4_attention
+    rng = np.random.default_rng(B)
+    cd = Cached(rng, B, T, Hkv, D, P)
+    q = t(1.5 * rng.standard_normal((B, L, Hq * D)), BF)
+    start = np.array([(37 * b * b) % (T - L + 1) for b in range(B)], np.int32)
+    count = np.array([L if b % 5 else b % 3 * L // 2 for b in range(B)], np.int32)
+    out = torch.full((B, L, Hq * D), 9.0, dtype=BF, device=DEV)
+    for _ in range(2):
+        kv4_attention(q, cd.cache, cd.table, t(start, torch.int32), count=t(count, torch.int32), window=window, sinks=sinks, out=out)
+    check_device()
+    want, tol = attend_oracle(cd, n64(q), start, count, window, sinks, 1 / np.sqrt(D))
+    got = n64(out)
+    for b in range(B):
+        assert (np.abs(got[b, :count[b]] - want[b, :count[b]]) <= tol[b, :count[b]]).all(), b
+        assert (got[b, count[b]:] == 9).all()
 
 
 def test_kv4_attention_counts_strides_and_rows_left_alone():
