@@ -277,18 +277,20 @@ __device__ __forceinline__ uint32_t dequant(uint32_t x, ScalePair s) {
   return fma_bf16x2(mask_or(m, 0x00780078u, 0x3F803F80u), s.s16, s.m24);
 }
 
-// N 32-bit words from shared memory (1, 2 or 4 aligned).
+// N 32-bit words (1, 2 or 4 aligned), or a scale, from shared memory.
 template <int N>
-__device__ __forceinline__ void load_words(const uint8_t* src, uint32_t* w) {
-  if constexpr (N == 1) {
-    w[0] = *reinterpret_cast<const uint32_t*>(src);
-  } else if constexpr (N == 2) {
-    const uint2 v = *reinterpret_cast<const uint2*>(src);
-    w[0] = v.x; w[1] = v.y;
-  } else {
-    const uint4 v = *reinterpret_cast<const uint4*>(src);
-    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
-  }
+__device__ __forceinline__ void load_words(uint32_t at, uint32_t* w) {
+  if constexpr (N == 1)
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[0]) : "r"(at));
+  else if constexpr (N == 2)
+    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(at));
+  else
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at));
+}
+__device__ __forceinline__ uint32_t load_scale(uint32_t at) {
+  uint16_t v;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at));
+  return v;
 }
 
 __device__ __forceinline__ void copy16_async(uint32_t dst, const void* src) {
@@ -424,8 +426,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, ctas_per_sm(D, NT)) kv4_atten
   const uint8_t* codes = kv.codes + lane * 16;
   const bool copies_scales = lane < D / 8, value_scales = lane >= D / 16;
   const uint8_t* scales = reinterpret_cast<const uint8_t*>(kv.scales) + (value_scales ? (uint64_t)to_values * D : 0) + lane % (D / 16) * 16;
-  uint8_t* ring = smem + AttnSmem<D, NT>::q + warp * STAGES * Stage<D>::bytes;
-  const uint32_t ring_at = smem_u32(ring);
+  const uint32_t ring_at = smem_u32(smem + AttnSmem<D, NT>::q) + warp * STAGES * Stage<D>::bytes;
   uint32_t code_at[Stage<D>::copies];
 #pragma unroll
   for (int x = 0; x < Stage<D>::copies; ++x) {
@@ -434,19 +435,17 @@ __global__ void __launch_bounds__(kAttnWarps * 32, ctas_per_sm(D, NT)) kv4_atten
   }
   const uint32_t scale_at = Stage<D>::scales + (value_scales ? D : 0) + lane % (D / 16) * 16;
   // what the lane reads of a stage: its key words of tokens r and r + 8, value words of tokens 2c, 2c + 1, 2c + 8, 2c + 9
-  int k_at[2][KW > 4 ? 2 : 1], v_at[4];
+  // (eight tokens on is 4 D bytes on, pieces moved alike)
+  uint32_t k_at[KW > 4 ? 2 : 1], v_at[2];
 #pragma unroll
-  for (int x = 0; x < 2; ++x)
+  for (int y = 0; y < (KW > 4 ? 2 : 1); ++y) k_at[y] = D == 64 ? Stage<D>::at(r, c / 2) + c % 2 * 8 : Stage<D>::at(r, c + 4 * y);
 #pragma unroll
-    for (int y = 0; y < (KW > 4 ? 2 : 1); ++y)
-      k_at[x][y] = D == 64 ? Stage<D>::at(r + 8 * x, c / 2) + c % 2 * 8 : Stage<D>::at(r + 8 * x, c + 4 * y);
-#pragma unroll
-  for (int x = 0; x < 4; ++x) {
-    const int t = 2 * c + (x & 1) + 8 * (x >> 1);
+  for (int x = 0; x < 2; ++x) {
+    const int t = 2 * c + x;
     v_at[x] = Stage<D>::values + (D == 256 ? Stage<D>::at(t, r) : D == 128 ? Stage<D>::at(t, r / 2) + r % 2 * 8 : Stage<D>::at(t, r / 4) + r % 4 * 4);
   }
-  const int ks_at = Stage<D>::scales + r * (D / 16) + 2 * (D == 64 ? c / 2 : c);
-  const int vs_at = Stage<D>::scales + D + 2 * c * (D / 16) + r * VW / 4 * 2;
+  const uint32_t ks_at = Stage<D>::scales + r * (D / 16) + 2 * (D == 64 ? c / 2 : c);
+  const uint32_t vs_at = Stage<D>::scales + D + 2 * c * (D / 16) + r * VW / 4 * 2;
 
   for (int g = g0; g < g1;) {
   const int b = entry / p.row_tiles, rt = entry % p.row_tiles;
@@ -523,7 +522,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, ctas_per_sm(D, NT)) kv4_atten
       if (copies_scales) copy16_async(to + scale_at, scales + (uint64_t)at * D);
 #pragma unroll
       for (int x = 0; x < Stage<D>::copies; ++x) copy16_async(to + Stage<D>::values + code_at[x], v + 512 * x);
-      absent = (absent & ~(1u << st)) | ((uint32_t)missing << st);
+      if (missing || absent) absent = (absent & ~(1u << st)) | ((uint32_t)missing << st);
       ++w_t;
       ++at;
       --left;
@@ -547,8 +546,9 @@ __global__ void __launch_bounds__(kAttnWarps * 32, ctas_per_sm(D, NT)) kv4_atten
       const int k = 8 * t + 2 * c + j, i = token_of(kv, row0 + k, group);
       pos[t][j] = k < rows && i <= i_last && bl.n > 0 && pmin + (i - tl.i_first) <= pmax ? pmin + (i - tl.i_first) : -1;
     }
-  // blocks whose every token every row sees start in [whole_from, whole_to], or before `sinks` - 15
-  const int whole_to = tl.outside ? -1 : pmin - 15, whole_from = p.window > 0 ? pmax - p.window + 1 : 0;
+  // every row sees every token of the blocks numbered [whole0, whole1)
+  const int whole0 = p.window > 0 ? bl.sink_blocks + (max(pmax - p.window + 1, 0) + 15) / 16 - bl.first : 0;
+  const int whole1 = tl.outside ? 0 : bl.sink_blocks + (pmin + 1) / 16 - bl.first;
 
   // Q^T fragments: for k-step 2w + s of lane (r, c), words of row r's dims in the order of the lane's key words
   uint2* qs = reinterpret_cast<uint2*>(smem);
@@ -590,16 +590,16 @@ __global__ void __launch_bounds__(kAttnWarps * 32, ctas_per_sm(D, NT)) kv4_atten
       copy_wait<STAGES - 2>();
       __syncwarp();   // the block is there for all lanes, and all lanes are done with the stage that is filled next
       fetch(stage == 0 ? STAGES - 1 : stage - 1);
-      const uint8_t* blk = ring + stage * Stage<D>::bytes;
-      const bool gone = absent >> stage & 1;
+      const uint32_t blk = ring_at + stage * Stage<D>::bytes;
+      const bool gone = absent && (absent >> stage & 1);
       stage = stage == STAGES - 1 ? 0 : stage + 1;
       uint32_t kw[2][KW], ks[2][KG];
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        load_words<(KW > 4 ? 4 : KW)>(blk + k_at[x][0], kw[x]);
-        if constexpr (KW > 4) load_words<4>(blk + k_at[x][1], kw[x] + 4);
+        load_words<(KW > 4 ? 4 : KW)>(blk + k_at[0] + x * 4 * D, kw[x]);
+        if constexpr (KW > 4) load_words<4>(blk + k_at[1] + x * 4 * D, kw[x] + 4);
 #pragma unroll
-        for (int y = 0; y < KG; ++y) ks[x][y] = *reinterpret_cast<const uint16_t*>(blk + ks_at + x * (D / 2) + 8 * y);
+        for (int y = 0; y < KG; ++y) ks[x][y] = load_scale(blk + ks_at + x * (D / 2) + 8 * y);
       }
       float s[NT][2][4];
 #pragma unroll
@@ -624,8 +624,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32, ctas_per_sm(D, NT)) kv4_atten
       uint32_t vw[4][VW], vs[4];
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
-        load_words<VW>(blk + v_at[x], vw[x]);
-        vs[x] = *reinterpret_cast<const uint16_t*>(blk + vs_at + ((x & 1) + 8 * (x >> 1)) * (D / 16));
+        load_words<VW>(blk + v_at[x & 1] + (x >> 1) * 4 * D, vw[x]);
+        vs[x] = load_scale(blk + vs_at + ((x & 1) + 8 * (x >> 1)) * (D / 16));
       }
       const auto see = [&](int ps, int j) {
         return !gone && j <= ps && (p.window == 0 || j > ps - p.window || j < p.sinks);
@@ -635,7 +635,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, ctas_per_sm(D, NT)) kv4_atten
       for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int y = 0; y < 4; ++y) x[t][y] = s[t][0][y] + s[t][1][y];
-      if (__any_sync(0xffffffffu, gone || j_now > whole_to || (j_now < whole_from && j_now + 15 >= p.sinks))) {
+      if (__any_sync(0xffffffffu, tt < whole0 || tt >= whole1 || gone)) {
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -828,14 +828,17 @@ __global__ void __launch_bounds__(kAttnWarps * 32, ctas_per_sm(D, NT)) kv4_atten
   }
 }
 
-// Joins a shared unit: one CTA per (CTA of the first kernel, row), exiting where that names none; a thread per dim or two.
+// Joins a shared unit: one CTA per (CTA of the first kernel, row), exiting where that names none; each of its warps takes
+// a quarter of the shares, D / 32 dims a lane.
 template <int D>
 __global__ void __launch_bounds__(128) kv4_join_kernel(const Kv4AttnParams p) {
+  constexpr int V = D / 32;
+  __shared__ float part[4][D], sums[4];
   const Kv4Params& kv = p.kv;
   asm volatile("griddepcontrol.wait;" ::: "memory");   // launched while the first kernel runs
   const int2 head = p.part_head[blockIdx.x];
   if (head.x < 0) return;
-  const int group = p.Hq / kv.Hkv, rows = 8 * p.row_nt, k = blockIdx.y, lane = threadIdx.x % 32;
+  const int group = p.Hq / kv.Hkv, rows = 8 * p.row_nt, k = blockIdx.y, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const int hk = head.x % kv.Hkv, entry = head.x / kv.Hkv, rt = entry % p.row_tiles, b = entry / p.row_tiles;
   const int R = rt * rows + k, i = token_of(kv, R, group);
   if (R >= kv.L * group || i >= new_tokens(kv, b)) return;
@@ -847,39 +850,28 @@ __global__ void __launch_bounds__(128) kv4_join_kernel(const Kv4AttnParams p) {
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
   const float z = M == -INFINITY ? 0.f : M;
-  constexpr int V = D == 256 ? 2 : 1;
   float l = 0.f, acc[V] = {};
-  for (int s0 = 0; s0 < shares; s0 += 32) {
-    float f = 0.f;
-    if (s0 + lane < shares) {
-      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + slot(s0 + lane) * 2);
-      f = ex2(ml.x - z);
-      l = fmaf(f, ml.y, l);
-    }
-    const int n = min(32, shares - s0);
-#pragma unroll 8
-    for (int j = 0; j < n; ++j) {
-      const float w = __shfl_sync(0xffffffffu, f, j);
-      if (D < 128 && threadIdx.x >= D) continue;
-      const float* src = p.part_o + slot(s0 + j) * D + threadIdx.x * V;
-      if constexpr (V == 2) {
-        const float2 v = *reinterpret_cast<const float2*>(src);
-        acc[0] = fmaf(w, v.x, acc[0]);
-        acc[1] = fmaf(w, v.y, acc[1]);
-      } else {
-        acc[0] = fmaf(w, *src, acc[0]);
-      }
+#pragma unroll 4
+  for (int s = warp; s < shares; s += 4) {
+    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + slot(s) * 2);
+    const float f = ex2(ml.x - z);
+    l = fmaf(f, ml.y, l);
+    const float* src = p.part_o + slot(s) * D + lane * 2;
+#pragma unroll
+    for (int v = 0; v < V; v += 2) {
+      const float2 x = *reinterpret_cast<const float2*>(src + 32 * v);
+      acc[v] = fmaf(f, x.x, acc[v]);
+      acc[v + 1] = fmaf(f, x.y, acc[v + 1]);
     }
   }
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
-  if (D < 128 && threadIdx.x >= D) return;
+  for (int v = 0; v < V; v += 2) *reinterpret_cast<float2*>(part[warp] + 32 * v + lane * 2) = make_float2(acc[v], acc[v + 1]);
+  if (lane == 0) sums[warp] = l;
+  __syncthreads();
+  l = sums[0] + sums[1] + sums[2] + sums[3];
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  __nv_bfloat16* dst = p.out + b * p.o_bstride + i * p.o_ld + (int64_t)(hk * group + R - i * group) * D + threadIdx.x * V;
-  if constexpr (V == 2)
-    *reinterpret_cast<uint32_t*>(dst) = pack_bf16x2(acc[0] * inv, acc[1] * inv);
-  else
-    *dst = __float2bfloat16_rn(acc[0] * inv);
+  __nv_bfloat16* dst = p.out + b * p.o_bstride + i * p.o_ld + (int64_t)(hk * group + R - i * group) * D;
+  for (int d = threadIdx.x; d < D; d += 128) dst[d] = __float2bfloat16_rn((part[0][d] + part[1][d] + part[2][d] + part[3][d]) * inv);
 }
 
 template <typename T>
