@@ -293,15 +293,6 @@ __device__ __forceinline__ uint32_t load_scale(uint32_t at) {
   return v;
 }
 
-__device__ __forceinline__ void copy16_async(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copy_wait() {   // all but the N latest groups of this lane are done
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
 // Which 16-token blocks the rows at positions pmin .. pmax see: [0, sink_blocks), then from first on; n in all.
 struct Blocks {
   int sink_blocks, first, n;
@@ -368,7 +359,7 @@ struct AttnSmem {
   static constexpr size_t bytes = (q + ring > o ? q + ring : o) + ml;
 };
 
-constexpr int ctas_per_sm(int D, int NT) { return NT == 1 ? (D == 256 ? 3 : 4) : (D == 256 ? 2 : 3); }
+constexpr int ctas_per_sm(int D, int NT) { return NT == 1 ? 3 : 2; }
 
 // NT: tiles of eight query rows.  CL: 1, or the CTAs of a cluster that takes one unit.
 template <int D, int NT, int CL>

@@ -7,6 +7,8 @@
 // at 16 c + 4 i holds the values 32 i + 8 c .. + 7 (nibble order: q4_nibble).
 #include <algorithm>
 
+#include <cooperative_groups.h>
+
 #include "nsa_internal.h"
 #include "ptx.cuh"
 #include "q4.cuh"
@@ -113,21 +115,29 @@ __global__ void __launch_bounds__(256) expand4_kernel(const Quant4Params p, __nv
 // (q4_nibble), so X's own 16 bytes of values 32 i + 8 c .. + 7 are the B fragments.  A nibble n set into a bf16
 // mantissa is 128 + n; minus 136 it is the code, exactly.
 //
-// One CTA of 16 warps per SM takes TN = 16 / WK tiles at a time, the WK warps of a tile its chunks in turn, each
-// with kStages chunks in flight across tile ends, and joins them in shared memory.  The rows of X that the pass
-// covers are staged once per CTA, in the fragments' order.
+// One CTA of 16 warps per SM takes TN = 16 / WK tiles at a time, the WK warps of a tile its chunks in turn.  Each warp
+// copies its chunks into a ring of its own, several ahead of their use and across tile ends; the rows of X that the
+// pass covers are staged once per CTA, in the fragments' order.  With more rows, staging all of K in every CTA would
+// cost more than the weights, so a cluster of CS CTAs shares K: each stages its part of X, goes over the cluster's
+// tiles with it, and the parts of the sums are joined through the shared memories at the end.
 
-constexpr int kStages = 4;
 constexpr int kWarps = 16;
 constexpr int kSmemMax = 227 * 1024;
+constexpr int kMaxCluster = 8;
 
-// Scales of a row's chunk: 128 / G bf16 in one load.
+constexpr int kStages = 3;   // of kStep chunks each
+constexpr int kStep = 2;
+// CTAs per SM where their shared memory allows it: with few rows of X a warp's registers do
+__host__ __device__ constexpr int most_ctas(int NT) { return NT <= 2 ? 2 : 1; }
+__host__ __device__ constexpr int stage_bytes(int G) { return kStep * kRowTile * (kChunk / 2 + kChunk / G * 2); }
+
+// Scales of a row's chunk in shared memory: 128 / G bf16 in one load.
 template <int G>
 struct ChunkScales;
 template <>
 struct ChunkScales<32> {
   uint2 v;
-  __device__ __forceinline__ void load(const __nv_bfloat16* p) { v = __ldg(reinterpret_cast<const uint2*>(p)); }
+  __device__ __forceinline__ void load(const uint8_t* p) { v = *reinterpret_cast<const uint2*>(p); }
   __device__ __forceinline__ float get(int i) const {
     const uint32_t u = i < 2 ? v.x : v.y;
     return __uint_as_float(i % 2 ? u & 0xFFFF0000u : u << 16);
@@ -136,60 +146,89 @@ struct ChunkScales<32> {
 template <>
 struct ChunkScales<64> {
   uint32_t v;
-  __device__ __forceinline__ void load(const __nv_bfloat16* p) { v = __ldg(reinterpret_cast<const uint32_t*>(p)); }
+  __device__ __forceinline__ void load(const uint8_t* p) { v = *reinterpret_cast<const uint32_t*>(p); }
   __device__ __forceinline__ float get(int i) const { return __uint_as_float(i ? v & 0xFFFF0000u : v << 16); }
 };
 template <>
 struct ChunkScales<128> {
-  uint16_t v;
-  __device__ __forceinline__ void load(const __nv_bfloat16* p) { v = __ldg(reinterpret_cast<const uint16_t*>(p)); }
-  __device__ __forceinline__ float get(int) const { return __uint_as_float((uint32_t)v << 16); }
+  uint32_t v;
+  __device__ __forceinline__ void load(const uint8_t* p) { v = *reinterpret_cast<const uint16_t*>(p); }
+  __device__ __forceinline__ float get(int) const { return __uint_as_float(v << 16); }
 };
+
+__device__ __forceinline__ void write_out(const Linear4Params& p, int m, int n, float v) {
+  if (p.bias) v += p.bias[n];
+  const int64_t o = m * p.ldc + n;
+  if (p.out_bf16) static_cast<__nv_bfloat16*>(p.c)[o] = __float2bfloat16_rn(v);
+  else if (p.resid) static_cast<float*>(p.c)[o] += v;
+  else static_cast<float*>(p.c)[o] = v;
+}
 
 // NT: tiles of eight rows of X.
 template <int G, int NT>
-__global__ void __launch_bounds__(kWarps * 32) linear4_kernel(const Linear4Params p) {
-  extern __shared__ __align__(16) uint8_t smem[];
-  constexpr int kOut = 16 * 8 * NT;                              // values of a tile
-  float* red = reinterpret_cast<float*>(smem);                   // [kWarps][m][16]
-  uint4* xs = reinterpret_cast<uint4*>(smem + kWarps * kOut * 4);   // [Kc][4 words i][rows][4 pieces c]
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, r = lane / 4, c = lane % 4;
+__global__ void __launch_bounds__(kWarps * 32, most_ctas(NT)) linear4_kernel(const Linear4Params p) {
+  constexpr int STAGES = kStages, STAGE = stage_bytes(G), CODES = kRowTile * kChunk / 2, SCALES = STAGE / kStep - CODES;   // bytes
+  constexpr int kOut = 16 * 8 * NT;                                 // values of a tile
+  extern __shared__ __align__(128) uint8_t smem[];
+  uint8_t* rings = smem;                                            // [kWarps][STAGES][STAGE]
+  float* red = reinterpret_cast<float*>(smem + kWarps * STAGES * STAGE);   // [kWarps][m][16]
+  uint4* xs = reinterpret_cast<uint4*>(red + kWarps * kOut);        // [chunks][4 words i][rows][4 pieces c]
+  const int lane = threadIdx.x % 32, r = lane / 4, c = lane % 4;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0);
   const int wk = warp % p.WK, tn = warp / p.WK, TN = kWarps / p.WK;
   const int m0 = blockIdx.y * p.rows, rows = min(p.rows, p.M - m0);
-  const int steps = (p.Kc + p.WK - 1) / p.WK;                     // chunks of a tile per warp
-  const int stride = gridDim.x * TN;
-  const int tiles = (p.Nt - (int)blockIdx.x * TN + stride - 1) / stride;   // rounds of this CTA (>= 1)
+  // this CTA's part of K and its cluster's tiles
+  const int rank = blockIdx.x % p.CS, each = (p.Kc + p.CS - 1) / p.CS;
+  const int c0 = min(rank * each, p.Kc), chunks = min(each, p.Kc - c0);
+  const int steps = (each + kStep * p.WK - 1) / (kStep * p.WK);     // of kStep neighbouring chunks of a tile per warp
+  const int first = blockIdx.x / p.CS * TN, stride = gridDim.x / p.CS * TN;
+  const int rounds = (p.Nt - first + stride - 1) / stride;          // tiles of this cluster, TN at a time (>= 1)
+  float* part = reinterpret_cast<float*>(xs + (size_t)each * 16 * p.rows);   // [rounds * TN][rows][16], with CS > 1
 
-  uint4 qa[kStages], qb[kStages];
-  ChunkScales<G> sa[kStages], sb[kStages];
-  int f_tile = blockIdx.x * TN + tn, f_ch = wk, f_left = tiles * steps;   // what the next fetch takes
-  int f_step = 0;
-  const auto fetch = [&](int st) {
-    if (f_left-- > 0 && f_tile < p.Nt && f_ch < p.Kc) {
-      const int64_t at = (int64_t)f_tile * p.Kc + f_ch;
-      const uint4* codes = reinterpret_cast<const uint4*>(p.codes) + at * 64 + r * 4 + c;
-      const __nv_bfloat16* scales = p.scales + (at * 16 + r) * (kChunk / G);
-      qa[st] = __ldg(codes);
-      qb[st] = __ldg(codes + 32);
-      sa[st].load(scales);
-      sb[st].load(scales + 8 * (kChunk / G));
+  // rows of X: some warps a row, or some rows a warp, 16 bytes a lane (zeros past K)
+  {
+    int share = 1;                                                  // warps per row
+    while (2 * share * rows <= kWarps) share *= 2;
+    const uint32_t to = smem_u32(xs);
+    for (int m = warp / share; m < rows; m += kWarps / share) {
+      const __nv_bfloat16* src = p.x + (int64_t)(m0 + m) * p.ldx;
+      for (int w = (warp % share) * 32 + lane; w < chunks * 16; w += share * 32) {
+        const int k = c0 * kChunk + w * 8;
+        copy16_async_fill(to + (((w / 4) * rows + m) * 4 + w % 4) * 16, src + (k < p.K ? k : 0), k < p.K ? 16 : 0);
+      }
     }
-    f_ch += p.WK;
+    copy_commit();
+  }
+
+  const uint32_t ring = smem_u32(rings) + warp * STAGES * STAGE;
+  // a stage: kStep chunks' codes, then their scales
+  const uint8_t* codes = p.codes + lane * 16;
+  const uint8_t* scales = reinterpret_cast<const uint8_t*>(p.scales) + lane * 16;
+  int f_tile = first + tn, f_step = 0, f_stage = 0;                 // what the next fetch takes, and where
+  const auto fetch = [&] {
+    const int ch = (f_step * p.WK + wk) * kStep;
+    if (f_tile < p.Nt && ch < chunks) {
+      const uint64_t at = (uint32_t)f_tile * (uint32_t)p.Kc + (uint32_t)(c0 + ch);
+      const uint32_t to = ring + f_stage * STAGE + lane * 16;
+      const uint8_t* src = codes + at * CODES;
+      copy16_async(to, src);
+      copy16_async(to + 512, src + 512);
+      if (ch + 1 < chunks) {
+        copy16_async(to + 1024, src + 1024);
+        copy16_async(to + 1536, src + 1536);
+      }
+      if (lane * 16 < (ch + 1 < chunks ? 2 : 1) * SCALES) copy16_async(to + kStep * CODES, scales + at * SCALES);
+    }
+    copy_commit();
+    f_stage = f_stage == STAGES - 1 ? 0 : f_stage + 1;
     if (++f_step == steps) {
       f_step = 0;
-      f_ch = wk;
       f_tile += stride;
     }
   };
 #pragma unroll
-  for (int st = 0; st < kStages; ++st) fetch(st);
-
-  for (int e = threadIdx.x; e < p.Kc * 16 * rows; e += kWarps * 32) {
-    const int w = e / rows, m = e % rows;                         // word w of row m: value 8 w
-    const int ch = w / 16, i = w % 16 / 4, cc = w % 4;
-    xs[((ch * 4 + i) * rows + m) * 4 + cc] =
-        w * 8 < p.K ? __ldg(reinterpret_cast<const uint4*>(p.x + (int64_t)(m0 + m) * p.ldx + w * 8)) : make_uint4(0u, 0u, 0u, 0u);
-  }
+  for (int st = 0; st < STAGES - 1; ++st) fetch();
+  copy_wait<STAGES - 1>();   // X
   __syncthreads();
 
   // columns past the pass's rows repeat its last row; they are not stored
@@ -201,34 +240,39 @@ __global__ void __launch_bounds__(kWarps * 32) linear4_kernel(const Linear4Param
   for (int t = 0; t < NT; ++t)
 #pragma unroll
     for (int j = 0; j < 4; ++j) y[t][j] = 0.f;
-  int tile0 = blockIdx.x * TN, step = 0;
-  const int total = tiles * steps;
-  for (int f = 0; f < total; f += kStages) {
-#pragma unroll
-    for (int st = 0; st < kStages; ++st) {
-      if (f + st >= total) break;
-      const int ch = wk + step * p.WK;
-      if (ch < p.Kc && tile0 + tn < p.Nt) {
-        const uint32_t wa[4] = {qa[st].x, qa[st].y, qa[st].z, qa[st].w}, wb[4] = {qb[st].x, qb[st].y, qb[st].z, qb[st].w};
+  int stage = 0;
+  for (int round = 0; round < rounds; ++round) {
+    const int tile0 = first + round * stride;
+    for (int step = 0; step < steps; ++step) {
+      copy_wait<STAGES - 2>();
+      __syncwarp();   // the chunks are there for all lanes, and all lanes are done with the stage that is filled next
+      fetch();
+      const uint8_t* at = rings + (warp * STAGES + stage) * STAGE;
+      stage = stage == STAGES - 1 ? 0 : stage + 1;
+      const int ch = (step * p.WK + wk) * kStep;
+      if (ch >= chunks || tile0 + tn >= p.Nt) continue;
+      const auto multiply = [&](int half) {
+        const uint4 qa = *reinterpret_cast<const uint4*>(at + half * CODES + r * 64 + c * 16);
+        const uint4 qb = *reinterpret_cast<const uint4*>(at + half * CODES + (r + 8) * 64 + c * 16);
+        ChunkScales<G> sa, sb;
+        sa.load(at + kStep * CODES + half * SCALES + r * (kChunk / G * 2));
+        sb.load(at + kStep * CODES + half * SCALES + (r + 8) * (kChunk / G * 2));
+        const uint32_t wa[4] = {qa.x, qa.y, qa.z, qa.w}, wb[4] = {qb.x, qb.y, qb.z, qb.w};
+        const int xo = (ch + half) * 16 * rows;
         float acc[NT][4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          if (32 * i % G == 0) {
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-              for (int j = 0; j < 4; ++j) acc[t][j] = 0.f;
-          }
           const uint32_t a0 = code_pair<0>(wa[i]), a1 = code_pair<0>(wb[i]), a2 = code_pair<1>(wa[i]), a3 = code_pair<1>(wb[i]);
           const uint32_t a4 = code_pair<2>(wa[i]), a5 = code_pair<2>(wb[i]), a6 = code_pair<3>(wa[i]), a7 = code_pair<3>(wb[i]);
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
-            const uint4 x = xt[t][(ch * 4 + i) * rows * 4];
-            mma_bf16(acc[t], a0, a1, a2, a3, x.x, x.y);
+            const uint4 x = xt[t][xo + i * 4 * rows];
+            if (32 * i % G == 0) mma_bf16_zero(acc[t], a0, a1, a2, a3, x.x, x.y);
+            else mma_bf16(acc[t], a0, a1, a2, a3, x.x, x.y);
             mma_bf16(acc[t], a4, a5, a6, a7, x.z, x.w);
           }
           if (32 * (i + 1) % G == 0) {
-            const float fa = sa[st].get(32 * i / G), fb = sb[st].get(32 * i / G);
+            const float fa = sa.get(32 * i / G), fb = sb.get(32 * i / G);
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
               y[t][0] = fmaf(fa, acc[t][0], y[t][0]);
@@ -238,37 +282,43 @@ __global__ void __launch_bounds__(kWarps * 32) linear4_kernel(const Linear4Param
             }
           }
         }
-      }
-      fetch(st);
-      if (++step < steps) continue;
-      // the round's tiles are done: join their warps
-      step = 0;
-      __syncthreads();   // the previous round's sums have been read
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        float* d = red + warp * kOut + (8 * t + 2 * c) * 16 + r;
-        d[0] = y[t][0];
-        d[16] = y[t][1];
-        d[8] = y[t][2];
-        d[24] = y[t][3];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) y[t][j] = 0.f;
-      }
-      __syncthreads();
-      for (int e = threadIdx.x; e < TN * 16 * rows; e += kWarps * 32) {
-        const int g = e / (16 * rows), at = e % (16 * rows);
-        const int m = m0 + at / 16, n = (tile0 + g) * 16 + at % 16;
-        if (n >= p.N) continue;
-        float v = 0.f;
-        for (int w = 0; w < p.WK; ++w) v += red[(g * p.WK + w) * kOut + at];
-        if (p.bias) v += p.bias[n];
-        const int64_t o = m * p.ldc + n;
-        if (p.out_bf16) static_cast<__nv_bfloat16*>(p.c)[o] = __float2bfloat16_rn(v);
-        else if (p.resid) static_cast<float*>(p.c)[o] += v;
-        else static_cast<float*>(p.c)[o] = v;
-      }
-      tile0 += stride;
+      };
+      multiply(0);
+      if (ch + 1 < chunks) multiply(1);
     }
+    // the round's tiles are done: join their warps
+    __syncthreads();   // the previous round's sums have been read
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      float* d = red + warp * kOut + (8 * t + 2 * c) * 16 + r;
+      d[0] = y[t][0];
+      d[16] = y[t][1];
+      d[8] = y[t][2];
+      d[24] = y[t][3];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) y[t][j] = 0.f;
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < TN * kOut; e += kWarps * 32) {
+      const int g = e / kOut, at = e % kOut, m = at / 16, n = (tile0 + g) * 16 + at % 16;
+      if (m >= rows) continue;
+      float v = 0.f;
+      for (int w = 0; w < p.WK; ++w) v += red[(g * p.WK + w) * kOut + at];
+      if (p.CS > 1) part[((round * TN + g) * rows + m) * 16 + at % 16] = v;
+      else if (n < p.N) write_out(p, m0 + m, n, v);
+    }
+  }
+  if (p.CS > 1) {
+    const auto cluster = cooperative_groups::this_cluster();
+    cluster.sync();
+    for (int e = rank * kWarps * 32 + threadIdx.x; e < rounds * TN * rows * 16; e += p.CS * kWarps * 32) {
+      const int j = e / 16 / rows, m = e / 16 - j * rows, n = (first + j / TN * stride + j % TN) * 16 + e % 16;
+      if (n >= p.N) continue;
+      float v = 0.f;
+      for (int k = 0; k < p.CS; ++k) v += *cluster.map_shared_rank(part + e, k);
+      write_out(p, m0 + m, n, v);
+    }
+    cluster.sync();   // no CTA leaves while another reads its shared memory
   }
 }
 
@@ -279,15 +329,23 @@ cudaError_t launch_linear_gn(const Linear4Params& p, dim3 grid, size_t bytes, cu
     return cudaFuncSetAttribute(linear4_kernel<G, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax);
   });
   if (e != cudaSuccess) return e;
-  linear4_kernel<G, NT><<<grid, kWarps * 32, bytes, stream>>>(p);
-  return cudaGetLastError();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(kWarps * 32);
+  cfg.dynamicSmemBytes = bytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute cluster;
+  cluster.id = cudaLaunchAttributeClusterDimension;
+  cluster.val.clusterDim.x = p.CS;
+  cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+  cfg.attrs = &cluster;
+  cfg.numAttrs = p.CS > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, linear4_kernel<G, NT>, p);
 }
 
 template <int G>
-cudaError_t launch_linear_g(const Linear4Params& p, dim3 grid, cudaStream_t stream) {
-  const int nt = (p.rows + 7) / 8;
-  const size_t bytes = (size_t)kWarps * 16 * 8 * nt * 4 + (size_t)p.rows * p.Kc * kChunk * 2;
-  switch (nt) {
+cudaError_t launch_linear_g(const Linear4Params& p, dim3 grid, size_t bytes, cudaStream_t stream) {
+  switch ((p.rows + 7) / 8) {
     case 1: return launch_linear_gn<G, 1>(p, grid, bytes, stream);
     case 2: return launch_linear_gn<G, 2>(p, grid, bytes, stream);
     case 3: return launch_linear_gn<G, 3>(p, grid, bytes, stream);
@@ -326,29 +384,60 @@ cudaError_t launch_expand4(const Quant4Params& p, __nv_bfloat16* out, int64_t ld
   return cudaGetLastError();
 }
 
-// Rows of X per pass: up to 32, as many as shared memory holds beside the joins, evenly over the passes.
-// Warps per tile: the number with the fewest steps of a warp (rounds of tiles times chunks per warp); of equal
-// ones the largest, whose joins are the fewest tiles at a time.
+namespace {
+
+// A way to share the work of a pass of `rows` rows, and its estimated cycles.
+struct Linear4Plan {
+  int WK, CS, clusters;
+  size_t bytes;
+  double cost;
+};
+
+Linear4Plan linear4_plan(const Linear4Params& p, int rows, int sms) {
+  const int nt = (rows + 7) / 8;
+  Linear4Plan best{0, 0, 0, 0, 1e30};
+  for (int cs = 1; cs <= kMaxCluster; cs *= 2) {
+    if (cs > 1 && cs > p.Kc) break;
+    for (int per_sm = most_ctas(nt); per_sm >= 1; --per_sm) {
+      // clusters of 8 or 4 CTAs leave a few SMs of a processing cluster over
+      const int clusters = per_sm * (cs == 1 ? sms : cs == 2 ? sms / 2 : cs == 4 ? sms / 4 - 1 : sms / 8 - 2);
+      const int64_t each = (p.Kc + cs - 1) / cs;
+      for (int wk = kWarps; wk >= 1; wk /= 2) {
+        const int64_t tn = kWarps / wk, rounds = (p.Nt + tn * clusters - 1) / (tn * clusters);
+        const size_t bytes = (size_t)kWarps * kStages * stage_bytes(p.G) + (size_t)kWarps * 16 * 8 * nt * 4 +
+                             (size_t)each * 256 * rows + (cs > 1 ? (size_t)rounds * tn * rows * 64 : 0);
+        if (per_sm * (bytes + 1024) > kSmemMax + 1024) continue;
+        // a step: the instructions of a scheduler's warps; a round: its join; X at about 48 bytes a cycle; a
+        // cluster's join
+        const double cost = (double)rounds * ((each + kStep * wk - 1) / (kStep * wk)) * kStep * 4 * per_sm * (150 + 50 * nt) * (per_sm == 1 ? 1.6 : 1.2) +
+                            rounds * (per_sm == 1 ? 800.0 : 400.0) + each * 256.0 * rows / 48 + (cs > 1 ? 1500.0 : 0.0);
+        if (cost < best.cost) best = {wk, cs, (int)std::min<int64_t>(clusters, (p.Nt + tn - 1) / tn), bytes, cost};
+      }
+    }
+  }
+  return best;
+}
+
+}  // namespace
+
+// Rows of X per pass: up to 32, fewer where no cluster holds them, evenly over the passes.
 cudaError_t launch_linear4(Linear4Params p, cudaStream_t stream) {
-  if (p.Kc > kLinear4MaxK / kChunk) return cudaErrorInvalidValue;
   const int sms = device_sm_count();
-  int rows = 32;
-  while (rows > 1 && (size_t)kWarps * 16 * 4 * ((rows + 7) / 8 * 8) + (size_t)rows * p.Kc * kChunk * 2 > kSmemMax) --rows;
+  int rows = std::min(p.M, 32);
+  Linear4Plan plan = linear4_plan(p, rows, sms);
+  while (plan.WK == 0 && rows > 1) plan = linear4_plan(p, --rows, sms);
+  if (plan.WK == 0) return cudaErrorInvalidValue;
   const int passes = (p.M + rows - 1) / rows;
   if (passes > 65535) return cudaErrorInvalidValue;
   p.rows = (p.M + passes - 1) / passes;
-  int64_t best = INT64_MAX;
-  for (int wk = kWarps; wk >= 1; wk /= 2) {
-    const int64_t tn = kWarps / wk;
-    const int64_t steps = (p.Nt + tn * sms - 1) / (tn * sms) * ((p.Kc + wk - 1) / wk);
-    if (steps < best) best = steps, p.WK = wk;
-  }
-  const int tn = kWarps / p.WK;
-  const dim3 grid((unsigned)std::min((p.Nt + tn - 1) / tn, sms), (unsigned)passes);
+  if (p.rows < rows) plan = linear4_plan(p, p.rows, sms);
+  p.WK = plan.WK;
+  p.CS = plan.CS;
+  const dim3 grid((unsigned)(plan.clusters * p.CS), (unsigned)passes);
   switch (p.G) {
-    case 32: return launch_linear_g<32>(p, grid, stream);
-    case 64: return launch_linear_g<64>(p, grid, stream);
-    default: return launch_linear_g<128>(p, grid, stream);
+    case 32: return launch_linear_g<32>(p, grid, plan.bytes, stream);
+    case 64: return launch_linear_g<64>(p, grid, plan.bytes, stream);
+    default: return launch_linear_g<128>(p, grid, plan.bytes, stream);
   }
 }
 

@@ -303,9 +303,10 @@ struct Linear4Params {
   int out_bf16, resid;
   // set by the launch
   int WK;                   // warps that share a row tile's chunks
+  int CS;                   // CTAs of a cluster that share K
   int rows;                 // rows of X a pass covers
 };
-constexpr int kLinear4MaxK = 98304;   // one row of X in shared memory beside the joins
+constexpr int kLinear4MaxK = 98304;   // a row of X in the shared memories of a cluster, with room to spare
 cudaError_t launch_linear4(Linear4Params p, cudaStream_t stream);
 
 // 4-bit paged key/value cache (kv4.cu).

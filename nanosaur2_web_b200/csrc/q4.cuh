@@ -139,4 +139,18 @@ __device__ __forceinline__ void mma_bf16_zero(float* c, uint32_t a0, uint32_t a1
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 
+// Asynchronous 16-byte copies to shared memory (shared address, global source).
+__device__ __forceinline__ void copy16_async(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {   // all but the N latest groups of this lane are done
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+// The first `bytes` (0 or 16) of the source, zeros after them.
+__device__ __forceinline__ void copy16_async_fill(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+
 }  // namespace nsa
