@@ -82,26 +82,32 @@ nsa_weight4 weight(const Tensor& codes, const Tensor& scales, int64_t N, int64_t
   return {int32_of(N, "N"), int32_of(K, "K"), (int32_t)group, codes.data_ptr<uint8_t>(), scales.data_ptr()};
 }
 
-void quantize4(const Tensor& W, const Tensor& codes, const Tensor& scales, int64_t group) {
-  const auto dev = Devices()(W)(codes)(scales).index();
+std::pair<Tensor, Tensor> quantize4(const Tensor& W, int64_t group, const OptTensor& codes_, const OptTensor& scales_) {
+  const auto dev = Devices()(W)(codes_)(scales_).index();
   if (W.dim() != 2 || W.size(0) < 1 || W.size(1) < 1 || (W.size(1) > 1 && W.stride(1) != 1))
     invalid("W must be a non-empty [N, K] tensor with unit inner stride");
-  const int64_t N = W.size(0), K = W.size(1);
-  const nsa_weight4 w = weight(codes, scales, N, K, group);
-  const int64_t ld = N > 1 ? W.stride(0) : K;
+  const int64_t N = W.size(0), K = W.size(1), ld = N > 1 ? W.stride(0) : K;
   if (ld < K) invalid("the rows of W must not overlap");
+  if (group != 32 && group != 64 && group != 128) invalid("group must be 32, 64 or 128");
   OnDevice on(dev);
+  const int64_t t = (N + 15) / 16, k = (K + 127) / 128;
+  Tensor codes = codes_ ? *codes_ : at::empty({t, k, 16, 64}, W.options().dtype(at::kByte));
+  Tensor scales = scales_ ? *scales_ : at::empty({t, k, 16, 128 / group}, W.options().dtype(at::kBFloat16));
+  const nsa_weight4 w = weight(codes, scales, N, K, group);
   check(nsa_quantize4(&w, W.data_ptr(), dtype_code(W, "W"), ld, on.stream));
+  return {codes, scales};
 }
 
-void expand4(const Tensor& codes, const Tensor& scales, int64_t N, int64_t K, int64_t group, const Tensor& out) {
-  const auto dev = Devices()(codes)(scales)(out).index();
+Tensor expand4(const Tensor& codes, const Tensor& scales, int64_t N, int64_t K, int64_t group, const OptTensor& out_) {
+  const auto dev = Devices()(codes)(scales)(out_).index();
   const nsa_weight4 w = weight(codes, scales, N, K, group);
+  OnDevice on(dev);
+  const Tensor out = out_ ? *out_ : at::empty({N, K}, scales.options());
   if (out.scalar_type() != at::kBFloat16 || out.sizes() != at::IntArrayRef({N, K}) || (K > 1 && out.stride(1) != 1) ||
       (N > 1 && out.stride(0) < K))
     invalid("out must be a bfloat16 [N, K] tensor with unit inner stride");
-  OnDevice on(dev);
   check(nsa_expand4(&w, out.data_ptr(), N > 1 ? out.stride(0) : K, on.stream));
+  return out;
 }
 
 Tensor linear4(const Tensor& x, const Tensor& codes, const Tensor& scales, int64_t N, int64_t K, int64_t group,

@@ -444,25 +444,19 @@ def quantize4(W: torch.Tensor, group: int = 32, out: Optional[Weight4] = None) -
     if W.dim() != 2 or not W.numel():
         raise _invalid("W must be a non-empty [N, K] tensor with unit inner stride")
     N, K = W.shape
-    if group not in (32, 64, 128):
-        raise _invalid("group must be 32, 64 or 128")
-    if out is None:
-        t, k = (N + 15) // 16, (K + 127) // 128
-        out = Weight4(W.new_empty((t, k, 16, 64), dtype=torch.uint8),
-                      W.new_empty((t, k, 16, 128 // group), dtype=torch.bfloat16), N, K, group)
-    elif (out.N, out.K, out.group) != (N, K, group):
+    if out is not None and (out.N, out.K, out.group) != (N, K, group):
         raise _invalid(f"out is [{out.N}, {out.K}] in groups of {out.group}, W [{N}, {K}] in groups of {group}")
-    _native().quantize4(W, out.codes, out.scales, group)
+    if out is None:
+        codes, scales = _native().quantize4(W, group, None, None)
+        return Weight4(codes, scales, N, K, group)
+    _native().quantize4(W, group, out.codes, out.scales)
     return out
 
 
 def expand4(W: Weight4, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """A 4-bit weight's values as bf16 [N, K] (nsa_expand4; exact for ``quantize4``'s scales): the weight
     ``linear`` takes when a prompt brings many rows."""
-    if out is None:
-        out = W.scales.new_empty((W.N, W.K))
-    _native().expand4(W.codes, W.scales, W.N, W.K, W.group, out)
-    return out
+    return _native().expand4(W.codes, W.scales, W.N, W.K, W.group, out)
 
 
 def linear4(x: torch.Tensor, W: Weight4, *, bias: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,

@@ -156,8 +156,6 @@ def test_wrappers_refuse_host_tensors_and_wrong_shapes():
                  lambda: ops.kv4_append(torch.zeros((1, 1, 192)), cache, table, start, Hq=1, q_norm=w, k_norm=w, cs=None)):
         with pytest.raises(ops.NsaError, match="CUDA"):
             call()
-    with pytest.raises(ops.NsaError, match="group"):
-        ops.quantize4(x, 48)
     with pytest.raises(ops.NsaError, match="non-empty"):
         ops.quantize4(torch.zeros((0, 4)))
     with pytest.raises(ops.NsaError, match="head dims"):

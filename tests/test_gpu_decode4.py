@@ -180,6 +180,77 @@ def test_linear4_empty_and_other_stream():
     assert torch.equal(y, linear4(x, W))
 
 
+def test_weight_wrappers_refuse_and_reuse():
+    from nanosaur2_web_b200 import ops
+    W = torch.randn((20, 96), device=DEV)
+    q = ops.quantize4(W, 64)
+    again = ops.quantize4(W.bfloat16(), 64, out=q)
+    assert again is q and torch.equal(ops.expand4(q), ops.expand4(ops.quantize4(W.bfloat16(), 64)))
+    x = torch.randn((3, 96), device=DEV).bfloat16()
+    calls = [(lambda: ops.quantize4(W, 48), "group"), (lambda: ops.quantize4(W.T), "unit inner stride"),
+             (lambda: ops.quantize4(W[:1].expand(4, 96)), "overlap"), (lambda: ops.quantize4(W, 32, out=q), "groups of"),
+             (lambda: ops.quantize4(W.half()), "float32 or bfloat16"),
+             (lambda: ops.expand4(q, torch.empty((20, 96), device=DEV)), "bfloat16"),
+             (lambda: ops.linear4(x.float(), q), "bf16"), (lambda: ops.linear4(x[:, :88], q), "unit inner stride"),
+             (lambda: ops.linear4(x, q, bias=torch.zeros(19, device=DEV)), "bias"),
+             (lambda: ops.linear4(x, q, resid=True), "resid needs out"),
+             (lambda: ops.linear4(x, q, out=torch.zeros((3, 20), device=DEV, dtype=BF), resid=True), "resid"),
+             (lambda: ops.linear4(x, q, out=torch.zeros((1, 20), device=DEV).expand(3, 20)), "overlap"),
+             (lambda: ops.linear4(x, q, out_dtype=torch.float16), "float32 or bfloat16"),
+             (lambda: ops.linear4(x, ops.Weight4(q.codes, q.scales, 20, 200, 64)), "contiguous codes"),
+             (lambda: ops.linear4(x, ops.Weight4(q.codes, q.scales.float(), 20, 96, 64)), "contiguous codes"),
+             (lambda: ops.linear4(x.cpu(), q), "CUDA")]
+    for call, match in calls:
+        with pytest.raises(ops.NsaError, match=match):
+            call()
+
+
+def test_cache_wrappers_refuse():
+    from nanosaur2_web_b200 import ops
+    c = ops.kv4_cache(4, 2, 64, 16, DEV)
+    table, start = t([[0, 1], [2, 3]], torch.int32), t([3, 5], torch.int32)
+    q = torch.zeros((2, 1, 4 * 64), dtype=BF, device=DEV)
+    x, w = torch.zeros((2, 1, 8 * 64), device=DEV), torch.ones(64, device=DEV)
+    cs = ops.ropeTable(32, 64, 1e4, DEV)
+
+    def append(**kw):
+        a = dict(qkv=x, cache=c, table=table, start=start, Hq=4, q_norm=w, k_norm=w, cs=cs)
+        a.update(kw)
+        return ops.kv4_append(a.pop("qkv"), a.pop("cache"), a.pop("table"), a.pop("start"), **a)
+    append()
+    calls = [(lambda: ops.kv4_attention(q.float(), c, table, start), "bfloat16"),
+             (lambda: ops.kv4_attention(q[:, :, :100], c, table, start), "whole heads"),
+             (lambda: ops.kv4_attention(q[:, :, :64], c, table, start), "multiple of Hkv"),
+             (lambda: ops.kv4_attention(q, c, table.long(), start), "int32"),
+             (lambda: ops.kv4_attention(q, c, table[:1], start), "table"),
+             (lambda: ops.kv4_attention(q, c, table, start[:1]), "start"),
+             (lambda: ops.kv4_attention(q, c, table, start, count=start.long()), "count"),
+             (lambda: ops.kv4_attention(q, c, table, start, sinks=4), "window"),
+             (lambda: ops.kv4_attention(q, c, table, start, window=-1), "window"),
+             (lambda: ops.kv4_attention(q, c, table, start, scale=float("nan")), "scale"),
+             (lambda: ops.kv4_attention(q, c, table, start, out=q), "overlap"),
+             (lambda: ops.kv4_attention(q, c, table, start, workspace=torch.zeros(4, device=DEV)), "uint8"),
+             (lambda: ops.kv4_attention(q, ops.Kv4Cache(c.codes, c.scales[:, :1]), table, start), "contiguous codes"),
+             (lambda: ops.kv4_read(c, table, start, -1), "L >= 0"),
+             (lambda: ops.kv4_read(c, table, start, 1, out=torch.zeros((2, 1, 128), dtype=BF, device=DEV)), "bfloat16"),
+             (lambda: append(Hq=3), "multiple of Hkv"), (lambda: append(Hq=8), "inside"), (lambda: append(vOff=480), "inside"),
+             (lambda: append(qkv=x.half()), "float32 or bfloat16"), (lambda: append(q_norm=w[:32]), "float32 .64."),
+             (lambda: append(cs=ops.ropeTable(32, 128, 1e4, DEV)), "head dim"),
+             (lambda: append(cs=ops.RopeTable(cs.buf, cs.sinOff, 33, 64)), "head dim"), (lambda: append(eps=-1.0), "eps"),
+             (lambda: append(out=torch.zeros((2, 1, 512), dtype=BF, device=DEV)), "bfloat16"),
+             (lambda: append(start=start.cpu()), "CUDA")]
+    for call, match in calls:
+        with pytest.raises(ops.NsaError, match=match):
+            call()
+    # a table that broadcasts one row, and a workspace that is too small for a call that needs one
+    same = table[:1].expand(2, 2)
+    assert torch.equal(ops.kv4_read(c, same, start, 2), ops.kv4_read(c, same.contiguous(), start, 2))
+    big = torch.zeros((2, 1024), dtype=torch.int32, device=DEV)
+    with pytest.raises(ops.NsaError, match="workspace of"):
+        ops.kv4_attention(q, c, big, start, workspace=torch.zeros(16, dtype=torch.uint8, device=DEV))
+    check_device()
+
+
 # --------------------------------------------------------------------------------------------- cache
 
 class Cached:
