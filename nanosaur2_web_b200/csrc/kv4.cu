@@ -59,66 +59,50 @@ __device__ __forceinline__ void load4(const __nv_bfloat16* src, float* x) {
   x[2] = __uint_as_float(v.y << 16); x[3] = __uint_as_float(v.y & 0xFFFF0000u);
 }
 
-// RMSNorm and rotation of one head held by LANES lanes: x[0..3] are elements 4 hl .. of the first half, x[4..7] their
-// partners in the second; w the weights alike; c, s the cosines and sines of the four pairs.
+// Of one head held by LANES lanes: x[0..3] are elements 4 hl .. of the first half, x[4..7] their partners in the second.
+// 1 / rms of the head.
 template <typename T, int LANES>
-__device__ __forceinline__ void norm_rope(const float* x, const float* w, const float* c, const float* s, bool rope, float eps,
-                                          T* out) {
+__device__ __forceinline__ T inv_rms(const float* x, float eps) {
   T ss = 0;
 #pragma unroll
   for (int e = 0; e < 8; ++e) ss += (T)x[e] * (T)x[e];
 #pragma unroll
   for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-  T r;
-  if constexpr (sizeof(T) == 8)
-    r = rsqrt(ss * (1.0 / (8 * LANES)) + (double)eps);
-  else
-    r = rsqrtf(ss * (1.f / (8 * LANES)) + eps);
-#pragma unroll
-  for (int e = 0; e < 8; ++e) out[e] = (T)x[e] * r * (T)w[e];
-  if (rope) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const T a = out[e], b = out[4 + e];
-      out[e] = a * (T)c[e] - b * (T)s[e];
-      out[4 + e] = b * (T)c[e] + a * (T)s[e];
-    }
-  }
+  if constexpr (sizeof(T) == 8) return rsqrt(ss * (1.0 / (8 * LANES)) + (double)eps);
+  else return rsqrtf(ss * (1.f / (8 * LANES)) + eps);
 }
 
-// A lane's four values of each half of a head's row of the cache (the group of 32 is eight lanes): even lanes store the
-// pair's word of the first half, odd lanes that of the second.
-template <bool SHORT, typename T>
-__device__ __forceinline__ void store_codes(const T* x, uint8_t* codes, __nv_bfloat16* scales, int hl, int half, bool live) {
-  float s[2];
-  uint32_t bits[2];
-#pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    float xf[4], am = 0.f;
+// The norm weights with the rotation folded in: out[e] = r (x[e] own[e] + x[e ^ 4] mate[e]).
+struct Turn {
+  float own[8], mate[8];
+};
+__device__ __forceinline__ Turn turn_of(const float* w, const float* cs, int64_t sin_off, int64_t row, int half, int hl) {
+  Turn t;
+  float v[8];
+  load4(w + hl * 4, v);
+  load4(w + half + hl * 4, v + 4);
+  if (cs) {
+    float c[4], s[4];
+    load4(cs + row * half + hl * 4, c);
+    load4(cs + sin_off + row * half + hl * 4, s);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      xf[e] = (float)x[4 * k + e];
-      am = amax2(fabsf(xf[e]), am);
+      t.own[e] = v[e] * c[e];
+      t.mate[e] = -v[4 + e] * s[e];
+      t.own[4 + e] = v[4 + e] * c[e];
+      t.mate[4 + e] = v[e] * s[e];
     }
+  } else {
 #pragma unroll
-    for (int o = 1; o < 8; o <<= 1) am = amax2(__shfl_xor_sync(0xffffffffu, am, o), am);
-    s[k] = q4_scale(am);
-    if constexpr (sizeof(T) == 8) {
-      // fp64: where the rounded largest magnitude lies next to a border of two scales, the exact one decides (the
-      // eight lanes of a group agree on it)
-      const float below = __uint_as_float(__float_as_uint(s[k]) - 0x00080000u), near = am * 0x1p-22f;
-      if (fabsf(7.f * s[k] - am) <= near || fabsf(7.f * below - am) <= near || fabsf(am - 0x1p-110f) <= near || !isfinite(am)) {
-        const unsigned lanes = 0xFFu << (threadIdx.x & 24);
-        double exact = 0.0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) exact = amax2(fabs((double)x[4 * k + e]), exact);
-#pragma unroll
-        for (int o = 1; o < 8; o <<= 1) exact = amax2(__shfl_xor_sync(lanes, exact, o), exact);
-        s[k] = q4_scale(exact);
-      }
-    }
-    bits[k] = s[k] > 0.f ? q4_bits<4, q4_in_order, SHORT>(x + 4 * k, xf, s[k], am) : 0x8888u;
+    for (int e = 0; e < 8; ++e) t.own[e] = v[e], t.mate[e] = 0.f;
   }
+  return t;
+}
+
+// A lane's packed codes of its four values of each half and their scales into the head's row of the cache: even lanes
+// store the pair's word of the first half, odd lanes that of the second.
+__device__ __forceinline__ void store_bits(const uint32_t* bits, const float* s, uint8_t* codes, __nv_bfloat16* scales, int hl,
+                                           int half, bool live) {
   const bool odd = hl & 1;
   const uint32_t got = __shfl_xor_sync(0xffffffffu, odd ? bits[0] : bits[1], 1);
   if (!live) return;
@@ -127,16 +111,67 @@ __device__ __forceinline__ void store_codes(const T* x, uint8_t* codes, __nv_bfl
   if (hl % 8 < 2) scales[(odd ? half / kKvGroup : 0) + hl / 8] = __float2bfloat16_rn(odd ? s[1] : s[0]);
 }
 
-// A CTA per token; a warp takes 256 / D heads of one kind (q, k or v) at a time, eight values a lane.  Bound by the
-// bytes of q | k | v.  Keys are computed in fp64: the code of a value next to the border of two codes is
-// decided by the last bits, and the fp32 order of sums would decide it by chance.
+// Scales and codes of a lane's values (a group of 32 is eight lanes), from x in T.
+template <bool SHORT, typename T>
+__device__ __forceinline__ void quantise_halves(const T* x, uint32_t* bits, float* s) {
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    T am = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) am = amax2((T)fabs(x[4 * k + e]), am);
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) am = amax2(__shfl_xor_sync(0xffffffffu, am, o), am);
+    s[k] = q4_scale(am);
+    if (!(s[k] > 0.f)) bits[k] = 0x8888u;
+    else if constexpr (sizeof(T) == 8) bits[k] = q4_bits_exact<4, q4_in_order>(x + 4 * k, s[k]);
+    else bits[k] = q4_bits<4, q4_in_order, SHORT>(x + 4 * k, x + 4 * k, s[k], am);
+  }
+}
+
+// Keys.  The definition is in fp64: the code of a value next to the border of two codes is decided by the last bits, and
+// the fp32 order of sums would decide it by chance.  So fp32 decides where its error cannot matter.  The error of a
+// value is below 2^-19 r (|x own| + |mate's x mate|): 2^-22 of rsqrtf, half of 15 roundings of the mean square under its
+// root, five of the products.  A lane answers false where that is more than 2^-17 of the group's largest magnitude am, where am lies within
+// 2^-16 of a border of two scales, or where a code changes within +- 2^-17 am (with 2^-20 of x for 1 / s).
+__device__ __forceinline__ bool quantise_keys(const float* x, const Turn& t, float r, uint32_t* bits, float* s) {
+  bool sure = true;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    float v[4], am = 0.f, off = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float p0 = x[4 * k + e] * t.own[4 * k + e], p1 = x[4 * (1 - k) + e] * t.mate[4 * k + e];
+      v[e] = (p0 + p1) * r;
+      off = fmaxf(off, fabsf(p0) + fabsf(p1));
+      am = amax2(fabsf(v[e]), am);
+    }
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) am = amax2(__shfl_xor_sync(0xffffffffu, am, o), am);
+    s[k] = q4_scale(am);
+    const float below = __uint_as_float(__float_as_uint(s[k]) - 0x00080000u), near = am * 0x1p-16f, step = am * 0x1p-17f;
+    sure = sure && off * r * 0x1p-19f <= step && fabsf(7.f * s[k] - am) > near && fabsf(7.f * below - am) > near &&
+           am > 0x1p-109f && am < 0x1p119f;   // (no number: false)
+    const float inv = __fdividef(1.f, s[k]), lo = inv * (1.f - 0x1p-20f), hi = inv * (1.f + 0x1p-20f);
+    bits[k] = 0u - 0x4B400000u * 0x1111u;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t n = q4_round(fabsf(v[e]) - step, lo);   // magnitudes: the code's distance from 8
+      sure = sure && n == q4_round(fabsf(v[e]) + step, hi);
+      bits[k] += (v[e] < 0.f ? 16u - (n - 0x4B400000u) + 0x4B400000u : n) * (1u << (4 * e));
+    }
+  }
+  return sure;
+}
+
+// A CTA per token; a warp takes 256 / D heads of one kind (q, k or v) at a time, eight values a lane.  Instructions bound it
+// rather than the bytes of q | k | v: unpacking, norms and codes of a value cost about ten.
 template <typename T, int D>
-__global__ void __launch_bounds__(256, 3) kv4_append_kernel(const Kv4AppendParams p) {
+__global__ void __launch_bounds__(256, 6) kv4_append_kernel(const Kv4AppendParams p) {
   constexpr int LANES = D / 8, HPW = 32 / LANES, half = D / 2;
   const Kv4Params& kv = p.kv;
-  const int lane = threadIdx.x % 32, hl = lane % LANES;
+  const int lane = threadIdx.x % 32, hl = lane % LANES, warps = blockDim.x / 32;
   const int q_slots = (p.Hq + HPW - 1) / HPW, kv_slots = (kv.Hkv + HPW - 1) / HPW;
-  const int b = blockIdx.x / kv.L, i = blockIdx.x % kv.L;
+  const int b = blockIdx.x / kv.L, i = blockIdx.x - b * kv.L;
   if (i >= new_tokens(kv, b)) return;
   const int pos = position(kv, b, i);
   if (pos < 0) return;
@@ -144,77 +179,114 @@ __global__ void __launch_bounds__(256, 3) kv4_append_kernel(const Kv4AppendParam
     if (threadIdx.x == 0) atomicCAS(kv.err, 0, kErrKvPosition);
     return;
   }
-  const T* row = static_cast<const T*>(p.qkv) + b * p.bstride + i * p.ld;
-  for (int slot = threadIdx.x / 32; slot < q_slots + 2 * kv_slots; slot += blockDim.x / 32) {
-    const int kind = slot < q_slots ? 0 : slot < q_slots + kv_slots ? 1 : 2;
-    const int heads = kind == 0 ? p.Hq : kv.Hkv;
-    const int h = (kind == 0 ? slot : slot - q_slots - (kind - 1) * kv_slots) * HPW + lane / LANES;
-    const bool live = h < heads;                                   // lanes past the last head repeat it, storing nothing
-    const int hh = live ? h : heads - 1;
-    const T* src = row + (kind == 0 ? p.q_off : kind == 1 ? p.k_off : p.v_off) + (int64_t)hh * D + hl * 4;
-    float x[8], w[8], c[4], s[4];
-    load4(src, x);
-    load4(src + half, x + 4);
-    if (kind < 2) {
-      const float* wt = (kind == 0 ? p.q_w : p.k_w) + hl * 4;
-      load4(wt, w);
-      load4(wt + half, w + 4);
-      if (p.cs) {
-        const float* t = p.cs + (int64_t)pos * half + hl * 4;
-        load4(t, c);
-        load4(t + p.sin_off, s);
-      }
-    }
-    if (kind == 0) {
-      float o[8];
-      norm_rope<float, LANES>(x, w, c, s, p.cs != nullptr, p.eps, o);
+  const T* row = static_cast<const T*>(p.qkv) + b * p.bstride + i * p.ld + hl * 4;
+  int slot = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0);
+  if (slot < q_slots) {
+    const Turn t = turn_of(p.q_w, p.cs, p.sin_off, pos, half, hl);
+    __nv_bfloat16* out = p.q_out + b * p.qo_bstride + i * p.qo_ld + hl * 4;
+    for (; slot < q_slots; slot += warps) {
+      const int h = slot * HPW + lane / LANES;
+      const bool live = h < p.Hq;                                  // lanes past the last head repeat it, storing nothing
+      const int at = (live ? h : p.Hq - 1) * D;
+      float x[8], o[8];
+      load4(row + p.q_off + at, x);
+      load4(row + p.q_off + at + half, x + 4);
+      const float r = inv_rms<float, LANES>(x, p.eps);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] = fmaf(x[e ^ 4], t.mate[e], x[e] * t.own[e]) * r;
       if (live) {
-        __nv_bfloat16* dst = p.q_out + b * p.qo_bstride + i * p.qo_ld + (int64_t)hh * D + hl * 4;
-        *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]));
-        *reinterpret_cast<uint2*>(dst + half) = make_uint2(pack_bf16x2(o[4], o[5]), pack_bf16x2(o[6], o[7]));
+        *reinterpret_cast<uint2*>(out + at) = make_uint2(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]));
+        *reinterpret_cast<uint2*>(out + at + half) = make_uint2(pack_bf16x2(o[4], o[5]), pack_bf16x2(o[6], o[7]));
       }
-      continue;
     }
-    const int page = page_of(kv, b, pos);
-    if (page < 0) return;
-    const int64_t tok = cache_row(kv, page, kind - 1, hh, pos);
+  }
+  if (slot >= q_slots + 2 * kv_slots) return;
+  const int page = page_of(kv, b, pos);
+  if (page < 0) return;
+  for (slot -= q_slots; slot < 2 * kv_slots; slot += warps) {
+    const int which = slot < kv_slots ? 0 : 1;
+    const int h = (slot - which * kv_slots) * HPW + lane / LANES;
+    const bool live = h < kv.Hkv;
+    const int hh = live ? h : kv.Hkv - 1;
+    const int64_t tok = cache_row(kv, page, which, hh, pos);
     uint8_t* codes = kv.codes + tok * (D / 2);
     __nv_bfloat16* scales = kv.scales + tok * (D / kKvGroup);
-    if (kind == 1) {
-      double o[8];
-      norm_rope<double, LANES>(x, w, c, s, p.cs != nullptr, p.eps, o);
-      store_codes<false>(o, codes, scales, hl, half, live);
+    const T* src = row + (which ? p.v_off : p.k_off) + (int64_t)hh * D;
+    float x[8], s[2];
+    uint32_t bits[2];
+    load4(src, x);
+    load4(src + half, x + 4);
+    if (which) {
+      quantise_halves<sizeof(T) == 2>(x, bits, s);
     } else {
-      store_codes<sizeof(T) == 2>(x, codes, scales, hl, half, live);
+      const Turn t = turn_of(p.k_w, p.cs, p.sin_off, pos, half, hl);
+      if (__any_sync(0xffffffffu, !quantise_keys(x, t, inv_rms<float, LANES>(x, p.eps), bits, s))) {
+        float w[8], c[4], sn[4];
+        double y[8];
+        load4(p.k_w + hl * 4, w);
+        load4(p.k_w + half + hl * 4, w + 4);
+        const double r = inv_rms<double, LANES>(x, p.eps);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = (double)x[e] * r * (double)w[e];
+        if (p.cs) {
+          load4(p.cs + (int64_t)pos * half + hl * 4, c);
+          load4(p.cs + p.sin_off + (int64_t)pos * half + hl * 4, sn);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const double a = y[e], b2 = y[4 + e];
+            y[e] = a * (double)c[e] - b2 * (double)sn[e];
+            y[4 + e] = b2 * (double)c[e] + a * (double)sn[e];
+          }
+        }
+        quantise_halves<false>(y, bits, s);
+      }
     }
+    store_bits(bits, s, codes, scales, hl, half, live);
   }
 }
 
-// A CTA per row, a thread per word (8 values).
+// A CTA per R rows, a thread per word (8 values) of each: the rows' loads are under way together.
+template <int R>
 __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4Params p, __nv_bfloat16* __restrict__ out, int64_t ldo,
                                                        int64_t bstride) {
-  const int b = blockIdx.x / p.L, i = blockIdx.x % p.L;
-  if (i >= new_tokens(p, b)) return;
-  const int pos = position(p, b, i);
-  if (pos < 0) return;
-  const int page = page_of(p, b, pos);
-  if (page < 0) return;
-  const int words = p.D / 8;
+  const int words = p.D / 8, shift = 31 - __clz(words);
+  int64_t tok[R], to[R];
+#pragma unroll
+  for (int k = 0; k < R; ++k) {
+    const int64_t row = (int64_t)blockIdx.x * R + k;
+    tok[k] = -1;
+    if (row >= (int64_t)p.B * p.L) continue;
+    const int b = (int)(row / p.L), i = (int)(row - (int64_t)b * p.L);
+    if (i >= new_tokens(p, b)) continue;
+    const int pos = position(p, b, i);
+    if (pos < 0) continue;
+    const int page = page_of(p, b, pos);
+    if (page < 0) continue;
+    tok[k] = cache_row(p, page, 0, 0, pos);
+    to[k] = b * bstride + i * ldo;
+  }
   for (int e = threadIdx.x; e < 2 * p.Hkv * words; e += blockDim.x) {
-    const int w = e % words, h = e / words;                        // h: key heads, then value heads
-    const int64_t tok = cache_row(p, page, 0, h, pos);             // heads of both halves follow one another
-    const uint32_t v = __ldg(reinterpret_cast<const uint32_t*>(p.codes + tok * (p.D / 2)) + w);
-    const uint16_t sc = __ldg(reinterpret_cast<const uint16_t*>(p.scales) + tok * (p.D / kKvGroup) + w * 8 / kKvGroup);
-    uint32_t s2;
-    asm("mov.b32 %0, {%1, %1};" : "=r"(s2) : "h"(sc));
-    const uint32_t v04 = mul_bf16x2(code_pair<0>(v), s2), v15 = mul_bf16x2(code_pair<1>(v), s2);
-    const uint32_t v26 = mul_bf16x2(code_pair<2>(v), s2), v37 = mul_bf16x2(code_pair<3>(v), s2);
-    uint4 o;
-    o.x = __byte_perm(v04, v15, 0x5410);
-    o.y = __byte_perm(v26, v37, 0x5410);
-    o.z = __byte_perm(v04, v15, 0x7632);
-    o.w = __byte_perm(v26, v37, 0x7632);
-    reinterpret_cast<uint4*>(out + b * bstride + i * ldo)[e] = o;
+    const int w = e & (words - 1), h = e >> shift;                 // h: key heads, then value heads, P rows apart
+    uint32_t v[R], s2[R];
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      if (tok[k] < 0) continue;
+      const int64_t at = tok[k] + (int64_t)h * p.P;
+      v[k] = __ldg(reinterpret_cast<const uint32_t*>(p.codes + at * (p.D / 2)) + w);
+      s2[k] = __ldg(reinterpret_cast<const uint16_t*>(p.scales) + at * (p.D / kKvGroup) + w / 4) * 0x10001u;
+    }
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      if (tok[k] < 0) continue;
+      const uint32_t v04 = mul_bf16x2(code_pair<0>(v[k]), s2[k]), v15 = mul_bf16x2(code_pair<1>(v[k]), s2[k]);
+      const uint32_t v26 = mul_bf16x2(code_pair<2>(v[k]), s2[k]), v37 = mul_bf16x2(code_pair<3>(v[k]), s2[k]);
+      uint4 o;
+      o.x = __byte_perm(v04, v15, 0x5410);
+      o.y = __byte_perm(v26, v37, 0x5410);
+      o.z = __byte_perm(v04, v15, 0x7632);
+      o.w = __byte_perm(v26, v37, 0x7632);
+      reinterpret_cast<uint4*>(out + to[k])[e] = o;
+    }
   }
 }
 
@@ -869,7 +941,7 @@ template <typename T>
 cudaError_t launch_append_t(const Kv4AppendParams& p, unsigned rows, cudaStream_t stream) {
   const int hpw = 256 / p.kv.D;
   const int slots = (p.Hq + hpw - 1) / hpw + 2 * ((p.kv.Hkv + hpw - 1) / hpw);
-  const int threads = 32 * std::min(slots, 8);
+  const int threads = 32 * std::min(slots, rows >= 8 * 148 ? 4 : 8);   // with many tokens, fewer warps share a token's set-up
   switch (p.kv.D) {
     case 64: kv4_append_kernel<T, 64><<<rows, threads, 0, stream>>>(p); break;
     case 128: kv4_append_kernel<T, 128><<<rows, threads, 0, stream>>>(p); break;
@@ -892,7 +964,10 @@ cudaError_t launch_kv4_read(const Kv4Params& p, __nv_bfloat16* out, int64_t ldo,
   const int64_t rows = (int64_t)p.B * p.L;
   if (rows > 0x7FFFFFFFLL) return cudaErrorInvalidValue;
   const int threads = std::min(256, (2 * p.Hkv * (p.D / 8) + 31) / 32 * 32);
-  kv4_read_kernel<<<(unsigned)rows, threads, 0, stream>>>(p, out, ldo, bstride);
+  if (rows >= 8 * 148)
+    kv4_read_kernel<2><<<(unsigned)((rows + 1) / 2), threads, 0, stream>>>(p, out, ldo, bstride);
+  else
+    kv4_read_kernel<1><<<(unsigned)rows, threads, 0, stream>>>(p, out, ldo, bstride);
   return cudaGetLastError();
 }
 

@@ -612,3 +612,33 @@ def test_kv4_step_captured_and_replayed():
             g.replay()
             assert torch.equal(out, eager[i])
     check_device()
+
+
+def test_kv4_append_and_read_of_many_tokens_exactly():
+    """Enough tokens that fp32 leaves some keys undecided (outlying channels, cancelling rotations, exact borders):
+    every cached value equals the fp64 definition."""
+    from nanosaur2_web_b200 import ops
+    rng = np.random.default_rng(12)
+    for D, Hkv, dtype in ((128, 2, BF), (64, 3, torch.float32), (256, 1, BF)):
+        B, L, P = 3, 500, 32
+        x = rng.standard_normal((B, L, (2 + 2) * Hkv * D)) * np.exp(1.5 * rng.standard_normal((4 * Hkv * D)))
+        x[:, ::7, 2 * Hkv * D:3 * Hkv * D] = np.round(x[:, ::7, 2 * Hkv * D:3 * Hkv * D])     # many equal and zero keys
+        x[0, 5:9, 2 * Hkv * D:3 * Hkv * D] *= 1e-25
+        x[1, 5:9, 2 * Hkv * D:3 * Hkv * D] *= 1e15
+        qkv = t(x, dtype)
+        w = 1 + 0.3 * rng.standard_normal(D)
+        w[::9] *= 300
+        w[1::9] *= 1e-4
+        kw = t(w)
+        cs = ops.ropeTable(L, D, 1e4, DEV)
+        mp = -(-L // P)
+        cache, table = ops.kv4_cache(B * mp, Hkv, D, P, DEV), t(rng.permutation(B * mp).reshape(B, mp), torch.int32)
+        start = torch.zeros(B, dtype=torch.int32, device=DEV)
+        ops.kv4_append(qkv, cache, table, start, Hq=2 * Hkv, q_norm=kw, k_norm=kw, cs=cs)
+        kv = ops.kv4_read(cache, table, start, L)
+        check_device()
+        cos, sin = n64(cs.buf[:cs.sinOff]).reshape(L, 1, D // 2), n64(cs.buf[cs.sinOff:]).reshape(L, 1, D // 2)
+        xk, xv = n64(qkv[:, :, 2 * Hkv * D:3 * Hkv * D]).reshape(B, L, Hkv, D), n64(qkv[:, :, 3 * Hkv * D:])
+        k = O4.norm_rope(xk, n64(kw), cos, sin, np.float64(np.float32(1e-6)))
+        want = np.concatenate([O4.values(*O4.quantise(k.reshape(B, L, -1), 32)), O4.values(*O4.quantise(xv, 32))], -1)
+        np.testing.assert_array_equal(n64(kv), want)
