@@ -23,6 +23,9 @@
 * ``gemma_mlp_sublayer(...)`` / ``gemma_layer(...)``: the MLP half (app/models/gemma3.js:78-89: pre-MLP
   RMSNorm, gate_up linear, GELU-tanh GLU, down linear, post-MLP RMSNorm accumulated) and the whole
   layer, attention half then MLP half.
+* ``gemma_layer_decode(...)``: one Gemma layer for a few new tokens per sequence over the 4-bit cache of the earlier
+  ones (nsa_kv4_append / nsa_kv4_attention), its linears in 4 bits (nsa_linear4) or bf16; the reference runs
+  whole prompts only (app/models/gemma3.js:49-96).
 * ``vae_attention(...)``: the VAE decoder's single-head attention over all latent pixels, head dim C
   = 512 (app/models/vae.js:77-88; tools/reference.py:352-357): ``ops.attention`` with H = 1, D = C on
   the packed qkv rows of the group-normed input.
@@ -41,7 +44,8 @@ import torch
 
 from . import _lib
 from ._lib import FusedDesc, NsaError, ProjDesc, SeqShard, check, lib
-from .ops import RopeTable, dtype_code, glu, linear, rmsnorm, stream_handle
+from .ops import (Kv4Cache, RopeTable, Weight4, dtype_code, glu, kv4_append, kv4_attention, linear, linear4, rmsnorm,
+                  stream_handle)
 
 DIT_HEADS, DIT_HEAD_DIM = 16, 96
 GEMMA_HEADS, GEMMA_KV_HEADS, GEMMA_HEAD_DIM = 4, 1, 256
@@ -416,6 +420,73 @@ def gemma_layer(x: torch.Tensor, *, attn: dict, mlp: dict, cs: RopeTable, window
                              next_norm=mlp["pre_norm"], next_out=mb["h"])
     return gemma_mlp_sublayer(x, **mlp, eps=eps, buffers=mb, h_ready=True, next_norm=next_norm,
                               next_out=ab["h"] if next_norm is not None else None)
+
+
+def gemma_decode_buffers(B: int, L: int, hidden: int, inter: int, device) -> dict:
+    """Intermediates of ``gemma_layer_decode`` for B sequences of up to L new tokens: the normalised rows and the MLP's
+    (bf16), the linears' fp32 results, q', the attention's rows.  Zeroed, so that rows past a sequence's count stay
+    finite."""
+    M, QKV, A = B * L, (GEMMA_HEADS + 2 * GEMMA_KV_HEADS) * GEMMA_HEAD_DIM, GEMMA_HEADS * GEMMA_HEAD_DIM
+
+    def zeros(shape, dtype):
+        return torch.zeros(shape, dtype=dtype, device=device)
+    return {"h": zeros((M, hidden), torch.bfloat16), "qkv": zeros((B, L, QKV), torch.float32),
+            "q": zeros((B, L, A), torch.bfloat16), "a": zeros((B, L, A), torch.bfloat16),
+            "o": zeros((M, hidden), torch.float32), "h2": zeros((M, hidden), torch.bfloat16),
+            "gu": zeros((M, 2 * inter), torch.float32), "g": zeros((M, inter), torch.bfloat16)}
+
+
+def _any_linear(x: torch.Tensor, W, out: torch.Tensor) -> None:
+    if isinstance(W, Weight4):
+        linear4(x, W, out=out)
+    else:
+        linear(x, W, out=out)
+
+
+def gemma_layer_decode(x: torch.Tensor, *, attn: dict, mlp: dict, cs: RopeTable, cache: Kv4Cache, table: torch.Tensor,
+                       start: torch.Tensor, count: Optional[torch.Tensor] = None, window: int = 0, sinks: int = 0,
+                       eps: float = 1e-6, buffers: Optional[dict] = None, h_ready: bool = False,
+                       next_norm: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """One Gemma3 layer (app/models/gemma3.js:62-89) in place on the new tokens' residual rows x (fp32 [B, L, hidden]):
+        qkv = rmsnorm(x, in_norm) W_qkv^T                          nsa_rmsnorm + nsa_linear4
+        q'  = norm + RoPE of q; k', v into the layer's cache        nsa_kv4_append
+        a   = attention of q' over the cache                        nsa_kv4_attention
+        x  += rmsnorm(a W_o^T, post_norm), and h2 = rmsnorm(x, pre_norm)
+        x  += rmsnorm(GLU(h2 W_gate_up^T) W_down^T, post_norm)
+    Row i of sequence b is the token at position start[b] + i (start, count: device int32 [B] as in ``kv4_append``; rows
+    past count[b] are padding, whose x is not meaningful afterwards).  attn = {in_norm, w_qkv, q_norm, k_norm, w_o,
+    post_norm} and mlp = {pre_norm, w_gate_up ([gate; up] rows), w_down, post_norm} as in ``gemma_layer``, each
+    weight a ``Weight4`` (``quantize4``) or a bf16 tensor.  ``cache`` is this layer's; prompts enter it through the same
+    call, in chunks of any L.  ``window`` and ``sinks`` as in ``kv4_attention`` (Gemma's local layers: window 512).
+    ``buffers`` = gemma_decode_buffers(...), to reuse; with ``next_norm`` (the next layer's in_norm) buffers["h"] holds
+    the next layer's normalised rows and the next call passes ``h_ready=True``.  Returns x."""
+    if x.dim() != 3 or x.dtype != torch.float32 or not x.is_contiguous():
+        raise NsaError(_lib.NSA_ERR_INVALID_ARGUMENT, "x must be a contiguous float32 [B, L, hidden] tensor")
+    if cache.D != GEMMA_HEAD_DIM or cache.Hkv != GEMMA_KV_HEADS:
+        raise NsaError(_lib.NSA_ERR_INVALID_ARGUMENT, f"the cache must hold {GEMMA_KV_HEADS} head of {GEMMA_HEAD_DIM}")
+    if h_ready and buffers is None:
+        raise NsaError(_lib.NSA_ERR_INVALID_ARGUMENT, "h_ready needs the buffers that hold h")
+    B, L, hidden = x.shape
+    w_gu = mlp["w_gate_up"]
+    rows = w_gu.N if isinstance(w_gu, Weight4) else w_gu.shape[0]
+    if rows % 2:
+        raise NsaError(_lib.NSA_ERR_INVALID_ARGUMENT, "w_gate_up must have [gate; up] rows")
+    buf = buffers if buffers is not None else gemma_decode_buffers(B, L, hidden, rows // 2, x.device)
+    xs = x.view(B * L, hidden)
+    if not h_ready:
+        rmsnorm(xs, attn["in_norm"], hidden, eps, buf["h"])
+    _any_linear(buf["h"], attn["w_qkv"], buf["qkv"].view(B * L, -1))
+    kv4_append(buf["qkv"], cache, table, start, count=count, Hq=GEMMA_HEADS, q_norm=attn["q_norm"], k_norm=attn["k_norm"],
+               cs=cs, eps=eps, out=buf["q"])
+    kv4_attention(buf["q"], cache, table, start, count=count, window=window, sinks=sinks, out=buf["a"])
+    _any_linear(buf["a"].view(B * L, -1), attn["w_o"], buf["o"])
+    rmsnorm(buf["o"], attn["post_norm"], hidden, eps, xs, accumulate=True, next_weight=mlp["pre_norm"], next_out=buf["h2"])
+    _any_linear(buf["h2"], w_gu, buf["gu"])
+    glu(buf["gu"], "gelu_tanh", out=buf["g"])
+    _any_linear(buf["g"], mlp["w_down"], buf["o"])
+    rmsnorm(buf["o"], mlp["post_norm"], hidden, eps, xs, accumulate=True, next_weight=next_norm,
+            next_out=None if next_norm is None else buf["h"])
+    return x
 
 
 def text_refine_attention(qkv: torch.Tensor, *, q_norm: torch.Tensor, k_norm: torch.Tensor,
