@@ -1679,6 +1679,8 @@ static nsa_status kv4_params(const nsa_kv4_cache* c, const nsa_kv4_batch* s, nsa
     return fail(NSA_ERR_UNSUPPORTED, "the 4-bit cache holds head dims 64, 128 and 256");
   if (c->P < 16 || c->P > 1024 || c->P % 16) return fail(NSA_ERR_INVALID_ARGUMENT, "P must be a multiple of 16 in [16, 1024]");
   if (c->n_pages < 0 || c->Hkv < 1) return fail(NSA_ERR_INVALID_ARGUMENT, "need n_pages >= 0 and Hkv >= 1");
+  if ((double)c->n_pages * 2 * c->Hkv * (c->P / 16) >= 4294967296.0)   // blocks of 16 tokens are counted in 32 bits
+    return fail(NSA_ERR_UNSUPPORTED, "the pool holds 2^32 or more blocks of 16 tokens of a head");
   if (s->B < 0 || s->L < 0 || s->max_pages < 0) return fail(NSA_ERR_INVALID_ARGUMENT, "need B, L and max_pages >= 0");
   if ((int64_t)s->max_pages * c->P > 0x7FFFFFFFLL)
     return fail(NSA_ERR_INVALID_ARGUMENT, "the page table spans more than 2^31 - 1 tokens");

@@ -85,7 +85,7 @@ def batch_of(**kw):
 
 
 COMMON = [(dict(D=96), UNSUP), (dict(D=512), UNSUP), (dict(P=8), BAD), (dict(P=24), BAD), (dict(P=2048), BAD),
-          (dict(n_pages=-1), BAD), (dict(Hkv=0), BAD), (dict(B=-1), BAD), (dict(L=-1), BAD), (dict(max_pages=-1), BAD),
+          (dict(n_pages=-1), BAD), (dict(n_pages=1 << 30), UNSUP), (dict(Hkv=0), BAD), (dict(B=-1), BAD), (dict(L=-1), BAD), (dict(max_pages=-1), BAD),
           (dict(max_pages=1 << 27), BAD), (dict(table_ld=3), BAD), (dict(table=None), BAD), (dict(start=None), BAD),
           (dict(start=FAKE + 2), BAD), (dict(count=FAKE + 1), BAD), (dict(codes=FAKE + 4), BAD), (dict(scales=None), BAD)]
 
@@ -139,6 +139,16 @@ def test_read_and_attention_refusals():
         assert call(**kw) == BAD, kw
     assert b"overlap" in L.nsa_last_error()
     assert call(q=None, out=None, batch=dict(B=0)) == OK
+    assert call(batch=dict(B=1 << 20, L=64, max_pages=1 << 26), q_bstride=512 * 64, o_bstride=512 * 64) == UNSUP   # too many blocks
+    # a workspace where keys are split over CTAs: none for few short sequences, an error names the size otherwise
+    d = _lib.Kv4AttentionDesc(**base)
+    assert L.nsa_kv4_attention_workspace_size(ctypes.byref(d), ctypes.byref(c), ctypes.byref(b)) == 0
+    big = batch_of(max_pages=4096)
+    need = L.nsa_kv4_attention_workspace_size(ctypes.byref(d), ctypes.byref(c), ctypes.byref(big))
+    assert need > 0
+    for ws, n in ((None, 0), (FAKE, need - 1), (FAKE + 8, need)):
+        assert call(ws=ws, nbytes=n, batch=dict(max_pages=4096)) == _lib.NSA_ERR_WORKSPACE
+    assert str(need).encode() in L.nsa_last_error()
     d = _lib.Kv4AttentionDesc(**{**base, "Hq": 5})
     assert L.nsa_kv4_attention_workspace_size(ctypes.byref(d), ctypes.byref(c), ctypes.byref(b)) == 0
 

@@ -642,3 +642,54 @@ def test_kv4_append_and_read_of_many_tokens_exactly():
         k = O4.norm_rope(xk, n64(kw), cos, sin, np.float64(np.float32(1e-6)))
         want = np.concatenate([O4.values(*O4.quantise(k.reshape(B, L, -1), 32)), O4.values(*O4.quantise(xv, 32))], -1)
         np.testing.assert_array_equal(n64(kv), want)
+
+
+def test_kv4_attention_of_long_sequences_captured_and_on_two_streams():
+    """Keys split over CTAs and joined by the second kernel: replayed at several positions, and two calls at once."""
+    from nanosaur2_web_b200 import ops
+    rng = np.random.default_rng(20)
+    cd = Cached(rng, 1, 5200, 1, 64, 32)
+    q = t(rng.standard_normal((1, 2, 4 * 64)), BF)
+    start, out = t([5000], torch.int32), torch.zeros((1, 2, 4 * 64), dtype=BF, device=DEV)
+    side = torch.cuda.Stream(DEV)
+    side.wait_stream(torch.cuda.current_stream(DEV))
+    with torch.cuda.stream(side):
+        ops.kv4_attention(q, cd.cache, cd.table, start, out=out)
+    torch.cuda.current_stream(DEV).wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        ops.kv4_attention(q, cd.cache, cd.table, start, out=out)
+    for at in (5198, 0, 17, 4090):
+        start.fill_(at)
+        g.replay()
+        want, tol = attend_oracle(cd, n64(q), [at], [2], 0, 0, 1 / 8)
+        assert (np.abs(n64(out) - want) <= tol).all(), at
+    streams, outs = [torch.cuda.Stream(DEV) for _ in range(2)], []
+    starts = [t([a], torch.int32) for a in (5198, 3000)]
+    ref = [ops.kv4_attention(q, cd.cache, cd.table, s) for s in starts]
+    torch.cuda.synchronize()
+    for i in range(20):
+        with torch.cuda.stream(streams[i % 2]):
+            outs.append(ops.kv4_attention(q, cd.cache, cd.table, starts[i % 2]))
+    torch.cuda.synchronize()
+    check_device()
+    assert all(torch.equal(o, ref[i % 2]) for i, o in enumerate(outs))
+
+
+def test_kv4_empty_batches_and_pools():
+    from nanosaur2_web_b200 import ops
+    c = ops.kv4_cache(2, 1, 64, 16, DEV)
+    e = torch.zeros((0, 2), dtype=torch.int32, device=DEV)
+    s0 = torch.zeros(0, dtype=torch.int32, device=DEV)
+    assert ops.kv4_attention(torch.zeros((0, 1, 64), dtype=BF, device=DEV), c, e, s0).shape == (0, 1, 64)
+    table, start = t([[0, 1]], torch.int32), t([3], torch.int32)
+    assert ops.kv4_attention(torch.zeros((1, 0, 64), dtype=BF, device=DEV), c, table, start).shape == (1, 0, 64)
+    w = torch.ones(64, device=DEV)
+    assert ops.kv4_append(torch.zeros((0, 1, 192), device=DEV), c, e, s0, Hq=1, q_norm=w, k_norm=w, cs=None).shape == (0, 1, 64)
+    check_device()
+    # a pool or a table without a page: every key is missing, zeros and a report
+    q = torch.ones((1, 1, 64), dtype=BF, device=DEV)
+    for cache, tab, match in ((ops.kv4_cache(0, 1, 64, 16, DEV), table, "page table entry"), (c, table[:, :0], "position")):
+        assert (ops.kv4_attention(q, cache, tab, start) == 0).all()
+        with pytest.raises(ops.NsaError, match=match):
+            check_device()
