@@ -112,8 +112,9 @@ __global__ void __launch_bounds__(256) expand4_kernel(const Quant4Params p, __nv
 // A fragment's own order and converts them in registers.  Lane (r, c) holds rows r and r + 8, words i = 0..3 of
 // piece c: word i of all four c is group i of 32 values, so one product of k = 32 covers exactly one group,
 // starts from zero and enters the row's sum with the group's scale in fp32.  Nibble pairs are neighbours
-// (q4_nibble), so X's own 16 bytes of values 32 i + 8 c .. + 7 are the B fragments.  A nibble n set into a bf16
-// mantissa is 128 + n; minus 136 it is the code, exactly.
+// (q4_nibble), so X's own 16 bytes of values 32 i + 8 c .. + 7 are the B fragments.  A nibble n set into the mantissa
+// of 1 / 8 is (1 + n / 128) / 8; minus 17 / 128 it is the code / 1024, exactly, and 128 of them times the largest bf16 do
+// not overflow before the scale is applied.
 //
 // One CTA of 16 warps per SM takes TN = 16 / WK tiles at a time, the WK warps of a tile its chunks in turn.  Each warp
 // copies its chunks into a ring of its own, several ahead of their use and across tile ends; the rows of X that the
@@ -122,13 +123,12 @@ __global__ void __launch_bounds__(256) expand4_kernel(const Quant4Params p, __nv
 // tiles with it, and the parts of the sums are joined through the shared memories at the end.
 
 constexpr int kWarps = 16;
+constexpr float kCodeUnit = 1024.f;
 constexpr int kSmemMax = 227 * 1024;
 constexpr int kMaxCluster = 8;
 
 constexpr int kStages = 3;   // of kStep chunks each
 constexpr int kStep = 2;
-// CTAs per SM where their shared memory allows it: with few rows of X a warp's registers do
-__host__ __device__ constexpr int most_ctas(int NT) { return NT <= 2 ? 2 : 1; }
 __host__ __device__ constexpr int stage_bytes(int G) { return kStep * kRowTile * (kChunk / 2 + kChunk / G * 2); }
 
 // Scales of a row's chunk in shared memory: 128 / G bf16 in one load.
@@ -164,9 +164,17 @@ __device__ __forceinline__ void write_out(const Linear4Params& p, int m, int n, 
   else static_cast<float*>(p.c)[o] = v;
 }
 
+// Codes / kCodeUnit of nibbles P and P + 4 of a word as a bf16 pair.
+template <int P>
+__device__ __forceinline__ uint32_t small_pair(uint32_t w) {
+  uint32_t d;
+  asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(mask_or(w >> (4 * P), 0x000F000Fu, 0x3E003E00u)), "r"(0xBE08BE08u));
+  return d;
+}
+
 // NT: tiles of eight rows of X.
 template <int G, int NT>
-__global__ void __launch_bounds__(kWarps * 32, most_ctas(NT)) linear4_kernel(const Linear4Params p) {
+__global__ void __launch_bounds__(kWarps * 32, 1) linear4_kernel(const Linear4Params p) {
   constexpr int STAGES = kStages, STAGE = stage_bytes(G), CODES = kRowTile * kChunk / 2, SCALES = STAGE / kStep - CODES;   // bytes
   constexpr int kOut = 16 * 8 * NT;                                 // values of a tile
   extern __shared__ __align__(128) uint8_t smem[];
@@ -262,8 +270,8 @@ __global__ void __launch_bounds__(kWarps * 32, most_ctas(NT)) linear4_kernel(con
         float acc[NT][4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const uint32_t a0 = code_pair<0>(wa[i]), a1 = code_pair<0>(wb[i]), a2 = code_pair<1>(wa[i]), a3 = code_pair<1>(wb[i]);
-          const uint32_t a4 = code_pair<2>(wa[i]), a5 = code_pair<2>(wb[i]), a6 = code_pair<3>(wa[i]), a7 = code_pair<3>(wb[i]);
+          const uint32_t a0 = small_pair<0>(wa[i]), a1 = small_pair<0>(wb[i]), a2 = small_pair<1>(wa[i]), a3 = small_pair<1>(wb[i]);
+          const uint32_t a4 = small_pair<2>(wa[i]), a5 = small_pair<2>(wb[i]), a6 = small_pair<3>(wa[i]), a7 = small_pair<3>(wb[i]);
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
             const uint4 x = xt[t][xo + i * 4 * rows];
@@ -291,10 +299,10 @@ __global__ void __launch_bounds__(kWarps * 32, most_ctas(NT)) linear4_kernel(con
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       float* d = red + warp * kOut + (8 * t + 2 * c) * 16 + r;
-      d[0] = y[t][0];
-      d[16] = y[t][1];
-      d[8] = y[t][2];
-      d[24] = y[t][3];
+      d[0] = y[t][0] * kCodeUnit;
+      d[16] = y[t][1] * kCodeUnit;
+      d[8] = y[t][2] * kCodeUnit;
+      d[24] = y[t][3] * kCodeUnit;
 #pragma unroll
       for (int j = 0; j < 4; ++j) y[t][j] = 0.f;
     }
@@ -398,21 +406,19 @@ Linear4Plan linear4_plan(const Linear4Params& p, int rows, int sms) {
   Linear4Plan best{0, 0, 0, 0, 1e30};
   for (int cs = 1; cs <= kMaxCluster; cs *= 2) {
     if (cs > 1 && cs > p.Kc) break;
-    for (int per_sm = most_ctas(nt); per_sm >= 1; --per_sm) {
-      // clusters of 8 or 4 CTAs leave a few SMs of a processing cluster over
-      const int clusters = per_sm * (cs == 1 ? sms : cs == 2 ? sms / 2 : cs == 4 ? sms / 4 - 1 : sms / 8 - 2);
-      const int64_t each = (p.Kc + cs - 1) / cs;
-      for (int wk = kWarps; wk >= 1; wk /= 2) {
-        const int64_t tn = kWarps / wk, rounds = (p.Nt + tn * clusters - 1) / (tn * clusters);
-        const size_t bytes = (size_t)kWarps * kStages * stage_bytes(p.G) + (size_t)kWarps * 16 * 8 * nt * 4 +
-                             (size_t)each * 256 * rows + (cs > 1 ? (size_t)rounds * tn * rows * 64 : 0);
-        if (per_sm * (bytes + 1024) > kSmemMax + 1024) continue;
-        // a step: the instructions of a scheduler's warps; a round: its join; X at about 48 bytes a cycle; a
-        // cluster's join
-        const double cost = (double)rounds * ((each + kStep * wk - 1) / (kStep * wk)) * kStep * 4 * per_sm * (150 + 50 * nt) * (per_sm == 1 ? 1.6 : 1.2) +
-                            rounds * (per_sm == 1 ? 800.0 : 400.0) + each * 256.0 * rows / 48 + (cs > 1 ? 1500.0 : 0.0);
-        if (cost < best.cost) best = {wk, cs, (int)std::min<int64_t>(clusters, (p.Nt + tn - 1) / tn), bytes, cost};
-      }
+    // clusters of 8 or 4 CTAs leave a few SMs of a processing cluster over
+    const int clusters = cs == 1 ? sms : cs == 2 ? sms / 2 : cs == 4 ? sms / 4 - 1 : sms / 8 - 2;
+    const int64_t each = (p.Kc + cs - 1) / cs;
+    for (int wk = kWarps; wk >= 1; wk /= 2) {
+      const int64_t tn = kWarps / wk, rounds = (p.Nt + tn * clusters - 1) / (tn * clusters);
+      const size_t bytes = (size_t)kWarps * kStages * stage_bytes(p.G) + (size_t)kWarps * 16 * 8 * nt * 4 +
+                           (size_t)each * 256 * rows + (cs > 1 ? (size_t)rounds * tn * rows * 64 : 0);
+      if (bytes > kSmemMax) continue;
+      // a step: the instructions of a scheduler's warps; a round: its join; X at about 48 bytes a cycle; a
+      // cluster's join
+      const double cost = (double)rounds * ((each + kStep * wk - 1) / (kStep * wk)) * kStep * 4 * (150 + 50 * nt) * 1.6 +
+                          rounds * 800.0 + each * 256.0 * rows / 48 + (cs > 1 ? 1500.0 : 0.0);
+      if (cost < best.cost) best = {wk, cs, (int)std::min<int64_t>(clusters, (p.Nt + tn - 1) / tn), bytes, cost};
     }
   }
   return best;

@@ -167,6 +167,38 @@ def test_linear4_takes_any_bf16_scales_and_propagates_nonfinite_rows():
     assert torch.isnan(yi[1]).all() and torch.equal(yi[0], y[0]) and torch.equal(yi[2], y[2])
 
 
+@pytest.mark.parametrize("M", [1, 2, 3, 4, 5])
+def test_linear4_rows_of_wide_range_and_infinities(M):
+    """Rows whose values span the whole of bf16 zero and subnormal
+    groups, the largest finite values; infinities, which reach their row as the formula has it."""
+    from nanosaur2_web_b200.ops import linear4
+    rng = np.random.default_rng(M)
+    W, Wv, _ = linear_case(rng, 1, 100, 640, 32)
+    x = rng.standard_normal((M, 640)) * np.exp2(rng.integers(-30, 30, (M, 640)))
+    x[0, :32] = 0
+    x[0, 32:64] *= 2.0 ** -100
+    x[M - 1, 64:96] = rng.standard_normal(32) * 2.0 ** -131          # subnormal in bf16
+    x[0, 96:128] *= 2.0 ** 60
+    x = t(x, BF)
+    y = n64(linear4(x, W))
+    want = n64(x) @ Wv.T
+    assert (np.abs(y - want) <= linear_tol(n64(x), Wv, 32) + 1e-37).all()
+    big = t(rng.choice([-1.0, 1.0], (M, 640)) * 3.0e38 * (rng.random((M, 640)) < 0.002), BF)
+    with np.errstate(over="ignore", invalid="ignore"):
+        want = n64(big) @ Wv.T
+    y = n64(linear4(big, W))
+    fine = np.abs(n64(big)) @ np.abs(Wv).T < 3e38      # else a sum of fp32 products overflows in one order or another
+    assert (np.abs(y - want)[fine] <= (linear_tol(n64(big), Wv, 32) + 1e-30)[fine]).all()
+    xi = x.clone()
+    xi[0, 201], xi[M - 1, 500] = float("inf"), float("-inf")
+    with np.errstate(invalid="ignore"):
+        want = (n64(xi)[:, None, :] * Wv[None]).sum(-1)
+    y = n64(linear4(xi, W))
+    check_device()
+    assert np.array_equal(np.isnan(y), np.isnan(want)) and np.array_equal(np.isinf(y), np.isinf(want))
+    assert (np.sign(y[np.isinf(y)]) == np.sign(want[np.isinf(want)])).all()
+
+
 def test_linear4_empty_and_other_stream():
     from nanosaur2_web_b200.ops import linear4
     rng = np.random.default_rng(9)
