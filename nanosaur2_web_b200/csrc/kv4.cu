@@ -314,11 +314,22 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4Params p, __nv_b
 // scale has five significant bits (q4.cuh).
 //
 // P^T is P's accumulator transposed: packed to bf16 and turned by movmatrix.  P is split into two bf16 terms
-// (16 bits together): one bf16 would add an error as large as the output's own rounding.
+// (16 bits together): one bf16 would add an error as large as the output's own rounding.  Where a unit has at most four
+// rows, half of the columns would be empty: they take the same rows again, the scores there are the same, and the low
+// terms are what they multiply the values with, so that one product does for both.
+//
+// What bounds it is the issue of instructions: an mma.m16n8k16 holds a scheduler for about 5 cycles (and its tensor unit
+// for 8), a pair of converted values costs 3 instructions, two of them at half rate.  With the copies taken out, 8192
+// blocks of 8 heads for 16 rows (D 128) take the time that they take with them; without the products and conversions,
+// 40 us of 64.  Two blocks at a time give the scheduler independent chains (D 256: 33.2 -> 29.7 us at 8 x 32768 tokens)
+// and share the walk, the tests of masks and maxima (466 instead of 594 instructions a block).
 // The running maximum moves only when a score exceeds it by 2^8 in the exponent's base, which keeps sums in
 // range without a reduction over lanes per block.
 
 constexpr int kAttnWarps = 4;
+constexpr int kAtOnce = 2;          // blocks that a warp takes at a time
+constexpr int kSetup = 20;          // what another unit costs a CTA, in blocks (0, 8, 20, 32: 69.6, 67.6, 64.3, 64.9 us
+                                    // at 4 tokens over 131071; 74.7, 73.0, 72.5, 72.6 us at 40 sequences up to 8192)
 constexpr float kMaxSlack = 8.f;   // exp2 of a score may reach 2^8 before the maximum is moved
 
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
@@ -423,7 +434,7 @@ struct Stage {
 
 template <int D, int NT>
 struct AttnSmem {
-  static constexpr int stages = D == 256 ? 3 : 4;
+  static constexpr int stages = D == 256 ? 4 : 6;
   static constexpr size_t q = (size_t)D / 16 * NT * 32 * 8;                         // Q^T fragments
   static constexpr size_t ring = (size_t)kAttnWarps * stages * Stage<D>::bytes;
   static constexpr size_t o = (size_t)kAttnWarps * 8 * NT * (D + 4) * 4;            // warps' outputs, rows padded
@@ -431,15 +442,16 @@ struct AttnSmem {
   static constexpr size_t bytes = (q + ring > o ? q + ring : o) + ml;
 };
 
-constexpr int ctas_per_sm(int D, int NT) { return NT == 1 ? 3 : 2; }
+constexpr int ctas_per_sm(int D, int NT) { return NT == 1 && D < 256 ? 3 : 2; }
 
-// NT: tiles of eight query rows.  CL: 1, or the CTAs of a cluster that takes one unit.
-template <int D, int NT, int CL>
+// NT: tiles of eight query rows; SPLIT: one tile of at most four, whose columns 4 .. 7 are its rows again.  CL: 1, or the
+// CTAs of a cluster that takes one unit.
+template <int D, int NT, bool SPLIT, int CL>
 __global__ void __launch_bounds__(kAttnWarps * 32, ctas_per_sm(D, NT)) kv4_attention_kernel(const Kv4AttnParams p) {
   constexpr int KW = D / 32;   // words of a token's keys per lane
   constexpr int VW = D / 64;   // words of a token's values per lane
   constexpr int KG = D == 256 ? 2 : 1;
-  constexpr int ROWS = 8 * NT, STAGES = AttnSmem<D, NT>::stages;
+  constexpr int ROWS = 8 * NT, STAGES = AttnSmem<D, NT>::stages, U = kAtOnce;
   extern __shared__ __align__(16) uint8_t smem[];
   const Kv4Params& kv = p.kv;
   const int lane = threadIdx.x % 32, r = lane / 4, c = lane % 4;
@@ -451,7 +463,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32, ctas_per_sm(D, NT)) kv4_atten
   if constexpr (CL == 1) {
     const int tiles = kv.B * p.row_tiles;
     const auto blocks_at = [&](int e) {
-      return e < tiles ? kv.Hkv * unit_blocks(tile_of(p, e / p.row_tiles, e % p.row_tiles, ROWS, group)) : 0;
+      const int n = e < tiles ? unit_blocks(tile_of(p, e / p.row_tiles, e % p.row_tiles, ROWS, group)) : 0;
+      return n ? kv.Hkv * (n + kSetup) : 0;
     };
     int own = blocks_at(lane), total = __reduce_add_sync(0xffffffffu, own);
     for (int e0 = 32; e0 < tiles; e0 += 32) total += __reduce_add_sync(0xffffffffu, blocks_at(e0 + lane));
@@ -515,16 +528,19 @@ __global__ void __launch_bounds__(kAttnWarps * 32, ctas_per_sm(D, NT)) kv4_atten
   const Tile tl = tile_of(p, b, rt, ROWS, group);
   const Blocks bl = tl.bl;
   const int n = unit_blocks(tl);
-  int hk, first, last;   // this CTA's blocks of the unit: [first, last)
+  int hk, first, last, begins = 0;   // this CTA's blocks of the unit: [first, last); where the unit begins
   if constexpr (CL == 1) {
-    if (g - before >= kv.Hkv * n) {   // on to the next tile with rows
-      before += kv.Hkv * n;
+    const int all = n ? n + kSetup : 0;
+    if (g - before >= kv.Hkv * all) {   // on to the next tile with rows
+      before += kv.Hkv * all;
       ++entry;
       continue;
     }
-    hk = (g - before) / n;
-    first = g - before - hk * n;
-    last = min(n, first + (g1 - g));
+    hk = (g - before) / all;
+    begins = before + hk * all;
+    first = max(g - begins - kSetup, 0);
+    last = min(n, g1 - begins - kSetup);
+    if (last <= 0) return;   // no more than the unit's set-up: the next CTA has its first block
   } else {
     if (n == 0) return;   // the whole cluster
     hk = blockIdx.x / CL % kv.Hkv;
@@ -542,7 +558,21 @@ __global__ void __launch_bounds__(kAttnWarps * 32, ctas_per_sm(D, NT)) kv4_atten
   const int ta = min(first + warp * each, last), tb = bl.n > 0 ? min(ta + each, last) : ta;
   const int* table = kv.table + (int64_t)b * kv.table_ld;
 
-  // Walks the warp's blocks, STAGES - 1 ahead of their use: `at` and `left` are the next block's index and the blocks
+  // The rows of Q, 16 bytes (a word's dims) a thread at a time; under way while the first blocks are.
+  constexpr int Q = (KW * NT + kAttnWarps - 1) / kAttnWarps;
+  uint4 qv[Q];
+#pragma unroll
+  for (int x = 0; x < Q; ++x) {
+    const int e = threadIdx.x + x * kAttnWarps * 32, ln = e % 32, cc = ln % 4, w = e / 32 / NT;
+    const int rr = SPLIT ? ln / 4 % 4 : 8 * (e / 32 % NT) + ln / 4;
+    const int word = D == 256 ? 4 * (cc + 4 * (w / 4)) + w % 4 : KW * cc + w;
+    const int i = token_of(kv, row0 + rr, group);
+    qv[x] = make_uint4(0u, 0u, 0u, 0u);
+    if (e < KW * NT * 32 && rr < rows && i <= i_last)
+      qv[x] = __ldg(reinterpret_cast<const uint4*>(p.q + b * p.q_bstride + i * p.q_ld + (int64_t)(hk * group + row0 + rr - i * group) * D + word * 8));
+  }
+
+  // Walks the warp's blocks, STAGES - U ahead of their use: `at` and `left` are the next block's index and the blocks
   // until another page (or the jump from the first tokens to the window).  A missing page stands on page 0, masked
   // (`absent`, one bit per stage).  The ids of the two pages ahead are loaded early.
   int w_t, left, id1, id2;
@@ -597,7 +627,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, ctas_per_sm(D, NT)) kv4_atten
     left = 0;
     absent = 0;
 #pragma unroll
-    for (int st = 0; st < STAGES - 1; ++st) fetch(st);
+    for (int st = 0; st < STAGES - U; ++st) fetch(st);
   };
   begin();
 
@@ -606,28 +636,23 @@ __global__ void __launch_bounds__(kAttnWarps * 32, ctas_per_sm(D, NT)) kv4_atten
   for (int t = 0; t < NT; ++t)
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const int k = 8 * t + 2 * c + j, i = token_of(kv, row0 + k, group);
+      const int k = SPLIT ? (2 * c + j) % 4 : 8 * t + 2 * c + j, i = token_of(kv, row0 + k, group);
       pos[t][j] = k < rows && i <= i_last && bl.n > 0 && pmin + (i - tl.i_first) <= pmax ? pmin + (i - tl.i_first) : -1;
     }
   // every row sees every token of the blocks numbered [whole0, whole1)
   const int whole0 = p.window > 0 ? bl.sink_blocks + (max(pmax - p.window + 1, 0) + 15) / 16 - bl.first : 0;
+  const int jump_by = 16 * (bl.first - bl.sink_blocks);
   const int whole1 = tl.outside ? 0 : bl.sink_blocks + (pmin + 1) / 16 - bl.first;
 
   // Q^T fragments: for k-step 2w + s of lane (r, c), words of row r's dims in the order of the lane's key words
   uint2* qs = reinterpret_cast<uint2*>(smem);
-  for (int e = threadIdx.x; e < D / 16 * NT * 32; e += kAttnWarps * 32) {
-    const int ln = e % 32, t = e / 32 % NT, ks = e / 32 / NT, rr = 8 * t + ln / 4, cc = ln % 4, w = ks / 2;
-    const int word = D == 256 ? 4 * (cc + 4 * (w / 4)) + w % 4 : KW * cc + w;
-    uint2 f = make_uint2(0u, 0u);
-    const int i = token_of(kv, row0 + rr, group);
-    if (rr < rows && i <= i_last) {
-      const uint4 v = *reinterpret_cast<const uint4*>(p.q + b * p.q_bstride + i * p.q_ld +
-                                                      (int64_t)(hk * group + row0 + rr - i * group) * D + word * 8);
-      // pairs (e, e + 4): e = 2 s and 2 s + 1
-      const uint32_t lo = ks % 2 ? v.y : v.x, hi = ks % 2 ? v.w : v.z;
-      f = make_uint2(__byte_perm(lo, hi, 0x5410), __byte_perm(lo, hi, 0x7632));
-    }
-    qs[e] = f;
+#pragma unroll
+  for (int x = 0; x < Q; ++x) {
+    const int e = threadIdx.x + x * kAttnWarps * 32, ln = e % 32, t = e / 32 % NT, w = e / 32 / NT;
+    if (e >= KW * NT * 32) break;
+    // pairs (e, e + 4): e = 2 s and 2 s + 1
+    qs[(2 * w * NT + t) * 32 + ln] = make_uint2(__byte_perm(qv[x].x, qv[x].z, 0x5410), __byte_perm(qv[x].x, qv[x].z, 0x7632));
+    qs[((2 * w + 1) * NT + t) * 32 + ln] = make_uint2(__byte_perm(qv[x].y, qv[x].w, 0x5410), __byte_perm(qv[x].y, qv[x].w, 0x7632));
   }
   __syncthreads();
 
@@ -647,80 +672,95 @@ __global__ void __launch_bounds__(kAttnWarps * 32, ctas_per_sm(D, NT)) kv4_atten
 #pragma unroll
       for (int j = 0; j < 2; ++j) m[t][j] = lim[t][j] = -INFINITY, z[t][j] = 0.f, l[t][j] = 0.f;
     }
-    int j_now = 16 * (ta < bl.sink_blocks ? ta : bl.first + ta - bl.sink_blocks) - 16, stage = 0;
-    for (int tt = ta; tt < tb; ++tt) {
-      j_now = tt == bl.sink_blocks ? 16 * bl.first : j_now + 16;
-      copy_wait<STAGES - 2>();
-      __syncwarp();   // the block is there for all lanes, and all lanes are done with the stage that is filled next
-      fetch(stage == 0 ? STAGES - 1 : stage - 1);
+    int stage = 0;
+    for (int tt = ta; tt < tb; tt += U) {
+      copy_wait<STAGES - 2 * U>();
+      __syncwarp();   // the blocks are there for all lanes, and all lanes are done with the stages that are filled next
+#pragma unroll
+      for (int u = 0; u < U; ++u) fetch((stage == 0 ? STAGES - U : stage - U) + u);
       const uint32_t blk = ring_at + stage * Stage<D>::bytes;
-      const bool gone = absent && (absent >> stage & 1);
-      stage = stage == STAGES - 1 ? 0 : stage + 1;
-      uint32_t kw[2][KW], ks[2][KG];
+      // first token of each block; past the warp's last block, and where a page is missing, there is nothing
+      int j_now[U];
+      bool gone[U], part = false;
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        load_words<(KW > 4 ? 4 : KW)>(blk + k_at[0] + x * 4 * D, kw[x]);
-        if constexpr (KW > 4) load_words<4>(blk + k_at[1] + x * 4 * D, kw[x] + 4);
-#pragma unroll
-        for (int y = 0; y < KG; ++y) ks[x][y] = load_scale(blk + ks_at + x * (D / 2) + 8 * y);
+      for (int u = 0; u < U; ++u) {
+        j_now[u] = 16 * (tt + u) + (tt + u < bl.sink_blocks ? 0 : jump_by);
+        gone[u] = (absent && (absent >> (stage + u) & 1)) || tt + u >= tb;
+        part = part || tt + u < whole0 || tt + u >= whole1 || gone[u];
       }
-      float s[NT][2][4];
+      stage = stage == STAGES - U ? 0 : stage + U;
+      float x[U][NT][4];
 #pragma unroll
-      for (int w = 0; w < KW; ++w) {
-        const int g2 = KG == 2 ? w / 4 : 0;
-        const ScalePair sa = scale_pair(ks[0][g2], ks[0][g2]), sb = scale_pair(ks[1][g2], ks[1][g2]);
-        const uint32_t a0 = dequant<0>(kw[0][w], sa), a1 = dequant<0>(kw[1][w], sb), a2 = dequant<1>(kw[0][w], sa),
-                       a3 = dequant<1>(kw[1][w], sb), a4 = dequant<2>(kw[0][w], sa), a5 = dequant<2>(kw[1][w], sb),
-                       a6 = dequant<3>(kw[0][w], sa), a7 = dequant<3>(kw[1][w], sb);
+      for (int u = 0; u < U; ++u) {
+        uint32_t kw[2][KW], ks[2][KG];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          const uint2 q0 = qs[(2 * w * NT + t) * 32 + lane], q1 = qs[((2 * w + 1) * NT + t) * 32 + lane];
-          if (w == 0) {
-            mma_bf16_zero(s[t][0], a0, a1, a2, a3, q0.x, q0.y);
-            mma_bf16_zero(s[t][1], a4, a5, a6, a7, q1.x, q1.y);
-          } else {
-            mma_bf16(s[t][0], a0, a1, a2, a3, q0.x, q0.y);
-            mma_bf16(s[t][1], a4, a5, a6, a7, q1.x, q1.y);
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t at = blk + u * Stage<D>::bytes;
+          load_words<(KW > 4 ? 4 : KW)>(at + k_at[0] + h * 4 * D, kw[h]);
+          if constexpr (KW > 4) load_words<4>(at + k_at[1] + h * 4 * D, kw[h] + 4);
+#pragma unroll
+          for (int y = 0; y < KG; ++y) ks[h][y] = load_scale(at + ks_at + h * (D / 2) + 8 * y);
+        }
+#pragma unroll
+        for (int w = 0; w < KW; ++w) {
+          const int g2 = KG == 2 ? w / 4 : 0;
+          const ScalePair sa = scale_pair(ks[0][g2], ks[0][g2]), sb = scale_pair(ks[1][g2], ks[1][g2]);
+          const uint32_t a0 = dequant<0>(kw[0][w], sa), a1 = dequant<0>(kw[1][w], sb), a2 = dequant<1>(kw[0][w], sa),
+                         a3 = dequant<1>(kw[1][w], sb), a4 = dequant<2>(kw[0][w], sa), a5 = dequant<2>(kw[1][w], sb),
+                         a6 = dequant<3>(kw[0][w], sa), a7 = dequant<3>(kw[1][w], sb);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            const uint2 q0 = qs[(2 * w * NT + t) * 32 + lane], q1 = qs[((2 * w + 1) * NT + t) * 32 + lane];
+            if (w == 0) mma_bf16_zero(x[u][t], a0, a1, a2, a3, q0.x, q0.y);
+            else mma_bf16(x[u][t], a0, a1, a2, a3, q0.x, q0.y);
+            mma_bf16(x[u][t], a4, a5, a6, a7, q1.x, q1.y);
           }
         }
       }
-      uint32_t vw[4][VW], vs[4];
+      uint32_t vw[U][4][VW], vs[U][4];
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        load_words<VW>(blk + v_at[x & 1] + (x >> 1) * 4 * D, vw[x]);
-        vs[x] = load_scale(blk + vs_at + ((x & 1) + 8 * (x >> 1)) * (D / 16));
-      }
-      const auto see = [&](int ps, int j) {
-        return !gone && j <= ps && (p.window == 0 || j > ps - p.window || j < p.sinks);
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          const uint32_t at = blk + u * Stage<D>::bytes;
+          load_words<VW>(at + v_at[y & 1] + (y >> 1) * 4 * D, vw[u][y]);
+          vs[u][y] = load_scale(at + vs_at + ((y & 1) + 8 * (y >> 1)) * (D / 16));
+        }
+      const auto see = [&](int u, int ps, int j) {
+        return !gone[u] && j <= ps && (p.window == 0 || j > ps - p.window || j < p.sinks);
       };
-      float x[NT][4];
+      if (__any_sync(0xffffffffu, part)) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+              if (!see(u, pos[t][y & 1], j_now[u] + r + 8 * (y >> 1))) x[u][t][y] = -INFINITY;
+          // tokens no row sees may hold anything: their values become zeros
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            const int j = j_now[u] + 2 * c + (y & 1) + 8 * (y >> 1);
+            if (gone[u] || j > pmax || (p.window > 0 && j <= pmin - p.window && j >= p.sinks)) vs[u][y] = 0;
+          }
+        }
+      }
+      float top[NT][2];
+      bool up = false;
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int y = 0; y < 4; ++y) x[t][y] = s[t][0][y] + s[t][1][y];
-      if (__any_sync(0xffffffffu, tt < whole0 || tt >= whole1 || gone)) {
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int y = 0; y < 4; ++y)
-            if (!see(pos[t][y & 1], j_now + r + 8 * (y >> 1))) x[t][y] = -INFINITY;
-        // tokens no row sees may hold anything: their values become zeros
-#pragma unroll
-        for (int y = 0; y < 4; ++y) {
-          const int j = j_now + 2 * c + (y & 1) + 8 * (y >> 1);
-          if (gone || j > pmax || (p.window > 0 && j <= pmin - p.window && j >= p.sinks)) vs[y] = 0;
+        for (int j = 0; j < 2; ++j) {
+          top[t][j] = fmaxf(fmaxf(x[0][t][j], x[0][t][j + 2]), fmaxf(x[1][t][j], x[1][t][j + 2]));
+          up |= top[t][j] > lim[t][j];
         }
-      }
-      bool up = false;
-#pragma unroll
-      for (int t = 0; t < NT; ++t) up |= fmaxf(x[t][0], x[t][2]) > lim[t][0] || fmaxf(x[t][1], x[t][3]) > lim[t][1];
       if (__any_sync(0xffffffffu, up)) {
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
           float f[2];
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            float n2 = fmaxf(x[t][j], x[t][j + 2]);
+            float n2 = top[t][j];
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) n2 = fmaxf(n2, __shfl_xor_sync(0xffffffffu, n2, d));
             n2 = fmaxf(n2, m[t][j]);
@@ -737,58 +777,68 @@ __global__ void __launch_bounds__(kAttnWarps * 32, ctas_per_sm(D, NT)) kv4_atten
           }
         }
       }
-      uint32_t ph[NT][2], pl[NT][2];
+      uint32_t ph[U][NT][2], pl[U][NT][2];
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
+      for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int y = 0; y < 4; ++y) x[t][y] = ex2(fmaf(x[t][y], p.scale_log2, -z[t][y & 1]));
-        l[t][0] += x[t][0] + x[t][2];
-        l[t][1] += x[t][1] + x[t][3];
+        for (int t = 0; t < NT; ++t) {
+          float* e = x[u][t];
 #pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          const uint32_t h = pack_bf16x2(x[t][2 * y], x[t][2 * y + 1]);
-          const uint32_t e = pack_bf16x2(x[t][2 * y] - __uint_as_float(h << 16), x[t][2 * y + 1] - __uint_as_float(h & 0xFFFF0000u));
-          ph[t][y] = transpose8x8(h);
-          pl[t][y] = transpose8x8(e);
+          for (int y = 0; y < 4; ++y) e[y] = ex2(fmaf(e[y], p.scale_log2, -z[t][y & 1]));
+          l[t][0] += e[0] + e[2];
+          l[t][1] += e[1] + e[3];
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            const uint32_t hi = pack_bf16x2(e[2 * y], e[2 * y + 1]);
+            const uint32_t lo = pack_bf16x2(e[2 * y] - __uint_as_float(hi << 16), e[2 * y + 1] - __uint_as_float(hi & 0xFFFF0000u));
+            ph[u][t][y] = transpose8x8(SPLIT && c >= 2 ? lo : hi);
+            if constexpr (!SPLIT) pl[u][t][y] = transpose8x8(lo);
+          }
         }
-      }
       // A value group with an infinity or a NaN is NaN in the outputs of the rows that see it; as a factor it
       // reaches the others of the tile too (0 * NaN).  Where an output came out as no number the blocks are walked
       // again with such groups taken out of the product and added to their rows here.
       if (careful) {
-        for (int k = 0; k < 16; ++k) {
-          const int y = (k & 1) + 2 * (k >> 3), src = r * 4 + (k % 8) / 2;
-          const uint32_t sk = __shfl_sync(0xffffffffu, y == 0 ? vs[0] : y == 1 ? vs[1] : y == 2 ? vs[2] : vs[3], src);
-          if ((sk & 0x7F80u) != 0x7F80u) continue;
 #pragma unroll
-          for (int t = 0; t < NT; ++t)
+        for (int u = 0; u < U; ++u) {
+          for (int k = 0; k < 16; ++k) {
+            const int y = (k & 1) + 2 * (k >> 3), src = r * 4 + (k % 8) / 2;
+            const uint32_t own = y == 0 ? vs[u][0] : y == 1 ? vs[u][1] : y == 2 ? vs[u][2] : vs[u][3];
+            const uint32_t sk = __shfl_sync(0xffffffffu, own, src);
+            if ((sk & 0x7F80u) != 0x7F80u) continue;
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
-              if (see(pos[t][j], j_now + k)) {
+            for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int w = 0; w < VW * 4; ++w) o[t][w][j] = o[t][w][j + 2] = __uint_as_float(0x7FC00000u);
-              }
-        }
+              for (int j = 0; j < 2; ++j)
+                if (see(u, pos[t][j], j_now[u] + k)) {
 #pragma unroll
-        for (int y = 0; y < 4; ++y)
-          if ((vs[y] & 0x7F80u) == 0x7F80u) vs[y] = 0;
-      }
-      const ScalePair va = scale_pair(vs[0], vs[1]), vb = scale_pair(vs[2], vs[3]);
-#pragma unroll
-      for (int w = 0; w < VW; ++w) {
-        const uint32_t xa = __byte_perm(vw[0][w], vw[1][w], 0x5410), ya = __byte_perm(vw[0][w], vw[1][w], 0x7632);
-        const uint32_t xb = __byte_perm(vw[2][w], vw[3][w], 0x5410), yb = __byte_perm(vw[2][w], vw[3][w], 0x7632);
-        const auto tile = [&](int x4, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
-#pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            mma_bf16(o[t][x4], a0, a1, a2, a3, ph[t][0], ph[t][1]);
-            mma_bf16(o[t][x4], a0, a1, a2, a3, pl[t][0], pl[t][1]);
+                  for (int w = 0; w < VW * 4; ++w) o[t][w][j] = o[t][w][j + 2] = __uint_as_float(0x7FC00000u);
+                }
           }
-        };
-        tile(4 * w + 0, dequant<0>(xa, va), dequant<0>(ya, va), dequant<0>(xb, vb), dequant<0>(yb, vb));
-        tile(4 * w + 1, dequant<1>(xa, va), dequant<1>(ya, va), dequant<1>(xb, vb), dequant<1>(yb, vb));
-        tile(4 * w + 2, dequant<2>(xa, va), dequant<2>(ya, va), dequant<2>(xb, vb), dequant<2>(yb, vb));
-        tile(4 * w + 3, dequant<3>(xa, va), dequant<3>(ya, va), dequant<3>(xb, vb), dequant<3>(yb, vb));
+#pragma unroll
+          for (int y = 0; y < 4; ++y)
+            if ((vs[u][y] & 0x7F80u) == 0x7F80u) vs[u][y] = 0;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const ScalePair va = scale_pair(vs[u][0], vs[u][1]), vb = scale_pair(vs[u][2], vs[u][3]);
+#pragma unroll
+        for (int w = 0; w < VW; ++w) {
+          const uint32_t xa = __byte_perm(vw[u][0][w], vw[u][1][w], 0x5410), ya = __byte_perm(vw[u][0][w], vw[u][1][w], 0x7632);
+          const uint32_t xb = __byte_perm(vw[u][2][w], vw[u][3][w], 0x5410), yb = __byte_perm(vw[u][2][w], vw[u][3][w], 0x7632);
+          const auto tile = [&](int x4, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+              mma_bf16(o[t][x4], a0, a1, a2, a3, ph[u][t][0], ph[u][t][1]);
+              if constexpr (!SPLIT) mma_bf16(o[t][x4], a0, a1, a2, a3, pl[u][t][0], pl[u][t][1]);
+            }
+          };
+          tile(4 * w + 0, dequant<0>(xa, va), dequant<0>(ya, va), dequant<0>(xb, vb), dequant<0>(yb, vb));
+          tile(4 * w + 1, dequant<1>(xa, va), dequant<1>(ya, va), dequant<1>(xb, vb), dequant<1>(yb, vb));
+          tile(4 * w + 2, dequant<2>(xa, va), dequant<2>(ya, va), dequant<2>(xb, vb), dequant<2>(yb, vb));
+          tile(4 * w + 3, dequant<3>(xa, va), dequant<3>(ya, va), dequant<3>(xb, vb), dequant<3>(yb, vb));
+        }
       }
     }
     float sum = 0.f;
@@ -814,6 +864,13 @@ __global__ void __launch_bounds__(kAttnWarps * 32, ctas_per_sm(D, NT)) kv4_atten
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     const int k = warp * ROWS + 8 * t + 2 * c;
+    if constexpr (SPLIT) {   // columns 4 .. 7 have what P's low parts gave
+#pragma unroll
+      for (int x = 0; x < VW * 4; ++x)
+#pragma unroll
+        for (int y = 0; y < 4; ++y) o[t][x][y] += __shfl_down_sync(0xffffffffu, o[t][x][y], 2);
+      if (c >= 2) continue;
+    }
 #pragma unroll
     for (int w = 0; w < VW; ++w)
 #pragma unroll
@@ -871,7 +928,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32, ctas_per_sm(D, NT)) kv4_atten
       *reinterpret_cast<uint2*>(p.out + b * p.o_bstride + i * p.o_ld + (int64_t)(hk * group + row0 + k - i * group) * D + d) = w;
     } else {
       // a unit shared with other CTAs: a CTA has at most two, at its first block and at its last
-      const int64_t pr = ((int64_t)blockIdx.x * 2 + (g == g0 ? 0 : 1)) * ROWS + k;
+      const int64_t pr = ((int64_t)blockIdx.x * 2 + (begins <= g0 ? 0 : 1)) * ROWS + k;
       *reinterpret_cast<float4*>(p.part_o + pr * D + d) = acc;
       if (d == 0) {
         p.part_ml[pr * 2] = M;
@@ -885,8 +942,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32, ctas_per_sm(D, NT)) kv4_atten
   }
   // who has the first of a shared unit's blocks names it: the entry and head, and the CTAs that share it
   if (threadIdx.x == 0 && first == 0 && last < n)
-    p.part_head[blockIdx.x] = make_int2(entry * kv.Hkv + hk, (int)((g + n - 1) / per) - (int)blockIdx.x + 1 + (g == g0 ? 0 : 1 << 30));
-  g += last - first;
+    p.part_head[blockIdx.x] = make_int2(entry * kv.Hkv + hk, (begins + kSetup + n - 1) / per - (int)blockIdx.x + 1 + (begins <= g0 ? 0 : 1 << 30));
+  g = begins + kSetup + last;
   if (g < g1) __syncthreads();   // the next unit stages its rows where the sums were
   }
 }
@@ -994,7 +1051,7 @@ void kv4_attention_plan(Kv4AttnParams* p) {
 bool kv4_attention_fits(Kv4AttnParams p) {
   const Kv4Params& kv = p.kv;
   const double tiles = (double)kv.B * kv.Hkv * (((double)kv.L * (p.Hq / kv.Hkv)) / 8 + 1);
-  return tiles * ((double)kv.max_pages * kv.P / 16 + 1) < 2147480000.0;
+  return tiles * ((double)kv.max_pages * kv.P / 16 + 1 + kSetup) < 2147480000.0;
 }
 
 // Two partial tiles per CTA (outputs, then maxima and sums), then the names of shared units.
@@ -1006,13 +1063,13 @@ size_t kv4_attention_workspace(Kv4AttnParams p) {
 
 namespace {
 
-template <int D, int NT, int CL>
+template <int D, int NT, bool SPLIT, int CL>
 cudaError_t launch_attention_t(const Kv4AttnParams& p, cudaStream_t stream) {
   constexpr int bytes = (int)AttnSmem<D, NT>::bytes;
   if (bytes > 48 * 1024) {
     static DeviceOnce once;
     const cudaError_t e = once_per_device(
-        once, [] { return cudaFuncSetAttribute(kv4_attention_kernel<D, NT, CL>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); });
+        once, [] { return cudaFuncSetAttribute(kv4_attention_kernel<D, NT, SPLIT, CL>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); });
     if (e != cudaSuccess) return e;
   }
   cudaLaunchConfig_t cfg = {};
@@ -1026,7 +1083,7 @@ cudaError_t launch_attention_t(const Kv4AttnParams& p, cudaStream_t stream) {
   cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
   cfg.attrs = &cluster;
   cfg.numAttrs = CL > 1 ? 1 : 0;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, kv4_attention_kernel<D, NT, CL>, p);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kv4_attention_kernel<D, NT, SPLIT, CL>, p);
   if (e != cudaSuccess || CL > 1 || p.ctas == 1) return e;
   cudaLaunchAttribute early;   // set up while the first kernel runs; it waits for that kernel's end by itself
   early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -1039,11 +1096,17 @@ cudaError_t launch_attention_t(const Kv4AttnParams& p, cudaStream_t stream) {
   return cudaLaunchKernelEx(&cfg, kv4_join_kernel<D>, p);
 }
 
+template <int D, int CL>
+cudaError_t launch_attention_r(const Kv4AttnParams& p, cudaStream_t stream) {
+  if (p.kv.L * (p.Hq / p.kv.Hkv) <= 4) return launch_attention_t<D, 1, true, CL>(p, stream);
+  return p.row_nt == 1 ? launch_attention_t<D, 1, false, CL>(p, stream) : launch_attention_t<D, 2, false, CL>(p, stream);
+}
+
 template <int D>
 cudaError_t launch_attention_d(const Kv4AttnParams& p, cudaStream_t stream) {
   if (p.cluster)
-    return p.row_nt == 1 ? launch_attention_t<D, 1, kCluster>(p, stream) : launch_attention_t<D, 2, kCluster>(p, stream);
-  return p.row_nt == 1 ? launch_attention_t<D, 1, 1>(p, stream) : launch_attention_t<D, 2, 1>(p, stream);
+    return launch_attention_r<D, kCluster>(p, stream);
+  return launch_attention_r<D, 1>(p, stream);
 }
 
 }  // namespace
