@@ -164,7 +164,9 @@ __device__ __forceinline__ bool quantise_keys(const float* x, const Turn& t, flo
 }
 
 // A CTA per token; a warp takes 256 / D heads of one kind (q, k or v) at a time, eight values a lane.  Instructions bound it
-// rather than the bytes of q | k | v: unpacking, norms and codes of a value cost about ten.
+// rather than the bytes of q | k | v: unpacking, norms and codes of a value cost about ten.  16 x 500 tokens of 32 + 2 x 8
+// heads of 128: 49.7 us from bf16 (3.5 TB/s), 52.8 us from fp32 (5.1 TB/s).  Six CTAs of eight warps fit an SM; loading
+// the next head ahead cost registers for that and was slower (72.8 against 64.8 us when it was tried).
 template <typename T, int D>
 __global__ void __launch_bounds__(256, 6) kv4_append_kernel(const Kv4AppendParams p) {
   constexpr int LANES = D / 8, HPW = 32 / LANES, half = D / 2;
@@ -245,7 +247,8 @@ __global__ void __launch_bounds__(256, 6) kv4_append_kernel(const Kv4AppendParam
   }
 }
 
-// A CTA per R rows, a thread per word (8 values) of each: the rows' loads are under way together.
+// A CTA per R rows, a thread per word (8 values) of each: the rows' loads are under way together.  Bound by the latency of
+// table, codes and stores in turn: 16 x 500 tokens of 8 heads of 128 in 15.3 us (2.7 TB/s).
 template <int R>
 __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4Params p, __nv_bfloat16* __restrict__ out, int64_t ldo,
                                                        int64_t bstride) {
@@ -326,7 +329,7 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4Params p, __nv_b
 // The running maximum moves only when a score exceeds it by 2^8 in the exponent's base, which keeps sums in
 // range without a reduction over lanes per block.
 
-constexpr int kAttnWarps = 4;
+constexpr int kAttnWarps = 4;       // with 8, a call over 1024 tokens took 10.6 us instead of 7.7
 constexpr int kAtOnce = 2;          // blocks that a warp takes at a time
 constexpr int kSetup = 20;          // what another unit costs a CTA, in blocks (0, 8, 20, 32: 69.6, 67.6, 64.3, 64.9 us
                                     // at 4 tokens over 131071; 74.7, 73.0, 72.5, 72.6 us at 40 sequences up to 8192)
@@ -442,6 +445,7 @@ struct AttnSmem {
   static constexpr size_t bytes = (q + ring > o ? q + ring : o) + ml;
 };
 
+// As many as registers and shared memory hold.  More (4 and 5 of fewer registers) took 80.7 and 84.8 us where 3 took 78.7.
 constexpr int ctas_per_sm(int D, int NT) { return NT == 1 && D < 256 ? 3 : 2; }
 
 // NT: tiles of eight query rows; SPLIT: one tile of at most four, whose columns 4 .. 7 are its rows again.  CL: 1, or the
@@ -998,7 +1002,9 @@ template <typename T>
 cudaError_t launch_append_t(const Kv4AppendParams& p, unsigned rows, cudaStream_t stream) {
   const int hpw = 256 / p.kv.D;
   const int slots = (p.Hq + hpw - 1) / hpw + 2 * ((p.kv.Hkv + hpw - 1) / hpw);
-  const int threads = 32 * std::min(slots, rows >= 8 * 148 ? 4 : 8);   // with many tokens, fewer warps share a token's set-up
+  // with many tokens, fewer warps share a token's set-up (heads 32 + 2 x 8 of 128, 4 and 8 warps: 1 token 5.1 and 4.0 us,
+  // 2048 tokens 19.0 and 18.4 us, 8000 tokens 49.8 and 55.9 us)
+  const int threads = 32 * std::min(slots, rows >= 8 * 148 ? 4 : 8);
   switch (p.kv.D) {
     case 64: kv4_append_kernel<T, 64><<<rows, threads, 0, stream>>>(p); break;
     case 128: kv4_append_kernel<T, 128><<<rows, threads, 0, stream>>>(p); break;
@@ -1021,7 +1027,7 @@ cudaError_t launch_kv4_read(const Kv4Params& p, __nv_bfloat16* out, int64_t ldo,
   const int64_t rows = (int64_t)p.B * p.L;
   if (rows > 0x7FFFFFFFLL) return cudaErrorInvalidValue;
   const int threads = std::min(256, (2 * p.Hkv * (p.D / 8) + 31) / 32 * 32);
-  if (rows >= 8 * 148)
+  if (rows >= 8 * 148)   // one and two rows per CTA, 8 heads of 128: 1024 rows 3.4 and 3.7 us, 2048 5.2 and 4.9, 8000 17.2 and 15.3
     kv4_read_kernel<2><<<(unsigned)((rows + 1) / 2), threads, 0, stream>>>(p, out, ldo, bstride);
   else
     kv4_read_kernel<1><<<(unsigned)rows, threads, 0, stream>>>(p, out, ldo, bstride);
@@ -1032,7 +1038,11 @@ constexpr int kCluster = 8;
 
 // Row tiles (two tiles of eight rows at a time share the converted operand where there are more than eight rows), and the
 // CTAs: a cluster per unit where these fit one wave and no unit is longer than eight blocks per warp, else one wave, but
-// at least a block of 16 tokens for each warp of the longest sequences.
+// at least a block of 16 tokens for each warp of the longest sequences.  Measured in us, 4 query heads per kv head:
+//   cluster / wave            1 sequence of 1024: 7.5 / 9.8 (D 256), 6.3 / 8.4 (D 128);  16384: 27.2 / 29.7, 19.5 / 18.5;
+//                             16 of 4096: 15.2 / 15.0, 11.2 / 12.6
+//   16 rows, two tiles / one  2 x 32768 tokens, 8 kv heads of 128: 39.0 / 47.9;  12 rows: 37.7 / 47.4
+//   4 rows, the low terms of P in the spare columns / in products of their own: 40 x 8192 tokens, 8 kv heads: 97.3 / 101.2
 void kv4_attention_plan(Kv4AttnParams* p) {
   const Kv4Params& kv = p->kv;
   const int64_t rows = (int64_t)kv.L * (p->Hq / kv.Hkv);
