@@ -454,8 +454,8 @@ nsa_status nsa_expand4(const nsa_weight4* w, void* out, int64_t ldo, void* strea
 
 /* nsa_linear4: ops.linear (app/gpu/ops.js:50-66) with a 4-bit weight, for decode steps:
  *   C[m*ldc + n] = r, or += r with resid, where r = sum_k A[m][k] W[n][k] (+ bias[n]).
- * A bf16 [M][lda]; K and lda multiples of 8, K at most 98304 (NSA_ERR_UNSUPPORTED), A 16-byte aligned; C fp32 or (store form) bf16, at its
- * element alignment; C must not overlap A.  The products are exact and sums are kept in fp32, so the result
+ * A bf16 [M][lda]; K and lda multiples of 8, A 16-byte aligned; C fp32 or (store form) bf16, at its element
+ * alignment; C must not overlap A.  K up to 98304; above 49152, N up to 524288 (NSA_ERR_UNSUPPORTED beyond).  The products are exact and sums are kept in fp32, so the result
  * is the fp32 linear's.  Any M runs; the weights are read once per 32 rows of A (fewer where 32 rows of K do not
  * fit shared memory), so for hundreds of rows nsa_linear over the nsa_expand4 copy is faster. */
 typedef struct nsa_linear4_desc {

@@ -1668,6 +1668,9 @@ nsa_status nsa_linear4(const nsa_linear4_desc* d, const nsa_weight4* w, const vo
   const double bytes = (double)w->N * w->K * (0.5 + 2.0 / w->group) + 2.0 * d->M * w->K +
                        (double)d->M * w->N * esz * (d->resid ? 2 : 1);
   cudaError_t e = profiled("linear4", 2.0 * d->M * w->N * w->K, bytes, strm, [&] { return nsa::launch_linear4(p, strm); });
+  if (e == cudaErrorNotSupported)
+    return fail(NSA_ERR_UNSUPPORTED, "a row of " + std::to_string(w->K) + " values for " + std::to_string(w->N) +
+                                         " outputs does not fit the shared memories of a cluster");
   if (e != cudaSuccess) return cuda_fail(e, "linear4 launch");
   return NSA_OK;
 }
@@ -1813,7 +1816,8 @@ static nsa_status kv4_attention_params(const nsa_kv4_attention_desc* d, const ns
   if (d->Hq < 1 || d->Hq % cache->Hkv) return fail(NSA_ERR_INVALID_ARGUMENT, "Hq must be a positive multiple of Hkv");
   if (d->window < 0 || d->sinks < 0) return fail(NSA_ERR_INVALID_ARGUMENT, "window and sinks must be >= 0");
   if (d->sinks > 0 && d->window == 0) return fail(NSA_ERR_INVALID_ARGUMENT, "sinks needs a window");
-  if (!(d->scale >= 0.f) || d->scale > 3.0e38f) return fail(NSA_ERR_INVALID_ARGUMENT, "scale must be finite and >= 0");
+  if (!(d->scale >= 0.f) || d->scale > 2.0e38f)   // times log2 e
+    return fail(NSA_ERR_INVALID_ARGUMENT, "scale must be >= 0 and at most 2e38");
   if ((d->q_ld | d->q_bstride | d->o_ld | d->o_bstride) % 8 || d->q_ld < 0 || d->q_bstride < 0)
     return fail(NSA_ERR_INVALID_ARGUMENT, "the q and out pitches must be multiples of 8, >= 0");
   p->Hq = d->Hq;

@@ -436,25 +436,31 @@ Linear4Plan linear4_plan(const Linear4Params& p, int rows, int sms) {
 
 }  // namespace
 
-// Rows of X per pass: up to 32, fewer where no cluster holds them, evenly over the passes.
+// Rows of X per pass: up to 32, fewer where no cluster holds them, evenly over the passes; passes are the grid's second
+// axis, of at most 65535.  cudaErrorNotSupported: not even one row fits.
 cudaError_t launch_linear4(Linear4Params p, cudaStream_t stream) {
   const int sms = device_sm_count();
-  int rows = std::min(p.M, 32);
-  Linear4Plan plan = linear4_plan(p, rows, sms);
-  while (plan.WK == 0 && rows > 1) plan = linear4_plan(p, --rows, sms);
-  if (plan.WK == 0) return cudaErrorInvalidValue;
-  const int passes = (p.M + rows - 1) / rows;
-  if (passes > 65535) return cudaErrorInvalidValue;
-  p.rows = (p.M + passes - 1) / passes;
-  if (p.rows < rows) plan = linear4_plan(p, p.rows, sms);
-  p.WK = plan.WK;
-  p.CS = plan.CS;
-  const dim3 grid((unsigned)(plan.clusters * p.CS), (unsigned)passes);
-  switch (p.G) {
-    case 32: return launch_linear_g<32>(p, grid, plan.bytes, stream);
-    case 64: return launch_linear_g<64>(p, grid, plan.bytes, stream);
-    default: return launch_linear_g<128>(p, grid, plan.bytes, stream);
+  int most = std::min(p.M, 32);
+  Linear4Plan plan = linear4_plan(p, most, sms);
+  while (plan.WK == 0 && most > 1) plan = linear4_plan(p, --most, sms);
+  if (plan.WK == 0) return cudaErrorNotSupported;
+  const int size = p.out_bf16 ? 2 : 4;
+  for (int left = p.M; left > 0; left -= p.M) {
+    p.M = (int)std::min<int64_t>(left, (int64_t)most * 65535);
+    const int passes = (p.M + most - 1) / most;
+    p.rows = (p.M + passes - 1) / passes;
+    plan = linear4_plan(p, p.rows, sms);
+    p.WK = plan.WK;
+    p.CS = plan.CS;
+    const dim3 grid((unsigned)(plan.clusters * p.CS), (unsigned)passes);
+    const cudaError_t e = p.G == 32   ? launch_linear_g<32>(p, grid, plan.bytes, stream)
+                          : p.G == 64 ? launch_linear_g<64>(p, grid, plan.bytes, stream)
+                                      : launch_linear_g<128>(p, grid, plan.bytes, stream);
+    if (e != cudaSuccess) return e;
+    p.x += (int64_t)p.M * p.ldx;
+    p.c = static_cast<char*>(p.c) + (int64_t)p.M * p.ldc * size;
   }
+  return cudaSuccess;
 }
 
 }  // namespace nsa

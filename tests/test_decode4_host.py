@@ -174,6 +174,14 @@ def test_wrappers_refuse_host_tensors_and_wrong_shapes():
         ops.kv4_cache(4, 1, 64, page=20)
 
 
+def test_linear4_refuses_rows_that_fit_no_cluster():
+    """K = 98304 leaves room for 2^19 outputs, not for 2^22: refused before anything is launched."""
+    w = _lib.Weight4Desc(1 << 22, 98304, 32, FAKE, FAKE)
+    d = _lib.Linear4Desc(1, 0, 0, 0, 0)
+    assert _lib.lib().nsa_linear4(ctypes.byref(d), ctypes.byref(w), FAKE, None, FAKE + (1 << 30), None) == UNSUP
+    assert b"shared memories" in _lib.lib().nsa_last_error()
+
+
 def test_oracle_format():
     """Scales have five significant bits, are the smallest that reach the largest value, and every value of the
     format is a bf16 number within half a step of the input."""

@@ -199,6 +199,21 @@ def test_linear4_rows_of_wide_range_and_infinities(M):
     assert (np.sign(y[np.isinf(y)]) == np.sign(want[np.isinf(want)])).all()
 
 
+def test_linear4_more_rows_than_one_grid_takes():
+    """65535 passes of 32 rows are one launch; the rows behind them are another, with the same sums."""
+    from nanosaur2_web_b200.ops import linear4
+    rng = np.random.default_rng(5)
+    W, Wv, _ = linear_case(rng, 1, 9, 8, 32)
+    M = 32 * 65535 + 5
+    x = torch.randint(-8, 9, (M, 8), device="cuda").to(BF)
+    out = torch.zeros((M + 1, 9), device="cuda")
+    linear4(x, W, out=out[:M])
+    check_device()
+    want = x.double() @ t(Wv, torch.float64).T
+    tol = (32 + 1 + 16) * 2.0 ** -23 * (x.double().abs() @ t(np.abs(Wv), torch.float64).T)   # linear_tol's factor
+    assert ((out[:M].double() - want).abs() <= tol + 1e-37).all() and (out[M] == 0).all()
+
+
 def test_linear4_empty_and_other_stream():
     from nanosaur2_web_b200.ops import linear4
     rng = np.random.default_rng(9)
