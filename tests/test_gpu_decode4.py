@@ -403,6 +403,30 @@ def test_kv4_attention_long_and_split(D, Hkv, P, T):
     assert (np.abs(n64(got) - want) <= tol).all(), float((np.abs(n64(got) - want) / tol).max())
 
 
+@pytest.mark.parametrize("D,group,L", [(64, 4, 1), (128, 2, 2), (256, 1, 1), (128, 1, 4), (256, 3, 1), (64, 5, 1)])
+def test_kv4_attention_few_rows_of_long_sequences(D, group, L):
+    """Up to four rows per kv head share one tile's columns with their low parts; five do not.  Long sequences of other
+    lengths, so that units are shared out and joined; a token whose values are infinite counts for the rows that see it."""
+    from nanosaur2_web_b200.ops import kv4_attention
+    rng = np.random.default_rng(D + group)
+    B, Hkv, P, T = 2, 2, 32, 4600
+    cd = Cached(rng, B, T, Hkv, D, P)
+    q = t(2 * rng.standard_normal((B, L, group * Hkv * D)), BF)
+    start = np.array([T - L, 4200], np.int32)
+    run = lambda: n64(kv4_attention(q, cd.cache, cd.table, t(start, torch.int32)))
+    got = run()
+    want, tol = attend_oracle(cd, n64(q), start, [L] * B, 0, 0, 1 / np.sqrt(D))
+    assert (np.abs(got - want) <= tol).all(), float((np.abs(got - want) / tol).max())
+    k, v = cd.k.copy(), cd.v.copy()
+    v[0, T - 1] = np.inf                                              # seen by the last new token of sequence 0 alone
+    cd.fill(k, v)
+    again = run()
+    check_device()
+    assert np.isnan(again[0, L - 1]).all()
+    got[0, L - 1] = again[0, L - 1] = 0
+    assert (np.abs(again - want)[:, :max(L - 1, 0)] <= tol[:, :max(L - 1, 0)]).all() and np.array_equal(again[1], got[1])
+
+
 @pytest.mark.parametrize("B,L,Hq,Hkv,D,P,T,window,sinks", [(90, 1, 4, 2, 64, 16, 60, 0, 0), (70, 3, 6, 1, 128, 16, 45, 0, 0),
                                                            (37, 2, 4, 4, 256, 16, 40, 9, 3), (100, 1, 1, 1, 64, 16, 300, 33, 0),
                                                            (3, 70, 3, 3, 64, 16, 90, 0, 0)])
