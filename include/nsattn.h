@@ -498,7 +498,7 @@ typedef struct nsa_kv4_batch {
 /* nsa_kv4_append: the step's q | k | v rows, element (b, i, col) at qkv[b*bstride + i*ld + col], q heads at
  * qOff + h*D, k at kOff, v at vOff.  Per head, q and k get the RMSNorm and the split-half RoPE of
  * ops.headNorm (app/gpu/ops.js:131-138) in the same pass, at RoPE row position; q' is written as bf16 to
- * q_out[b*qo_bstride + i*qo_ld + h*D], k' and v are quantised into the cache.  Keys are computed in fp64, so
+ * q_out[b*qo_bstride + i*qo_ld + h*D], k' and v are quantised into the cache.  Keys are defined in fp64, so
  * which code a value on the border of two gets does not depend on an order of sums.  cs NULL: no rotation.
  * qkv fp32 or bf16; its base 16-byte aligned, ld, bstride and offsets multiples of 4 elements. */
 typedef struct nsa_kv4_append_desc {
