@@ -27,7 +27,7 @@
 extern "C" {
 #endif
 
-#define NSA_ABI_VERSION 5
+#define NSA_ABI_VERSION 6
 
 typedef enum nsa_status {
   NSA_OK = 0,
@@ -471,8 +471,8 @@ nsa_status nsa_linear4(const nsa_linear4_desc* desc, const nsa_weight4* w, const
 /* The cache: a pool of pages of P tokens for Hkv key/value heads of D values, in groups of 32 along D:
  *   codes  uint8 [n_pages][2][Hkv][P][D / 2] (keys, then values; value 2 j in the low nibble of byte j),
  *   scales bf16 [n_pages][2][Hkv][P][D / 32].
- * D 64, 128 or 256; P a multiple of 16, at most 1024; both 16-byte aligned.  A slot that was never written
- * is never read. */
+ * D 64, 128 or 256; P a multiple of 16, at most 1024; both 16-byte aligned.  What a slot that was never written
+ * holds does not matter. */
 typedef struct nsa_kv4_cache {
   int32_t n_pages, P, Hkv, D;
   uint8_t* codes;
@@ -483,9 +483,11 @@ typedef struct nsa_kv4_cache {
  * stored before the step.  count (optional): new tokens of each sequence, clamped to [0, L]; rows past them
  * are neither read nor written.  table, start and count are device int32 arrays, read when the kernels run.
  * Pages may be shared between sequences for reading; no slot may be written twice in one call.
- * A position outside the table, or past the RoPE table, and a page id outside the pool are skipped and
+ * A position outside the table, or at `positions` or past it, and a page id outside the pool are skipped and
  * recorded: nsa_check_device then returns NSA_ERR_DEVICE.  Skipped tokens are not written; as keys they are
- * masked. */
+ * masked, as queries they see nothing.  nsa_kv4_append skips tokens past its RoPE table as well: where the page table
+ * spans more tokens than that has rows, set `positions` to the rows, so that reads and attention leave the same
+ * tokens out. */
 typedef struct nsa_kv4_batch {
   int32_t B, L;
   int32_t max_pages;     /* page table columns; max_pages * P <= 2^31 - 1 */
@@ -493,6 +495,7 @@ typedef struct nsa_kv4_batch {
   const int32_t* table;
   const int32_t* start;
   const int32_t* count;  /* or NULL */
+  int32_t positions;     /* positions there are (0: max_pages * P) */
 } nsa_kv4_batch;
 
 /* nsa_kv4_append: the step's q | k | v rows, element (b, i, col) at qkv[b*bstride + i*ld + col], q heads at

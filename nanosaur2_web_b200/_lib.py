@@ -116,7 +116,7 @@ class Kv4CacheDesc(ctypes.Structure):
 class Kv4Batch(ctypes.Structure):
     """nsa_kv4_batch (include/nsattn.h)."""
     _fields_ = [("B", _i32), ("L", _i32), ("max_pages", _i32), ("table_ld", _i64), ("table", _vp), ("start", _vp),
-                ("count", _vp)]
+                ("count", _vp), ("positions", _i32)]
 
 
 class Kv4AppendDesc(ctypes.Structure):

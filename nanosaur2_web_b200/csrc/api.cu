@@ -756,7 +756,7 @@ nsa_status nsa_check_device(void* stream) {
   if (e != cudaSuccess) return cuda_fail(e, "device check");
   if (host != 0) {
     const char* what = host == nsa::kErrKvPage       ? "a page table entry outside the cache's pool"
-                       : host == nsa::kErrKvPosition ? "a token position outside the page table or the RoPE table"
+                       : host == nsa::kErrKvPosition ? "a token position outside the page table, the RoPE table or the batch's positions"
                                                      : "a bounded wait expired";
     char buf[128];
     std::snprintf(buf, sizeof buf, "device-side error 0x%x (%s)", host, what);
@@ -1684,7 +1684,8 @@ static nsa_status kv4_params(const nsa_kv4_cache* c, const nsa_kv4_batch* s, nsa
   if (c->n_pages < 0 || c->Hkv < 1) return fail(NSA_ERR_INVALID_ARGUMENT, "need n_pages >= 0 and Hkv >= 1");
   if ((double)c->n_pages * 2 * c->Hkv * (c->P / 16) >= 4294967296.0)   // blocks of 16 tokens are counted in 32 bits
     return fail(NSA_ERR_UNSUPPORTED, "the pool holds 2^32 or more blocks of 16 tokens of a head");
-  if (s->B < 0 || s->L < 0 || s->max_pages < 0) return fail(NSA_ERR_INVALID_ARGUMENT, "need B, L and max_pages >= 0");
+  if (s->B < 0 || s->L < 0 || s->max_pages < 0 || s->positions < 0)
+    return fail(NSA_ERR_INVALID_ARGUMENT, "need B, L, max_pages and positions >= 0");
   if ((int64_t)s->max_pages * c->P > 0x7FFFFFFFLL)
     return fail(NSA_ERR_INVALID_ARGUMENT, "the page table spans more than 2^31 - 1 tokens");
   const int64_t ld = s->table_ld ? s->table_ld : s->max_pages;
@@ -1700,6 +1701,8 @@ static nsa_status kv4_params(const nsa_kv4_cache* c, const nsa_kv4_batch* s, nsa
   p->B = s->B;
   p->L = s->L;
   p->max_pages = s->max_pages;
+  p->cap = s->max_pages * c->P;
+  if (s->positions > 0) p->cap = std::min(p->cap, s->positions);
   p->table = s->table;
   p->table_ld = ld;
   p->start = s->start;
@@ -1774,7 +1777,7 @@ nsa_status nsa_kv4_append(const nsa_kv4_append_desc* d, const nsa_kv4_cache* cac
   p.k_w = k_norm_w;
   p.cs = cs;
   p.sin_off = d->sinOff;
-  p.rope_rows = d->rope_rows;
+  if (cs) p.kv.cap = std::min(p.kv.cap, d->rope_rows);
   p.eps = d->eps;
   p.q_out = static_cast<__nv_bfloat16*>(q_out);
   p.qo_ld = d->qo_ld;

@@ -151,7 +151,7 @@ nsa_kv4_cache cache_of(const Tensor& codes, const Tensor& scales) {
 }
 
 // The step; *table may be replaced by a contiguous copy (to be kept until the launch).
-nsa_kv4_batch batch_of(int64_t B, int64_t L, Tensor* table, const Tensor& start, const OptTensor& count) {
+nsa_kv4_batch batch_of(int64_t B, int64_t L, Tensor* table, const Tensor& start, const OptTensor& count, int64_t positions) {
   if (table->dim() != 2 || table->size(0) != B || table->scalar_type() != at::kInt ||
       (table->size(1) > 1 && table->stride(1) != 1))
     invalid("table must be an int32 [" + std::to_string(B) + ", max_pages] tensor with unit inner stride");
@@ -171,6 +171,7 @@ nsa_kv4_batch batch_of(int64_t B, int64_t L, Tensor* table, const Tensor& start,
   b.table = table->data_ptr<int32_t>();
   b.start = start.data_ptr<int32_t>();
   b.count = static_cast<const int32_t*>(data(count));
+  b.positions = int32_of(positions, "positions");
   return b;
 }
 
@@ -215,7 +216,7 @@ Tensor kv4_append(const Tensor& qkv, const Tensor& codes, const Tensor& scales, 
   OnDevice on(dev);
   const Tensor out = out_ ? *out_ : at::empty({x.B, x.L, Hq * D}, qkv.options().dtype(at::kBFloat16));
   const Rows o = result_rows(out, "out", x.B, x.L, Hq * D);
-  const nsa_kv4_batch b = batch_of(x.B, x.L, &table, start, count);
+  const nsa_kv4_batch b = batch_of(x.B, x.L, &table, start, count, 0);
   nsa_kv4_append_desc d{};
   d.Hq = (int32_t)Hq;
   d.in_dtype = dtype_code(qkv, "qkv");
@@ -234,7 +235,7 @@ Tensor kv4_append(const Tensor& qkv, const Tensor& codes, const Tensor& scales, 
   return out;
 }
 
-Tensor kv4_read(const Tensor& codes, const Tensor& scales, Tensor table, const Tensor& start, int64_t L,
+Tensor kv4_read(const Tensor& codes, const Tensor& scales, int64_t positions, Tensor table, const Tensor& start, int64_t L,
                 const OptTensor& count, const OptTensor& out_) {
   const auto dev = Devices()(codes)(scales)(table)(start)(count)(out_).index();
   const nsa_kv4_cache c = cache_of(codes, scales);
@@ -243,13 +244,13 @@ Tensor kv4_read(const Tensor& codes, const Tensor& scales, Tensor table, const T
   OnDevice on(dev);
   const Tensor out = out_ ? *out_ : at::zeros({B, L, width}, scales.options());
   const Rows o = result_rows(out, "out", B, L, width);
-  const nsa_kv4_batch b = batch_of(B, L, &table, start, count);
+  const nsa_kv4_batch b = batch_of(B, L, &table, start, count, positions);
   check(nsa_kv4_read(&c, &b, out.data_ptr(), o.ld, o.bstride, on.stream));
   return out;
 }
 
-Tensor kv4_attention(const Tensor& q, const Tensor& codes, const Tensor& scales, Tensor table, const Tensor& start,
-                     const OptTensor& count, int64_t window, int64_t sinks, double scale, const OptTensor& out_,
+Tensor kv4_attention(const Tensor& q, const Tensor& codes, const Tensor& scales, int64_t positions, Tensor table,
+                     const Tensor& start, const OptTensor& count, int64_t window, int64_t sinks, double scale, const OptTensor& out_,
                      const OptTensor& workspace_) {
   const auto dev = Devices()(q)(codes)(scales)(table)(start)(count)(out_)(workspace_).index();
   const nsa_kv4_cache c = cache_of(codes, scales);
@@ -259,7 +260,7 @@ Tensor kv4_attention(const Tensor& q, const Tensor& codes, const Tensor& scales,
   OnDevice on(dev);
   const Tensor out = out_ ? *out_ : at::empty({x.B, x.L, x.cols}, q.options());
   const Rows o = result_rows(out, "out", x.B, x.L, x.cols);
-  const nsa_kv4_batch b = batch_of(x.B, x.L, &table, start, count);
+  const nsa_kv4_batch b = batch_of(x.B, x.L, &table, start, count, positions);
   nsa_kv4_attention_desc d{};
   d.Hq = int32_of(x.cols / c.D, "Hq");
   d.q_ld = x.ld;

@@ -4,7 +4,7 @@
 //
 // Pages: codes [n_pages][2][Hkv][P][D / 2] (keys, then values; value 2j in the low, 2j + 1 in the high
 // nibble of byte j), scales [n_pages][2][Hkv][P][D / 32] bf16.  Token t of sequence b is slot t % P of page
-// table[b][t / P].  A page id outside the pool, and a position outside the table (or the RoPE table), is
+// table[b][t / P].  A page id outside the pool, and a position from `cap` on (past the page table, or the RoPE table), is
 // recorded in the device error word and its access skipped.
 #include <algorithm>
 
@@ -33,10 +33,10 @@ __device__ __forceinline__ int64_t cache_row(const Kv4Params& p, int page, int w
   return (((int64_t)page * 2 + which) * p.Hkv + h) * p.P + pos % p.P;
 }
 
-// Position of new token i of sequence b; -1 (recorded) when it lies outside the table.
+// Position of new token i of sequence b; -1 (recorded) when it lies outside.
 __device__ __forceinline__ int position(const Kv4Params& p, int b, int i) {
   const int64_t pos = (int64_t)p.start[b] + i;
-  if (p.start[b] < 0 || pos >= (int64_t)p.max_pages * p.P) {
+  if (p.start[b] < 0 || pos >= p.cap) {
     atomicCAS(p.err, 0, kErrKvPosition);
     return -1;
   }
@@ -177,10 +177,6 @@ __global__ void __launch_bounds__(256, 6) kv4_append_kernel(const Kv4AppendParam
   if (i >= new_tokens(kv, b)) return;
   const int pos = position(kv, b, i);
   if (pos < 0) return;
-  if (p.cs && pos >= p.rope_rows) {
-    if (threadIdx.x == 0) atomicCAS(kv.err, 0, kErrKvPosition);
-    return;
-  }
   const T* row = static_cast<const T*>(p.qkv) + b * p.bstride + i * p.ld + hl * 4;
   int slot = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0);
   if (slot < q_slots) {
@@ -394,7 +390,7 @@ __device__ __forceinline__ Blocks blocks_of(int pmin, int pmax, int window, int 
 __device__ __forceinline__ int token_of(const Kv4Params& kv, int R, int group) { return kv.L == 1 ? 0 : R / group; }
 
 // The rows of row tile rt of sequence b: new tokens i_first .. i_last (none: i_last < i_first) at positions pmin .. pmax;
-// outside: some of them lie outside the table and see nothing.
+// outside: some of them lie outside and see nothing.
 struct Tile {
   int row0, rows, i_first, i_last, pmin, pmax;
   bool outside;
@@ -407,7 +403,7 @@ __device__ __forceinline__ Tile tile_of(const Kv4AttnParams& p, int b, int rt, i
   t.rows = min(rows_per_tile, kv.L * group - t.row0);
   t.i_first = token_of(kv, t.row0, group);
   t.i_last = min(token_of(kv, t.row0 + t.rows - 1, group), new_tokens(kv, b) - 1);
-  const int64_t start = kv.start[b], cap = (int64_t)kv.max_pages * kv.P;
+  const int64_t start = kv.start[b], cap = kv.cap;
   t.outside = t.i_last >= t.i_first && (start < 0 || start + t.i_last >= cap);
   t.pmin = (int)(start + t.i_first);
   t.pmax = (int)min(start + t.i_last, cap - 1);

@@ -315,6 +315,7 @@ struct Kv4Params {
   uint8_t* codes;           // [n_pages][2][Hkv][P][D / 2]
   __nv_bfloat16* scales;    // [n_pages][2][Hkv][P][D / 32]
   int B, L, max_pages;      // sequences, rows of new tokens per sequence, page table width
+  int cap;                  // positions from here on are outside
   const int* table;         // [B][table_ld]
   int64_t table_ld;
   const int* start;         // [B] tokens stored before this step
@@ -328,9 +329,8 @@ struct Kv4AppendParams {
   int64_t ld, bstride, q_off, k_off, v_off;
   const float* q_w;
   const float* k_w;
-  const float* cs;          // RoPE table (cos [rope_rows][D / 2], sin at sin_off) or null
+  const float* cs;          // RoPE table (cos [kv.cap rows][D / 2], sin at sin_off) or null
   int64_t sin_off;
-  int rope_rows;
   float eps;
   __nv_bfloat16* q_out;     // row (b, i) at b * qo_bstride + i * qo_ld
   int64_t qo_ld, qo_bstride;

@@ -474,9 +474,12 @@ class Kv4Cache:
     """A pool of pages of keys and values in 4 bits: ``codes`` uint8 [n_pages, 2, Hkv, P, D/2] and ``scales``
     bf16 [n_pages, 2, Hkv, P, D/32] in the order of include/nsattn.h (nsa_kv4_cache).  Which page holds which
     tokens is the caller's page table: int32 [B, max_pages], position t of sequence b in slot t % P of page
-    table[b, t // P]."""
+    table[b, t // P].  ``positions`` (0: as many as the page table spans): tokens from this position on are outside, like
+    those past the page table.  ``kv4_append`` stores no token past its RoPE table and sets this to the table's rows (0 without
+    one), so that the calls that read the cache leave the same tokens out; another handle on the same memory is given it."""
     codes: torch.Tensor
     scales: torch.Tensor
+    positions: int = 0
 
     @property
     def page(self) -> int:
@@ -493,7 +496,7 @@ class Kv4Cache:
 
 def kv4_cache(n_pages: int, Hkv: int, D: int, page: int = 64, device=None) -> Kv4Cache:
     """An empty pool of ``n_pages`` pages of ``page`` tokens (a multiple of 16, at most 1024) for Hkv heads of
-    D (64, 128 or 256) values.  Unwritten slots are never read, so the memory is left as it is."""
+    D (64, 128 or 256) values.  What unwritten slots hold does not matter, so the memory is left as it is."""
     if D not in (64, 128, 256):
         raise NsaError(_lib.NSA_ERR_UNSUPPORTED, "the 4-bit cache holds head dims 64, 128 and 256")
     if n_pages < 0 or Hkv < 1 or page % 16 or not 16 <= page <= 1024:
@@ -512,18 +515,20 @@ def kv4_append(qkv: torch.Tensor, cache: Kv4Cache, table: torch.Tensor, start: t
     Per head q and k get the RMSNorm (q_norm, k_norm float32 [D]) and the split-half RoPE of ``headNorm`` at their
     position (``cs``, None for no rotation); k and v are stored in 4 bits in the pages of ``table``, and q comes back
     as bf16 [B, L, Hq*D] (``out``), ``kv4_attention``'s operand.  start and count are device int32 [B]; rows past
-    count[b] are neither read nor written."""
+    count[b], and tokens past the page table or ``cs`` (reported by ``check_device``), are neither read nor written."""
     buf, rows, dim, sin_off = (None, 0, 0, 0) if cs is None else (cs.buf, cs.L, cs.D, cs.sinOff)
-    return _native().kv4_append(qkv, cache.codes, cache.scales, table, start, count, Hq, q_norm, k_norm, buf, rows, dim,
-                                sin_off, eps, qOff, kOff, vOff, out)
+    out = _native().kv4_append(qkv, cache.codes, cache.scales, table, start, count, Hq, q_norm, k_norm, buf, rows, dim,
+                               sin_off, eps, qOff, kOff, vOff, out)
+    cache.positions = 0 if cs is None else cs.L
+    return out
 
 
 def kv4_read(cache: Kv4Cache, table: torch.Tensor, start: torch.Tensor, L: int, *, count: Optional[torch.Tensor] = None,
              out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Positions start[b] .. start[b] + L - 1 of every sequence back as bf16 rows [B, L, 2*Hkv*D], key heads then
     value heads (nsa_kv4_read; exact): what ``attention`` takes as k and v.  Rows past count[b] are left as they
-    were (zeros when ``out`` is not given)."""
-    return _native().kv4_read(cache.codes, cache.scales, table, start, L, count, out)
+    were (zeros when ``out`` is not given), and so are positions outside."""
+    return _native().kv4_read(cache.codes, cache.scales, cache.positions, table, start, L, count, out)
 
 
 def kv4_attention(q: torch.Tensor, cache: Kv4Cache, table: torch.Tensor, start: torch.Tensor, *,
@@ -533,7 +538,8 @@ def kv4_attention(q: torch.Tensor, cache: Kv4Cache, table: torch.Tensor, start: 
     (nsa_kv4_attention).  q bf16 [B, L, Hq*D] (``kv4_append``'s result), query heads h*Hq/Hkv .. sharing key/value
     head h; the query at position p = start[b] + i sees keys j <= p, with ``window`` > 0 only those with
     j > p - window or j < ``sinks``.  Returns bf16 [B, L, Hq*D] (``out``); rows past count[b] are left as they
-    were (``out`` not given: uninitialised).  scale 0 means 1/sqrt(D).  ``workspace``: a uint8 tensor to
+    were (``out`` not given: uninitialised), rows at positions outside are zeros.  scale 0 means 1/sqrt(D).  ``workspace``: a uint8 tensor to
     reuse, as large as the C call asks (nsa_kv4_attention_workspace_size; the error names the size), allocated per
     call when not given; calls that overlap on the GPU need one each."""
-    return _native().kv4_attention(q, cache.codes, cache.scales, table, start, count, window, sinks, scale, out, workspace)
+    return _native().kv4_attention(q, cache.codes, cache.scales, cache.positions, table, start, count, window, sinks, scale, out,
+                                   workspace)

@@ -195,3 +195,17 @@ def test_oracle_format():
     v = O4.values(c, s)
     assert (np.abs(v - x) <= s.repeat(32, -1) / 2).all()
     assert (torch.from_numpy(v).bfloat16().double().numpy() == v).all()
+
+
+def test_batch_positions():
+    """`positions` is refused below 0; the workspace's size does not depend on it."""
+    L = _lib.lib()
+    c, bad = cache_of(), _lib.Kv4Batch(**BATCH, positions=-1)
+    t = _lib.Kv4AttentionDesc(4, 512, 1536, 512, 1536, 0, 0, 0)
+    a = _lib.Kv4AppendDesc(Hq=4, in_dtype=0, ld=1024, bstride=3 * 1024, qOff=0, kOff=512, vOff=768, qo_ld=512, qo_bstride=1536, eps=1e-6)
+    assert L.nsa_kv4_append(ctypes.byref(a), ctypes.byref(c), ctypes.byref(bad), FAKE, FAKE, FAKE, None, OUT, None) == BAD
+    assert L.nsa_kv4_read(ctypes.byref(c), ctypes.byref(bad), OUT, 512, 1536, None) == BAD
+    assert L.nsa_kv4_attention(ctypes.byref(t), ctypes.byref(c), ctypes.byref(bad), FAKE, OUT, FAKE, 1 << 40, None) == BAD
+    assert b"positions" in L.nsa_last_error()
+    size = lambda n: L.nsa_kv4_attention_workspace_size(ctypes.byref(t), ctypes.byref(c), ctypes.byref(_lib.Kv4Batch(**{**BATCH, "max_pages": 4096}, positions=n)))
+    assert size(0) == size(50) == size(4096 * 16) == size(1 << 30) > 0

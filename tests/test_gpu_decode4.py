@@ -764,3 +764,69 @@ def test_kv4_empty_batches_and_pools():
         assert (ops.kv4_attention(q, cache, tab, start) == 0).all()
         with pytest.raises(ops.NsaError, match=match):
             check_device()
+
+
+def test_kv4_tokens_past_the_rope_table_are_masked_in_every_later_call():
+    """60 rows of RoPE over 4 pages of 16: tokens 60 .. 63 fit the page table but are not stored.  Their slots (NaN here) count
+    for nothing, their queries write zeros, in the same step and in later ones."""
+    from nanosaur2_web_b200 import ops
+    rng = np.random.default_rng(31)
+    B, Hq, Hkv, D, P, rows = 2, 4, 2, 128, 16, 60
+    cache = ops.kv4_cache(B * 4 + 1, Hkv, D, P, DEV)
+    cache.codes.fill_(0xFF)
+    cache.scales.fill_(float("nan"))
+    table = t(rng.permutation(B * 4 + 1)[:B * 4].reshape(B, 4), torch.int32)
+    w, cs = torch.ones(D, device=DEV), ops.ropeTable(rows, D, 1e4, DEV)
+
+    def append(L, start, count=None):
+        x = t(rng.standard_normal((B, L, (Hq + 2 * Hkv) * D)))
+        out = torch.full((B, L, Hq * D), 9.0, dtype=BF, device=DEV)
+        return ops.kv4_append(x, cache, table, t(start, torch.int32), count=None if count is None else t(count, torch.int32),
+                              Hq=Hq, q_norm=w, k_norm=w, cs=cs, out=out)
+
+    def attend(q, start):
+        out = torch.full_like(q, 7.0)
+        return ops.kv4_attention(q, cache, table, t(start, torch.int32), out=out)
+
+    def check(got, q, start, counts):
+        class Known:
+            pass
+        cd = Known()
+        kv = n64(ops.kv4_read(cache, table, t([0, 0], torch.int32), 60)).reshape(B, 60, 2, Hkv, D)
+        cd.k, cd.v, cd.D, cd.Hkv = kv[:, :, 0], kv[:, :, 1], D, Hkv
+        want, tol = attend_oracle(cd, n64(q), start, counts, 0, 0, 1 / np.sqrt(D))
+        got = n64(got)
+        for b in range(B):
+            assert (np.abs(got[b, :counts[b]] - want[b, :counts[b]]) <= tol[b, :counts[b]]).all(), b
+            assert (got[b, counts[b]:] == 0).all(), b
+    append(56, [0, 0], [56, 10])
+    check_device()
+    q = append(8, [56, 10])
+    with pytest.raises(ops.NsaError, match="position"):
+        check_device()
+    assert (q[0, 4:] == 9).all()
+    got = attend(q, [56, 10])
+    with pytest.raises(ops.NsaError, match="position"):
+        check_device()
+    check(got, q, [56, 10], [4, 8])
+    q = append(1, [62, 18])
+    with pytest.raises(ops.NsaError, match="position"):
+        check_device()
+    got = attend(q, [62, 18])
+    with pytest.raises(ops.NsaError, match="position"):
+        check_device()
+    check(got, q, [62, 18], [0, 1])
+    out = torch.full((B, 4, 2 * Hkv * D), 5.0, dtype=BF, device=DEV)
+    ops.kv4_read(cache, table, t([58, 0], torch.int32), 4, out=out)
+    with pytest.raises(ops.NsaError, match="position"):
+        check_device()
+    assert (out[0, 2:] == 5).all() and not torch.isnan(out).any()
+    # a longer table takes the same positions; another handle on the same memory is told the limit
+    cs = ops.ropeTable(64, D, 1e4, DEV)
+    q = append(2, [60, 19])
+    attend(q, [60, 19])
+    check_device()
+    other = ops.Kv4Cache(cache.codes, cache.scales, positions=60)
+    assert (ops.kv4_attention(q, other, table, t([60, 19], torch.int32))[0] == 0).all()
+    with pytest.raises(ops.NsaError, match="position"):
+        check_device()
