@@ -132,7 +132,9 @@ __device__ __forceinline__ void quantise_halves(const T* x, uint32_t* bits, floa
 // the fp32 order of sums would decide it by chance.  So fp32 decides where its error cannot matter.  The error of a
 // value is below 2^-19 r (|x own| + |mate's x mate|): 2^-22 of rsqrtf, half of 15 roundings of the mean square under its
 // root, five of the products.  A lane answers false where that is more than 2^-17 of the group's largest magnitude am, where am lies within
-// 2^-16 of a border of two scales, or where a code changes within +- 2^-17 am (with 2^-20 of x for 1 / s).
+// 2^-16 of a border of two scales, or where a code changes within +- 2^-17 am (with 2^-20 of x for 1 / s).  The bound of r
+// holds for squares that are normal numbers: with r below 2^50 the mean square is above 2^-101, and what the squares lose
+// as subnormals, 2^-150 each, is nothing to it.
 __device__ __forceinline__ bool quantise_keys(const float* x, const Turn& t, float r, uint32_t* bits, float* s) {
   bool sure = true;
 #pragma unroll
@@ -150,7 +152,7 @@ __device__ __forceinline__ bool quantise_keys(const float* x, const Turn& t, flo
     s[k] = q4_scale(am);
     const float below = __uint_as_float(__float_as_uint(s[k]) - 0x00080000u), near = am * 0x1p-16f, step = am * 0x1p-17f;
     sure = sure && off * r * 0x1p-19f <= step && fabsf(7.f * s[k] - am) > near && fabsf(7.f * below - am) > near &&
-           am > 0x1p-109f && am < 0x1p119f;   // (no number: false)
+           am > 0x1p-109f && am < 0x1p119f && r < 0x1p50f;   // (no number: false)
     const float inv = __fdividef(1.f, s[k]), lo = inv * (1.f - 0x1p-20f), hi = inv * (1.f + 0x1p-20f);
     bits[k] = 0u - 0x4B400000u * 0x1111u;
 #pragma unroll

@@ -830,3 +830,24 @@ def test_kv4_tokens_past_the_rope_table_are_masked_in_every_later_call():
     assert (ops.kv4_attention(q, other, table, t([60, 19], torch.int32))[0] == 0).all()
     with pytest.raises(ops.NsaError, match="position"):
         check_device()
+
+
+@pytest.mark.parametrize("size", [1e-19, 1e-21, 3e-22, 1e-23, 1e-37, 1e18, 1e25, 1e37])
+@pytest.mark.parametrize("D", [64, 256])
+def test_kv4_append_keys_of_any_size_without_eps(D, size):
+    """eps = 0 and heads whose squares are subnormal, zero or infinite in fp32: codes are those of fp64."""
+    from nanosaur2_web_b200 import ops
+    rng = np.random.default_rng(D)
+    B, L, Hkv, P = 1, 700, 4, 16
+    qkv = t(rng.standard_normal((B, L, 3 * Hkv * D)) * size)
+    kw = t(1 + 0.2 * rng.standard_normal(D))
+    mp = -(-L // P)
+    cache, table = ops.kv4_cache(mp, Hkv, D, P, DEV), t(rng.permutation(mp).reshape(1, mp), torch.int32)
+    start = torch.zeros(1, dtype=torch.int32, device=DEV)
+    cs = ops.ropeTable(L, D, 1e4, DEV)
+    ops.kv4_append(qkv, cache, table, start, Hq=Hkv, q_norm=kw, k_norm=kw, cs=cs, eps=0.0)
+    kv = n64(ops.kv4_read(cache, table, start, L))[:, :, :Hkv * D]
+    check_device()
+    cos, sin = n64(cs.buf[:cs.sinOff]).reshape(L, 1, D // 2), n64(cs.buf[cs.sinOff:]).reshape(L, 1, D // 2)
+    k = O4.norm_rope(n64(qkv[:, :, Hkv * D:2 * Hkv * D]).reshape(B, L, Hkv, D), n64(kw), cos, sin, 0.0)
+    np.testing.assert_array_equal(kv, O4.values(*O4.quantise(k.reshape(B, L, -1), 32)))
