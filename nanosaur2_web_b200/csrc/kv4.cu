@@ -191,7 +191,14 @@ __global__ void __launch_bounds__(256, 6) kv4_append_kernel(const Kv4AppendParam
       float x[8], o[8];
       load4(row + p.q_off + at, x);
       load4(row + p.q_off + at + half, x + 4);
-      const float r = inv_rms<float, LANES>(x, p.eps);
+      float r = inv_rms<float, LANES>(x, p.eps);
+      // squares that are infinite, or so small that subnormal ones weigh, are taken of the head times a power of two
+      if (__any_sync(0xffffffffu, !(r > 0.f && r < 0x1p50f))) {
+        const float c = r >= 0x1p50f ? 0x1p100f : r > 0.f ? 1.f : 0x1p-70f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] *= c;
+        r = inv_rms<float, LANES>(x, p.eps * c * c);
+      }
 #pragma unroll
       for (int e = 0; e < 8; ++e) o[e] = fmaf(x[e ^ 4], t.mate[e], x[e] * t.own[e]) * r;
       if (live) {

@@ -851,3 +851,26 @@ def test_kv4_append_keys_of_any_size_without_eps(D, size):
     cos, sin = n64(cs.buf[:cs.sinOff]).reshape(L, 1, D // 2), n64(cs.buf[cs.sinOff:]).reshape(L, 1, D // 2)
     k = O4.norm_rope(n64(qkv[:, :, Hkv * D:2 * Hkv * D]).reshape(B, L, Hkv, D), n64(kw), cos, sin, 0.0)
     np.testing.assert_array_equal(kv, O4.values(*O4.quantise(k.reshape(B, L, -1), 32)))
+
+
+@pytest.mark.parametrize("size", [1e-19, 1e-21, 1e-23, 1e-37, 1e18, 1e25, 1e37])
+@pytest.mark.parametrize("D", [64, 256])
+@pytest.mark.parametrize("rope", [True, False])
+def test_kv4_append_queries_of_any_size_without_eps(D, size, rope):
+    """The same for q': unit rows whatever the input's size, to the tolerance of ordinary ones."""
+    from nanosaur2_web_b200 import ops
+    rng = np.random.default_rng(D + 1)
+    B, L, Hq, P = 1, 20, 3, 32
+    qkv = t(rng.standard_normal((B, L, (Hq + 2) * D)) * size)
+    qkv[0, 3] = t(rng.standard_normal((Hq + 2) * D))                  # an ordinary token between them
+    w = t(1 + 0.2 * rng.standard_normal(D))
+    cache, table = ops.kv4_cache(1, 1, D, P, DEV), t([[0]], torch.int32)
+    cs = ops.ropeTable(L, D, 1e4, DEV) if rope else None
+    q = n64(ops.kv4_append(qkv, cache, table, t([0], torch.int32), Hq=Hq, q_norm=w, k_norm=w, cs=cs, eps=0.0)).reshape(L, Hq, D)
+    check_device()
+    cos = n64(cs.buf[:cs.sinOff]).reshape(L, 1, D // 2) if rope else None
+    sin = n64(cs.buf[cs.sinOff:]).reshape(L, 1, D // 2) if rope else None
+    x = n64(qkv)[0, :, :Hq * D].reshape(L, Hq, D)
+    want, plain = O4.norm_rope(x, n64(w), cos, sin, 0.0), np.abs(O4.norm_rope(x, n64(w), None, None, 0.0))
+    pair = plain + np.roll(plain, D // 2, -1)
+    assert (np.abs(q - want) <= 2.0 ** -8 * np.abs(want) + 20 * 2.0 ** -24 * pair + 1e-30).all()
