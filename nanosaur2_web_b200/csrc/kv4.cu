@@ -331,8 +331,9 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4Params p, __nv_b
 // blocks of 8 heads for 16 rows (D 128) take the time that they take with them; without the products and conversions,
 // 40 us of 64.  Two blocks at a time give the scheduler independent chains (D 256: 33.2 -> 29.7 us at 8 x 32768 tokens)
 // and share the walk, the tests of masks and maxima (466 instead of 594 instructions a block).
-// The running maximum moves only when a score exceeds it by 2^8 in the exponent's base, which keeps sums in
-// range without a reduction over lanes per block.
+// The running maximum moves only when a score exceeds it by 2^8 in the exponent's base, which spares a reduction over
+// lanes per block.  What is subtracted from the scores is the maximum and `shift` more, ceil(log2(tokens a row may see))
+// + 1, so that the weights of a row sum to at most 2^7 and the unnormalised outputs of the largest values, 2^120, stay finite.
 
 constexpr int kAttnWarps = 4;       // with 8, a call over 1024 tokens took 10.6 us instead of 7.7
 constexpr int kAtOnce = 2;          // blocks that a warp takes at a time
@@ -665,8 +666,8 @@ __global__ void __launch_bounds__(kAttnWarps * 32, ctas_per_sm(D, NT)) kv4_atten
   }
   __syncthreads();
 
-  // m: the largest raw score so far; lim: what a score may reach before m moves; z: the scaled maximum subtracted (0
-  // while there is none)
+  // m: the largest raw score so far; lim: what a score may reach before m moves; z: the scaled maximum + shift, which is
+  // subtracted (0 while there is none)
   const float slack = kMaxSlack / p.scale_log2;
   float o[NT][VW * 4][4], m[NT][2], lim[NT][2], z[NT][2], l[NT][2];
   // The second pass, only after an output that is not a number: see `careful` below.
@@ -773,8 +774,9 @@ __global__ void __launch_bounds__(kAttnWarps * 32, ctas_per_sm(D, NT)) kv4_atten
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) n2 = fmaxf(n2, __shfl_xor_sync(0xffffffffu, n2, d));
             n2 = fmaxf(n2, m[t][j]);
-            z[t][j] = n2 == -INFINITY ? 0.f : n2 * p.scale_log2;
-            f[j] = ex2(m[t][j] * p.scale_log2 - z[t][j]);
+            const float old = z[t][j];
+            z[t][j] = n2 == -INFINITY ? 0.f : fmaf(n2, p.scale_log2, p.shift);
+            f[j] = m[t][j] == -INFINITY ? 0.f : ex2(old - z[t][j]);
             m[t][j] = n2;
             lim[t][j] = n2 == -INFINITY ? n2 : n2 + slack;
             l[t][j] *= f[j];
@@ -1056,6 +1058,9 @@ void kv4_attention_plan(Kv4AttnParams* p) {
   const int64_t units = (int64_t)kv.B * kv.Hkv * p->row_tiles;
   const int64_t cap = (int64_t)kv.max_pages * kv.P / 16;
   const int64_t seen = p->window > 0 ? std::min(cap, ((int64_t)p->window + 8 * p->row_nt + 30) / 16 + (p->sinks + 15) / 16) : cap;
+  int bits = 4;   // 2^bits tokens at least that a row may see
+  while ((int64_t)1 << bits < seen * 16) ++bits;
+  p->shift = bits + 1.f;
   const int wave = 148 * ctas_per_sm(kv.D, p->row_nt);
   p->cluster = units * kCluster <= wave && seen <= kCluster * kAttnWarps * 8;
   const int64_t most = (units * std::max<int64_t>(seen, 1) + kAttnWarps - 1) / kAttnWarps;

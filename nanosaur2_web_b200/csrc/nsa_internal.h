@@ -346,11 +346,12 @@ struct Kv4AttnParams {
   __nv_bfloat16* out;
   int64_t o_ld, o_bstride;
   // set by the launch
+  float shift;              // what is subtracted from the scaled scores besides their maximum
   int row_nt, row_tiles;    // 8 row_nt query rows per row tile; row tiles per sequence and kv head
   int cluster;              // 1: a cluster of CTAs per unit, joined in shared memory (no workspace)
   int ctas;                 // CTAs that the blocks of 16 tokens are dealt out to
   float* part_o;            // [ctas][2][8 row_nt][D] unnormalised outputs of units shared with other CTAs
-  float* part_ml;           // [ctas][2][8 row_nt][2] maximum (base 2) and sum
+  float* part_ml;           // [ctas][2][8 row_nt][2] subtracted maximum (base 2) and sum
   int2* part_head;          // [ctas] the shared unit whose first block the CTA has (-1: none), and its CTAs
 };
 bool kv4_attention_fits(Kv4AttnParams p);           // sequences x heads x table width within one launch

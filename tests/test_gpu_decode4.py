@@ -874,3 +874,22 @@ def test_kv4_append_queries_of_any_size_without_eps(D, size, rope):
     want, plain = O4.norm_rope(x, n64(w), cos, sin, 0.0), np.abs(O4.norm_rope(x, n64(w), None, None, 0.0))
     pair = plain + np.roll(plain, D // 2, -1)
     assert (np.abs(q - want) <= 2.0 ** -8 * np.abs(want) + 20 * 2.0 ** -24 * pair + 1e-30).all()
+
+
+@pytest.mark.parametrize("D,group,L,T", [(128, 4, 1, 300), (256, 4, 1, 5000), (64, 2, 4, 9000), (128, 3, 4, 5000)])
+def test_kv4_attention_of_the_largest_values(D, group, L, T):
+    """Values of nearly 2^120, which the format holds, with scores that rise slowly (the running maximum lags behind), and
+    with equal scores of thousands of tokens: the average is finite, so is the result."""
+    from nanosaur2_web_b200.ops import kv4_attention
+    rng = np.random.default_rng(T)
+    cd = Cached(rng, 1, T, 1, D, 32)
+    k = np.zeros((1, T, 1, D))
+    k[..., :32] = 7.0 * np.linspace(-3, 3, T)[None, :, None, None]    # a group of equal values: stored as they are, nearly
+    v = (0.9 + 0.1 * rng.random((1, T, 1, D))) * 2.0 ** 119.9
+    cd.fill(k, v)
+    for size in (0.0, 0.02, 0.3):
+        q = t(size * np.ones((1, L, group * D)), BF)
+        got = n64(kv4_attention(q, cd.cache, cd.table, t([T - L], torch.int32)))
+        check_device()
+        want, tol = attend_oracle(cd, n64(q), [T - L], [L], 0, 0, 1 / np.sqrt(D))
+        assert (np.abs(got - want) <= tol).all(), (size, float(np.abs(got / want - 1).max()))
