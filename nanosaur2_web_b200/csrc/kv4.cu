@@ -1057,7 +1057,7 @@ void kv4_attention_plan(Kv4AttnParams* p) {
   p->row_tiles = (int)((rows + 8 * p->row_nt - 1) / (8 * p->row_nt));
   const int64_t units = (int64_t)kv.B * kv.Hkv * p->row_tiles;
   const int64_t cap = (int64_t)kv.max_pages * kv.P / 16;
-  const int64_t seen = p->window > 0 ? std::min(cap, ((int64_t)p->window + 8 * p->row_nt + 30) / 16 + (p->sinks + 15) / 16) : cap;
+  const int64_t seen = p->window > 0 ? std::min(cap, ((int64_t)p->window + 8 * p->row_nt + 30) / 16 + ((int64_t)p->sinks + 15) / 16) : cap;
   int bits = 4;   // 2^bits tokens at least that a row may see
   while ((int64_t)1 << bits < seen * 16) ++bits;
   p->shift = bits + 1.f;

@@ -209,3 +209,13 @@ def test_batch_positions():
     assert b"positions" in L.nsa_last_error()
     size = lambda n: L.nsa_kv4_attention_workspace_size(ctypes.byref(t), ctypes.byref(c), ctypes.byref(_lib.Kv4Batch(**{**BATCH, "max_pages": 4096}, positions=n)))
     assert size(0) == size(50) == size(4096 * 16) == size(1 << 30) > 0
+
+
+@pytest.mark.parametrize("sinks", [2 ** 31 - 1, 2 ** 31 - 15, 2 ** 31 - 16, 1 << 20])
+def test_attention_plan_of_any_number_of_sinks(sinks):
+    """Sinks that cover the whole table: planned like a call without a window."""
+    L = _lib.lib()
+    c, b = cache_of(), batch_of(max_pages=4096)
+    size = lambda window, n: L.nsa_kv4_attention_workspace_size(
+        ctypes.byref(_lib.Kv4AttentionDesc(4, 512, 1536, 512, 1536, window, n, 0)), ctypes.byref(c), ctypes.byref(b))
+    assert size(16, sinks) == size(0, 0) > 0
