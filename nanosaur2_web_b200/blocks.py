@@ -422,18 +422,58 @@ def gemma_layer(x: torch.Tensor, *, attn: dict, mlp: dict, cs: RopeTable, window
                               next_out=ab["h"] if next_norm is not None else None)
 
 
-def gemma_decode_buffers(B: int, L: int, hidden: int, inter: int, device) -> dict:
-    """Intermediates of ``gemma_layer_decode`` for B sequences of up to L new tokens: the normalised rows and the MLP's
-    (bf16), the linears' fp32 results, q', the attention's rows.  Zeroed, so that rows past a sequence's count stay
-    finite."""
-    M, QKV, A = B * L, (GEMMA_HEADS + 2 * GEMMA_KV_HEADS) * GEMMA_HEAD_DIM, GEMMA_HEADS * GEMMA_HEAD_DIM
+_GEMMA_QKV, _GEMMA_A = (GEMMA_HEADS + 2 * GEMMA_KV_HEADS) * GEMMA_HEAD_DIM, GEMMA_HEADS * GEMMA_HEAD_DIM
 
-    def zeros(shape, dtype):
-        return torch.zeros(shape, dtype=dtype, device=device)
-    return {"h": zeros((M, hidden), torch.bfloat16), "qkv": zeros((B, L, QKV), torch.float32),
-            "q": zeros((B, L, A), torch.bfloat16), "a": zeros((B, L, A), torch.bfloat16),
-            "o": zeros((M, hidden), torch.float32), "h2": zeros((M, hidden), torch.bfloat16),
-            "gu": zeros((M, 2 * inter), torch.float32), "g": zeros((M, inter), torch.bfloat16)}
+
+def _decode_buffer_specs(B: int, L: int, hidden: int, inter: int) -> tuple:
+    M, f32, bf16 = B * L, torch.float32, torch.bfloat16
+    return (("h", (M, hidden), bf16), ("qkv", (B, L, _GEMMA_QKV), f32), ("q", (B, L, _GEMMA_A), bf16), ("a", (B, L, _GEMMA_A), bf16),
+            ("o", (M, hidden), f32), ("h2", (M, hidden), bf16), ("gu", (M, 2 * inter), f32), ("g", (M, inter), bf16))
+
+
+def gemma_decode_buffers(B: int, L: int, hidden: int, inter: int, device) -> dict:
+    """Intermediates of ``gemma_layer_decode`` for x [B, L, hidden] (of other B or L: other buffers): the normalised rows
+    and the MLP's (bf16), the linears' fp32 results, q', the attention's rows.  Zeroed, so that rows past a sequence's
+    count stay finite."""
+    return {k: torch.zeros(shape, dtype=dtype, device=device) for k, shape, dtype in _decode_buffer_specs(B, L, hidden, inter)}
+
+
+def _check_decode(x: torch.Tensor, attn: dict, mlp: dict, buffers: Optional[dict], next_norm: Optional[torch.Tensor]) -> int:
+    """The sizes and devices that the layer's calls rely on (``linear`` takes pointers and pitches); returns inter."""
+    B, L, hidden = x.shape
+    device = x.device
+
+    def weight(d: dict, name: str, rows: int, cols: int) -> None:
+        W = d[name]
+        four = isinstance(W, Weight4)
+        if (four and (W.N != rows or W.K != cols)) or (not four and W.shape != (rows, cols)):
+            raise NsaError(_lib.NSA_ERR_INVALID_ARGUMENT, f"{name} must be [{rows}, {cols}]")
+        if (W.codes if four else W).device != device:
+            raise elsewhere()
+
+    def elsewhere() -> NsaError:
+        return NsaError(_lib.NSA_ERR_INVALID_ARGUMENT, "weights and buffers must live on x's device")
+    w_gu = mlp["w_gate_up"]
+    rows = w_gu.N if isinstance(w_gu, Weight4) else w_gu.shape[0]
+    if rows % 2:
+        raise NsaError(_lib.NSA_ERR_INVALID_ARGUMENT, "w_gate_up must have [gate; up] rows")
+    inter = rows // 2
+    weight(attn, "w_qkv", _GEMMA_QKV, hidden)
+    weight(attn, "w_o", hidden, _GEMMA_A)
+    weight(mlp, "w_gate_up", rows, hidden)
+    weight(mlp, "w_down", hidden, inter)
+    for norm in (attn["in_norm"], attn["post_norm"], mlp["pre_norm"], mlp["post_norm"], next_norm):
+        if norm is not None and norm.device != device:
+            raise elsewhere()
+    if buffers is not None:
+        for k, shape, dtype in _decode_buffer_specs(B, L, hidden, inter):
+            t = buffers.get(k)
+            if t is None or t.shape != shape or t.dtype != dtype or not t.is_contiguous():
+                raise NsaError(_lib.NSA_ERR_INVALID_ARGUMENT,
+                               f"the buffers are not gemma_decode_buffers({B}, {L}, {hidden}, {inter}): {k} must be {list(shape)}")
+            if t.device != device:
+                raise elsewhere()
+    return inter
 
 
 def _any_linear(x: torch.Tensor, W, out: torch.Tensor) -> None:
@@ -467,11 +507,8 @@ def gemma_layer_decode(x: torch.Tensor, *, attn: dict, mlp: dict, cs: RopeTable,
     if h_ready and buffers is None:
         raise NsaError(_lib.NSA_ERR_INVALID_ARGUMENT, "h_ready needs the buffers that hold h")
     B, L, hidden = x.shape
-    w_gu = mlp["w_gate_up"]
-    rows = w_gu.N if isinstance(w_gu, Weight4) else w_gu.shape[0]
-    if rows % 2:
-        raise NsaError(_lib.NSA_ERR_INVALID_ARGUMENT, "w_gate_up must have [gate; up] rows")
-    buf = buffers if buffers is not None else gemma_decode_buffers(B, L, hidden, rows // 2, x.device)
+    inter = _check_decode(x, attn, mlp, buffers, next_norm)
+    buf = buffers if buffers is not None else gemma_decode_buffers(B, L, hidden, inter, x.device)
     xs = x.view(B * L, hidden)
     if not h_ready:
         rmsnorm(xs, attn["in_norm"], hidden, eps, buf["h"])
@@ -481,7 +518,7 @@ def gemma_layer_decode(x: torch.Tensor, *, attn: dict, mlp: dict, cs: RopeTable,
     kv4_attention(buf["q"], cache, table, start, count=count, window=window, sinks=sinks, out=buf["a"])
     _any_linear(buf["a"].view(B * L, -1), attn["w_o"], buf["o"])
     rmsnorm(buf["o"], attn["post_norm"], hidden, eps, xs, accumulate=True, next_weight=mlp["pre_norm"], next_out=buf["h2"])
-    _any_linear(buf["h2"], w_gu, buf["gu"])
+    _any_linear(buf["h2"], mlp["w_gate_up"], buf["gu"])
     glu(buf["gu"], "gelu_tanh", out=buf["g"])
     _any_linear(buf["g"], mlp["w_down"], buf["o"])
     rmsnorm(buf["o"], mlp["post_norm"], hidden, eps, xs, accumulate=True, next_weight=next_norm,

@@ -219,3 +219,41 @@ def test_attention_plan_of_any_number_of_sinks(sinks):
     size = lambda window, n: L.nsa_kv4_attention_workspace_size(
         ctypes.byref(_lib.Kv4AttentionDesc(4, 512, 1536, 512, 1536, window, n, 0)), ctypes.byref(c), ctypes.byref(b))
     assert size(16, sinks) == size(0, 0) > 0
+
+
+def test_gemma_layer_decode_refuses_buffers_and_weights_of_other_sizes():
+    """`linear`, which takes bf16 weights, works on pointers and pitches: with h_ready, buffers of more rows than x would
+    have made it write past their qkv."""
+    from nanosaur2_web_b200 import blocks
+    bf, hid, inter = torch.bfloat16, 64, 48
+    w = lambda *s: torch.zeros(s, dtype=bf)
+    attn = dict(in_norm=torch.ones(hid), w_qkv=w(1536, hid), q_norm=torch.ones(256), k_norm=torch.ones(256), w_o=w(hid, 1024),
+                post_norm=torch.ones(hid))
+    mlp = dict(pre_norm=torch.ones(hid), w_gate_up=w(2 * inter, hid), w_down=w(hid, inter), post_norm=torch.ones(hid))
+    cache = ops.Kv4Cache(torch.zeros((2, 2, 1, 16, 128), dtype=torch.uint8), w(2, 2, 1, 16, 8))
+    make = lambda B, L, i=inter, dev="cpu": blocks.gemma_decode_buffers(B, L, hid, i, dev)
+
+    def call(attn=attn, mlp=mlp, **kw):
+        blocks.gemma_layer_decode(torch.zeros((1, 2, hid)), attn=attn, mlp=mlp, cs=None, cache=cache, h_ready="buffers" in kw,
+                                  table=torch.zeros((1, 2), dtype=torch.int32), start=torch.zeros(1, dtype=torch.int32), **kw)
+    good = make(1, 2)
+    bad = [dict(buffers=make(1, 4)), dict(buffers=make(2, 2)), dict(buffers=make(2, 1)), dict(buffers=make(1, 1)), dict(buffers=make(1, 2, inter + 8)),
+           dict(buffers={k: v for k, v in good.items() if k != "a"}), dict(buffers={**good, "gu": good["gu"].bfloat16()}),
+           dict(buffers={**good, "o": torch.zeros((hid, 2)).T})]
+    for kw in bad:
+        with pytest.raises(ops.NsaError, match="the buffers are not"):
+            call(**kw)
+    for name, W in (("w_qkv", w(1536, hid - 8)), ("w_qkv", w(1280, hid)), ("w_o", w(hid, 512)), ("w_o", w(8, 1024))):
+        with pytest.raises(ops.NsaError, match=name):
+            call(attn={**attn, name: W})
+    for name, W in (("w_gate_up", w(2 * inter, 8)), ("w_down", w(hid, inter + 8)), ("w_down", w(8, inter)), ("w_gate_up", w(95, hid))):
+        with pytest.raises(ops.NsaError, match=name):
+            call(mlp={**mlp, name: W})
+    q4 = ops.Weight4(torch.zeros((4, 1, 16, 64), dtype=torch.uint8), torch.zeros((4, 1, 16, 4), dtype=bf), hid, 40, 32)
+    with pytest.raises(ops.NsaError, match="w_down"):
+        call(mlp={**mlp, "w_down": q4})
+    for kw in (dict(buffers=make(1, 2, dev="meta")), dict(attn={**attn, "in_norm": torch.ones(hid, device="meta")})):
+        with pytest.raises(ops.NsaError, match="x's device"):
+            call(**kw)
+    with pytest.raises(ops.NsaError, match="CUDA"):   # the sizes are right: on to the calls
+        call(buffers=good)
