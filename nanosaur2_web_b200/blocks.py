@@ -508,6 +508,8 @@ def gemma_layer_decode(x: torch.Tensor, *, attn: dict, mlp: dict, cs: RopeTable,
         raise NsaError(_lib.NSA_ERR_INVALID_ARGUMENT, "h_ready needs the buffers that hold h")
     B, L, hidden = x.shape
     inter = _check_decode(x, attn, mlp, buffers, next_norm)
+    if not x.numel():
+        return x
     buf = buffers if buffers is not None else gemma_decode_buffers(B, L, hidden, inter, x.device)
     xs = x.view(B * L, hidden)
     if not h_ready:

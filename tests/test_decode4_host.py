@@ -257,3 +257,18 @@ def test_gemma_layer_decode_refuses_buffers_and_weights_of_other_sizes():
             call(**kw)
     with pytest.raises(ops.NsaError, match="CUDA"):   # the sizes are right: on to the calls
         call(buffers=good)
+
+
+@pytest.mark.parametrize("B,L", [(0, 1), (0, 3), (2, 0), (0, 0)])
+def test_gemma_layer_decode_of_no_sequences_or_no_tokens(B, L):
+    from nanosaur2_web_b200 import blocks
+    bf, hid, inter = torch.bfloat16, 64, 48
+    w = lambda *s: torch.zeros(s, dtype=bf)
+    one = torch.ones(hid)
+    attn = dict(in_norm=one, w_qkv=w(1536, hid), q_norm=torch.ones(256), k_norm=torch.ones(256), w_o=w(hid, 1024), post_norm=one)
+    mlp = dict(pre_norm=one, w_gate_up=w(2 * inter, hid), w_down=w(hid, inter), post_norm=one)
+    cache = ops.Kv4Cache(torch.zeros((2, 2, 1, 16, 128), dtype=torch.uint8), w(2, 2, 1, 16, 8))
+    x = torch.zeros((B, L, hid))
+    for buffers in (None, blocks.gemma_decode_buffers(B, L, hid, inter, "cpu")):
+        assert blocks.gemma_layer_decode(x, attn=attn, mlp=mlp, cs=None, cache=cache, table=torch.zeros((B, 2), dtype=torch.int32),
+                                         start=torch.zeros(B, dtype=torch.int32), buffers=buffers) is x
