@@ -210,9 +210,9 @@ Tensor kv4_append(const Tensor& qkv, const Tensor& codes, const Tensor& scales, 
   for (const Tensor* w : {&q_norm, &k_norm})
     if (w->scalar_type() != at::kFloat || w->sizes() != at::IntArrayRef({D}) || !w->is_contiguous())
       invalid("q_norm and k_norm must be contiguous float32 [" + std::to_string(D) + "] tensors");
-  if (cs && (cs_D != D || cs->scalar_type() != at::kFloat || !cs->is_contiguous() || sin_off < 0 || cs_rows < 0 ||
+  if (cs && (cs_D != D || cs->scalar_type() != at::kFloat || !cs->is_contiguous() || sin_off < 0 || cs_rows < 1 ||
              cs_rows > cs->numel() || cs_rows * (D / 2) > cs->numel() - sin_off))
-    invalid("cs must be a float32 table of head dim " + std::to_string(D));
+    invalid("cs must be a float32 table of one row or more of head dim " + std::to_string(D));
   OnDevice on(dev);
   const Tensor out = out_ ? *out_ : at::empty({x.B, x.L, Hq * D}, qkv.options().dtype(at::kBFloat16));
   const Rows o = result_rows(out, "out", x.B, x.L, Hq * D);

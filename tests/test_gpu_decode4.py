@@ -893,3 +893,14 @@ def test_kv4_attention_of_the_largest_values(D, group, L, T):
         check_device()
         want, tol = attend_oracle(cd, n64(q), [T - L], [L], 0, 0, 1 / np.sqrt(D))
         assert (np.abs(got - want) <= tol).all(), (size, float(np.abs(got / want - 1).max()))
+
+
+def test_append_refuses_an_empty_rope_table():
+    """Without rows the table's pointer is null, which the C call takes as no rotation."""
+    from nanosaur2_web_b200 import ops
+    c = ops.kv4_cache(2, 1, 64, 16, DEV)
+    table, start, w = t([[0, 1]], torch.int32), t([0], torch.int32), torch.ones(64, device=DEV)
+    x = torch.zeros((1, 1, 3 * 64), device=DEV)
+    none = ops.RopeTable(torch.empty(0, device=DEV), 0, 0, 64)
+    with pytest.raises(ops.NsaError, match="head dim"):
+        ops.kv4_append(x, c, table, start, Hq=1, q_norm=w, k_norm=w, cs=none)
