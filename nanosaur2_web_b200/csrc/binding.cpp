@@ -270,6 +270,7 @@ Tensor kv4_attention(const Tensor& q, const Tensor& codes, const Tensor& scales,
   d.window = int32_of(window, "window");
   d.sinks = int32_of(sinks, "sinks");
   d.scale = (float)scale;
+  if (scale != 0 && d.scale == 0.f) invalid("scale is 0 in fp32");
   OptTensor workspace = workspace_;
   if (!workspace) {
     const size_t need = nsa_kv4_attention_workspace_size(&d, &c, &b);

@@ -904,3 +904,16 @@ def test_append_refuses_an_empty_rope_table():
     none = ops.RopeTable(torch.empty(0, device=DEV), 0, 0, 64)
     with pytest.raises(ops.NsaError, match="head dim"):
         ops.kv4_append(x, c, table, start, Hq=1, q_norm=w, k_norm=w, cs=none)
+
+
+def test_attention_refuses_a_scale_that_underflows():
+    """A scale that is 0 in fp32 would be taken as the default, 1 / sqrt(D)."""
+    from nanosaur2_web_b200 import ops
+    c = ops.kv4_cache(2, 1, 64, 16, DEV)
+    c.codes.fill_(0x9A)
+    c.scales.fill_(1.0)
+    table, start, q = t([[0, 1]], torch.int32), t([5], torch.int32), torch.ones((1, 1, 64), dtype=BF, device=DEV)
+    with pytest.raises(ops.NsaError, match="scale"):
+        ops.kv4_attention(q, c, table, start, scale=1e-46)
+    ops.kv4_attention(q, c, table, start, scale=1e-44)
+    check_device()
