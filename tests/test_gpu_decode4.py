@@ -917,3 +917,29 @@ def test_attention_refuses_a_scale_that_underflows():
         ops.kv4_attention(q, c, table, start, scale=1e-46)
     ops.kv4_attention(q, c, table, start, scale=1e-44)
     check_device()
+
+
+def test_kv4_attention_repeats_itself_whatever_the_workspace_held():
+    """The same bits from every call, also over a workspace full of NaN, of ones, and of another call's sums."""
+    from nanosaur2_web_b200 import ops
+    rng = np.random.default_rng(40)
+    for B, L, Hq, Hkv, D, P, T in ((40, 1, 32, 8, 128, 64, 1100), (1, 4, 32, 8, 128, 128, 20000)):
+        mp = -(-T // P)
+        cache = ops.kv4_cache(B * mp, Hkv, D, P, DEV)
+        cache.codes.copy_(torch.randint(0, 256, cache.codes.shape, device=DEV, dtype=torch.uint8) | 0x11)
+        cache.scales.copy_(torch.randint(16, 32, cache.scales.shape, device=DEV) / 64)
+        table = t(rng.permutation(B * mp).reshape(B, mp), torch.int32)
+        start = t([max(0, T - L - 17 * b) for b in range(B)], torch.int32)
+        q, q2 = (torch.randn((B, L, Hq * D), device=DEV).to(BF) for _ in range(2))
+        want = ops.kv4_attention(q, cache, table, start)
+        ws = torch.empty(1 << 26, dtype=torch.uint8, device=DEV)
+        for i in range(12):
+            if i % 4 == 0:
+                ws.fill_(0xFF)
+            elif i % 4 == 1:
+                ws.fill_(0)
+                ws.view(torch.float32).fill_(1.0)
+            elif i % 4 == 2:
+                ops.kv4_attention(q2, cache, table, start, workspace=ws)
+            assert torch.equal(ops.kv4_attention(q, cache, table, start, workspace=ws), want), i
+    check_device()
