@@ -1011,7 +1011,7 @@ cudaError_t launch_append_t(const Kv4AppendParams& p, unsigned rows, cudaStream_
   const int slots = (p.Hq + hpw - 1) / hpw + 2 * ((p.kv.Hkv + hpw - 1) / hpw);
   // with many tokens, fewer warps share a token's set-up (heads 32 + 2 x 8 of 128, 4 and 8 warps: 1 token 5.1 and 4.0 us,
   // 2048 tokens 19.0 and 18.4 us, 8000 tokens 49.8 and 55.9 us)
-  const int threads = 32 * std::min(slots, rows >= 8 * 148 ? 4 : 8);
+  const int threads = 32 * std::min(slots, rows >= 8u * device_sm_count() ? 4 : 8);
   switch (p.kv.D) {
     case 64: kv4_append_kernel<T, 64><<<rows, threads, 0, stream>>>(p); break;
     case 128: kv4_append_kernel<T, 128><<<rows, threads, 0, stream>>>(p); break;
@@ -1034,7 +1034,7 @@ cudaError_t launch_kv4_read(const Kv4Params& p, __nv_bfloat16* out, int64_t ldo,
   const int64_t rows = (int64_t)p.B * p.L;
   if (rows > 0x7FFFFFFFLL) return cudaErrorInvalidValue;
   const int threads = std::min(256, (2 * p.Hkv * (p.D / 8) + 31) / 32 * 32);
-  if (rows >= 8 * 148)   // one and two rows per CTA, 8 heads of 128: 1024 rows 3.4 and 3.7 us, 2048 5.2 and 4.9, 8000 17.2 and 15.3
+  if (rows >= 8 * device_sm_count())   // one and two rows per CTA, 8 heads of 128: 1024 rows 3.4 and 3.7 us, 2048 5.2 and 4.9, 8000 17.2 and 15.3
     kv4_read_kernel<2><<<(unsigned)((rows + 1) / 2), threads, 0, stream>>>(p, out, ldo, bstride);
   else
     kv4_read_kernel<1><<<(unsigned)rows, threads, 0, stream>>>(p, out, ldo, bstride);
@@ -1061,7 +1061,7 @@ void kv4_attention_plan(Kv4AttnParams* p) {
   int bits = 4;   // 2^bits tokens at least that a row may see
   while ((int64_t)1 << bits < seen * 16) ++bits;
   p->shift = bits + 1.f;
-  const int wave = 148 * ctas_per_sm(kv.D, p->row_nt);
+  const int wave = device_sm_count() * ctas_per_sm(kv.D, p->row_nt);
   p->cluster = units * kCluster <= wave && seen <= kCluster * kAttnWarps * 8;
   const int64_t most = (units * std::max<int64_t>(seen, 1) + kAttnWarps - 1) / kAttnWarps;
   p->ctas = p->cluster ? (int)units * kCluster : (int)std::min<int64_t>(most, wave);
