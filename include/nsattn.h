@@ -456,8 +456,10 @@ nsa_status nsa_expand4(const nsa_weight4* w, void* out, int64_t ldo, void* strea
  *   C[m*ldc + n] = r, or += r with resid, where r = sum_k A[m][k] W[n][k] (+ bias[n]).
  * A bf16 [M][lda]; K and lda multiples of 8, A 16-byte aligned; C fp32 or (store form) bf16, at its element
  * alignment; C must not overlap A.  K up to 98304; above 49152, N up to 524288 (NSA_ERR_UNSUPPORTED beyond).  The products are exact and sums are kept in fp32, so the result
- * is the fp32 linear's.  Any M runs; the weights are read once per 32 rows of A (fewer where 32 rows of K do not
- * fit shared memory), so for hundreds of rows nsa_linear over the nsa_expand4 copy is faster. */
+ * is the fp32 linear's.  Any M runs; the weights are read once per 32 rows of A, or per fewer (16 at 16384 x 8192, 11
+ * at 8192 x 28672) where shared memory does not hold 32 rows of K, or of the sums of N.  nsa_linear over the
+ * nsa_expand4 copy takes about as long for 256 rows as for one; measured, it is the faster one from M = 64 at
+ * 8200 x 4096, 128 at 4096 x 640 and 512 at 640 x 1024. */
 typedef struct nsa_linear4_desc {
   int32_t M;
   int64_t lda;           /* A row pitch in elements (0: K) */
@@ -526,7 +528,8 @@ nsa_status nsa_kv4_read(const nsa_kv4_cache* cache, const nsa_kv4_batch* batch, 
  * holds the new tokens already.  The query at position p sees keys j <= p; with window > 0, only those with
  * j > p - window (nsa_attention's window) or j < sinks.  q and out bf16, head h of row (b, i) at
  * b*bstride + i*ld + h*D; bases 16-byte aligned, pitches multiples of 8.  out must not overlap q.  A query
- * with no key left (its pages or position invalid) writes zeros. */
+ * with no key left (its pages or position invalid) writes zeros.  Scores, sums of q k and their product with scale times
+ * log2 e, are fp32: they have to stay within its range. */
 typedef struct nsa_kv4_attention_desc {
   int32_t Hq;            /* a multiple of Hkv; query heads h*Hq/Hkv .. share key/value head h */
   int64_t q_ld, q_bstride;

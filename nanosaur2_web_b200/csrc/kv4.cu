@@ -165,10 +165,12 @@ __device__ __forceinline__ bool quantise_keys(const float* x, const Turn& t, flo
   return sure;
 }
 
-// A CTA per token; a warp takes 256 / D heads of one kind (q, k or v) at a time, eight values a lane.  Instructions bound it
-// rather than the bytes of q | k | v: unpacking, norms and codes of a value cost about ten.  16 x 500 tokens of 32 + 2 x 8
-// heads of 128: 49.7 us from bf16 (3.5 TB/s), 52.8 us from fp32 (5.1 TB/s).  Six CTAs of eight warps fit an SM; loading
-// the next head ahead cost registers for that and was slower (72.8 against 64.8 us when it was tried).
+// A CTA per token; a warp takes 256 / D heads of one kind (q, k or v) at a time, eight values a lane.  16 x 500 tokens of
+// 32 + 2 x 8 heads of 128: 49.7 us from bf16 (3.5 TB/s), 52.8 us from fp32 (5.1 TB/s).  From bf16 it is half issue and half
+// latency: 27 warp instructions per 32 values take 74% of the issue slots, and the longest stall is the wait for a head's
+// loads (5.3 of the 13.6 cycles between a warp's instructions).  The launch bound, eight warps in each of six CTAs, holds it
+// to 40 registers with 20 to 24 bytes spilled; long calls run four warps a CTA and would not need it.  Loading the next head
+// ahead under that bound was slower (72.8 against 64.8 us on an earlier form).
 template <typename T, int D>
 __global__ void __launch_bounds__(256, 6) kv4_append_kernel(const Kv4AppendParams p) {
   constexpr int LANES = D / 8, HPW = 32 / LANES, half = D / 2;
@@ -252,8 +254,9 @@ __global__ void __launch_bounds__(256, 6) kv4_append_kernel(const Kv4AppendParam
   }
 }
 
-// A CTA per R rows, a thread per word (8 values) of each: the rows' loads are under way together.  Bound by the latency of
-// table, codes and stores in turn: 16 x 500 tokens of 8 heads of 128 in 15.3 us (2.7 TB/s).
+// A CTA per R rows, a thread per word (8 values) of each: the rows' loads are under way together.  16 x 500 tokens of 8 heads
+// of 128 take 15.3 us (2.7 TB/s): a chain of start, table, codes and stores for little work per thread (72% of the issue
+// slots, 4.0 of 18.5 cycles per instruction waiting for loads).
 template <int R>
 __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4Params p, __nv_bfloat16* __restrict__ out, int64_t ldo,
                                                        int64_t bstride) {
@@ -306,7 +309,7 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4Params p, __nv_b
 // on the end of one unit, some whole ones and the beginning of another.  Within a CTA each warp walks its own blocks
 // with its own running maximum, sum and output, joined in shared memory; what CTAs have of a shared unit is joined
 // by a second kernel.  Few and short units are latency instead: a cluster of eight CTAs takes one unit and joins it
-// through its shared memories.
+// through its shared memories.  The host chooses, and by what it knows: the page table's width, not the sequences' lengths.
 //
 // Both products run on mma.m16n8k16 with the cached operand as A, so that the eight query rows fill N = 8 and
 // only the cache's bytes are converted:
@@ -327,9 +330,9 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4Params p, __nv_b
 // terms are what they multiply the values with, so that one product does for both.
 //
 // What bounds it is the issue of instructions: an mma.m16n8k16 holds a scheduler for about 5 cycles (and its tensor unit
-// for 8), a pair of converted values costs 3 instructions, two of them at half rate.  With the copies taken out, 8192
-// blocks of 8 heads for 16 rows (D 128) take the time that they take with them; without the products and conversions,
-// 40 us of 64.  Two blocks at a time give the scheduler independent chains (D 256: 33.2 -> 29.7 us at 8 x 32768 tokens)
+// for 8), a pair of converted values costs 3 instructions, two of them at half rate.  On a form that took 71.9 us for 8192
+// blocks of 8 heads and 16 rows (D 128; 63.5 us now), 71.2 without the copies and 39.8 without the products and
+// conversions.  Two blocks at a time give the scheduler independent chains (D 256: 33.2 -> 29.7 us at 8 x 32768 tokens)
 // and share the walk, the tests of masks and maxima (466 instead of 594 instructions a block).
 // The running maximum moves only when a score exceeds it by 2^8 in the exponent's base, which spares a reduction over
 // lanes per block.  What is subtracted from the scores is the maximum and `shift` more, ceil(log2(tokens a row may see))
@@ -1044,8 +1047,10 @@ cudaError_t launch_kv4_read(const Kv4Params& p, __nv_bfloat16* out, int64_t ldo,
 constexpr int kCluster = 8;
 
 // Row tiles (two tiles of eight rows at a time share the converted operand where there are more than eight rows), and the
-// CTAs: a cluster per unit where these fit one wave and no unit is longer than eight blocks per warp, else one wave, but
-// at least a block of 16 tokens for each warp of the longest sequences.  Measured in us, 4 query heads per kv head:
+// CTAs: a cluster per unit where these fit one wave and no unit can be longer than eight blocks per warp (4096 tokens, by the
+// page table's width or the window: lengths are on the device), else one wave, but at least a block of 16 tokens for each
+// warp of the longest sequences.  Short sequences in a wide table therefore take the wave: 1024 tokens of D 256 in a table of
+// 8192 10.4 us, in one of 1024 7.8.  Measured in us, 4 query heads per kv head:
 //   cluster / wave            1 sequence of 1024: 7.5 / 9.8 (D 256), 6.3 / 8.4 (D 128);  16384: 27.2 / 29.7, 19.5 / 18.5;
 //                             16 of 4096: 15.2 / 15.0, 11.2 / 12.6
 //   16 rows, two tiles / one  2 x 32768 tokens, 8 kv heads of 128: 39.0 / 47.9;  12 rows: 37.7 / 47.4

@@ -51,8 +51,9 @@ __device__ __forceinline__ void load8(const __nv_bfloat16* row, int k, int K, fl
 }
 
 // One CTA per tile chunk, one thread per word (8 values of one row); the 4, 8 or 16 neighbouring threads of a group
-// share its largest magnitude by shuffles.  fp32 weights are bound by their bytes, bf16 ones by the instructions of two
-// roundings per value: 8192 x 8200 in groups of 64 takes 55.1 us (5.5 TB/s) from fp32, 61.5 us (2.8 TB/s) from bf16.
+// share its largest magnitude by shuffles.  8192 x 8200 in groups of 64 takes 55.1 us (5.5 TB/s) from fp32, where the bytes
+// bound it, and 61.5 us (2.8 TB/s) from bf16: there 24 warp instructions per 32 values, two roundings each, take 75% of the
+// issue slots, and one load a thread leaves 5.6 of 17 cycles per instruction waiting for it.
 template <typename T, int G, bool VEC>
 __global__ void __launch_bounds__(256) quantize4_kernel(const Quant4Params p) {
   const int tile = blockIdx.x / p.Kc, ch = blockIdx.x % p.Kc;
@@ -78,7 +79,8 @@ __global__ void __launch_bounds__(256) quantize4_kernel(const Quant4Params p) {
 }
 
 // The same shape backwards: a thread per word, one 16-byte store where the rows of out are 16-byte aligned.  8192 x 8200:
-// 43.4 us (3.9 TB/s; a row's tile chunk is 256 contiguous bytes of out, which the stores' latency does not hide better).
+// 43.4 us (3.9 TB/s).  One load and one store a thread in short CTAs: 71% of the issue slots, and half of the cycles between
+// a warp's instructions waiting for loads (8.7 of 17); more words a thread would be the next step.
 template <bool VEC>
 __global__ void __launch_bounds__(256) expand4_kernel(const Quant4Params p, __nv_bfloat16* __restrict__ out, int64_t ldo) {
   const int tile = blockIdx.x / p.Kc, ch = blockIdx.x % p.Kc;
@@ -124,7 +126,8 @@ __global__ void __launch_bounds__(256) expand4_kernel(const Quant4Params p, __nv
 // cost more than the weights, so a cluster of CS CTAs shares K: each stages its part of X, goes over the cluster's
 // tiles with it, and the parts of the sums are joined through the shared memories at the end.
 //
-// One row of 16384 x 8192 (group 128) takes 19.5 us (3.6 TB/s); with the products left out the same copies take 14.9 us.
+// One row of 16384 x 8192 (group 128) takes 19.4 us (3.6 TB/s; the floor is 10.7); with the products left out the same
+// copies take 14.9 us.  (The alternatives below and in linear4_plan were timed beside a form that took 19.0.)
 // The rest is instructions: a chunk is 96 of them to convert and 8 products, each of which holds its scheduler for about 5
 // cycles.  24 rows of 8200 x 4096 take 15.4 us, 9.4 without the products.  A call of a few hundred kilobytes is its launch
 // and one trip to memory: 640 x 1024 in 3.1 us.  Two CTAs per SM with half the registers: 20.7 us instead of 19.0 at

@@ -464,8 +464,8 @@ def linear4(x: torch.Tensor, W: Weight4, *, bias: Optional[torch.Tensor] = None,
     """``linear`` with a 4-bit weight, for the few rows of a decode step (nsa_linear4): out = x @ W^T (+ bias),
     or out += with ``resid``.  x [M, K] bf16 (K and the row pitch multiples of 8); bias float32 [N]; out [M, N]
     float32 or (store form) bfloat16 with unit inner stride, allocated (``out_dtype``, default float32) when not
-    given.  Products are exact and sums in fp32.  Any M runs; the weight is read once per 32 rows, so for
-    hundreds of rows ``linear`` over ``expand4(W)`` is faster."""
+    given.  Products are exact and sums in fp32.  Any M runs, for few rows: the weight is read once per 32 rows or
+    fewer, and ``linear`` over ``expand4(W)`` is faster from 64 rows (8200 x 4096) to 512 (640 x 1024)."""
     return _native().linear4(x, W.codes, W.scales, W.N, W.K, W.group, bias, out, resid, out_dtype)
 
 
@@ -538,8 +538,8 @@ def kv4_attention(q: torch.Tensor, cache: Kv4Cache, table: torch.Tensor, start: 
     (nsa_kv4_attention).  q bf16 [B, L, Hq*D] (``kv4_append``'s result), query heads h*Hq/Hkv .. sharing key/value
     head h; the query at position p = start[b] + i sees keys j <= p, with ``window`` > 0 only those with
     j > p - window or j < ``sinks``.  Returns bf16 [B, L, Hq*D] (``out``); rows past count[b] are left as they
-    were (``out`` not given: uninitialised), rows at positions outside are zeros.  scale 0 means 1/sqrt(D).  ``workspace``: a uint8 tensor to
-    reuse, as large as the C call asks (nsa_kv4_attention_workspace_size; the error names the size), allocated per
+    were (``out`` not given: uninitialised), rows at positions outside are zeros.  scale 0 means 1/sqrt(D).
+    ``workspace``: a uint8 tensor to reuse, as large as the C call asks (nsa_kv4_attention_workspace_size; the error names the size), allocated per
     call when not given; calls that overlap on the GPU need one each."""
     return _native().kv4_attention(q, cache.codes, cache.scales, cache.positions, table, start, count, window, sinks, scale, out,
                                    workspace)
