@@ -469,14 +469,18 @@ def linear4(x: torch.Tensor, W: Weight4, *, bias: Optional[torch.Tensor] = None,
     return _native().linear4(x, W.codes, W.scales, W.N, W.K, W.group, bias, out, resid, out_dtype)
 
 
+_NO_LIMIT = 2 ** 31 - 1
+
+
 @dataclass
 class Kv4Cache:
     """A pool of pages of keys and values in 4 bits: ``codes`` uint8 [n_pages, 2, Hkv, P, D/2] and ``scales``
     bf16 [n_pages, 2, Hkv, P, D/32] in the order of include/nsattn.h (nsa_kv4_cache).  Which page holds which
     tokens is the caller's page table: int32 [B, max_pages], position t of sequence b in slot t % P of page
     table[b, t // P].  ``positions`` (0: as many as the page table spans): tokens from this position on are outside, like
-    those past the page table.  ``kv4_append`` stores no token past its RoPE table and sets this to the table's rows (0 without
-    one), so that the calls that read the cache leave the same tokens out; another handle on the same memory is given it."""
+    those past the page table.  ``kv4_append`` stores no token past its RoPE table and leaves the table's rows here (of tables
+    of several lengths the longest; without one there is no limit), so that the calls that read the cache leave the same
+    tokens out; another handle on the same memory is given it."""
     codes: torch.Tensor
     scales: torch.Tensor
     positions: int = 0
@@ -519,7 +523,7 @@ def kv4_append(qkv: torch.Tensor, cache: Kv4Cache, table: torch.Tensor, start: t
     buf, rows, dim, sin_off = (None, 0, 0, 0) if cs is None else (cs.buf, cs.L, cs.D, cs.sinOff)
     out = _native().kv4_append(qkv, cache.codes, cache.scales, table, start, count, Hq, q_norm, k_norm, buf, rows, dim,
                                sin_off, eps, qOff, kOff, vOff, out)
-    cache.positions = 0 if cs is None else cs.L
+    cache.positions = max(cache.positions, _NO_LIMIT if cs is None else cs.L)
     return out
 
 

@@ -943,3 +943,26 @@ def test_kv4_attention_repeats_itself_whatever_the_workspace_held():
                 ops.kv4_attention(q2, cache, table, start, workspace=ws)
             assert torch.equal(ops.kv4_attention(q, cache, table, start, workspace=ws), want), i
     check_device()
+
+
+def test_kv4_appends_with_rope_tables_of_several_lengths():
+    """Sequences that enter with tables of their own lengths: a shorter table later does not hide the tokens of a longer one, nor
+    one append without rotation any."""
+    from nanosaur2_web_b200 import ops
+    rng = np.random.default_rng(32)
+    Hq, Hkv, D, P = 2, 1, 64, 16
+    cache = ops.kv4_cache(8, Hkv, D, P, DEV)
+    table, w = t([[0, 1, 2, 3], [4, 5, 6, 7]], torch.int32), torch.ones(D, device=DEV)
+    for lengths in ((50, 20), (20, 50), (50, None), (20, None)):
+        cache.positions = 0
+        for b, rows in enumerate(lengths):
+            n = rows or 50
+            x = t(rng.standard_normal((1, n, (Hq + 2 * Hkv) * D)))
+            ops.kv4_append(x, cache, table[b:b + 1], t([0], torch.int32), Hq=Hq, q_norm=w, k_norm=w,
+                           cs=None if rows is None else ops.ropeTable(rows, D, 1e4, DEV))
+        start = t([n - 1 for n in (lengths[0], lengths[1] or 50)], torch.int32)
+        q = t(rng.standard_normal((2, 1, Hq * D)), BF)
+        got = ops.kv4_attention(q, cache, table, start)
+        check_device()
+        assert torch.equal(got, ops.kv4_attention(q, ops.Kv4Cache(cache.codes, cache.scales), table, start)) and (got != 0).any(-1).all()
+    check_device()
